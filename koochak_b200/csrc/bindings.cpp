@@ -17,6 +17,8 @@ void register_attention_ops(pybind11::module& m);
 void register_optim_ops(pybind11::module& m);
 void register_comm_ops(pybind11::module& m);
 void register_muon_gather_ops(pybind11::module& m);
+void register_token_logprobs_ops(pybind11::module& m);
+void register_topk_distillation_ops(pybind11::module& m);
 }  // namespace kb
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -64,4 +66,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   kb::register_optim_ops(m);
   kb::register_comm_ops(m);
   kb::register_muon_gather_ops(m);
+  kb::register_token_logprobs_ops(m);
+  kb::register_topk_distillation_ops(m);
 }

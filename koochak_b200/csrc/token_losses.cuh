@@ -1,0 +1,397 @@
+// Device and host pieces shared by the per-token losses over a vocabulary
+// (token_logprobs.cu, topk_distillation.cu).
+//
+// Notation: z is a row of V logits, c = log2(e) / T, m = max z,
+// S = sum_j 2^((z_j - m) c), so p_j = 2^((z_j - m) c) / S is softmax(z / T)
+// and ln p_j = ln 2 ((z_j - m) c - log2 S). Differences to the maximum are
+// taken before the scaling: they are exact for near values, and a row whose
+// entries all are the type's lowest value is a uniform one instead of an
+// overflow. A row of -inf only has no distribution and gives NaN.
+//
+// Statistics are held in fp32 per thread (maximum, sum, and for the entropy
+// A = sum 2^x x with x = (z_j - m) c), rescaled when the thread's maximum
+// grows, and joined in a fixed order, so results do not depend on timing.
+#pragma once
+
+#include <ATen/ATen.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cmath>
+
+#include "host_utils.h"
+
+namespace kb {
+namespace {  // per translation unit: each source compiles its own kernels from these
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMaxList = 128;  // alternatives, or teacher slots, per row
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<__nv_bfloat16> {
+  static constexpr int kUnit = 8;
+  static constexpr uint32_t kNegInf = 0xFF80FF80u;
+  static __device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&v)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // Largest of the unit's elements; NaN when there is one.
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  static __device__ __forceinline__ float widen_max(uint32_t w) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(__uint_as_float(w << 16)), "f"(__uint_as_float(w & 0xFFFF0000u)));
+    return d;
+  }
+};
+template <>
+struct Elem<__half> {
+  static constexpr int kUnit = 8;
+  static constexpr uint32_t kNegInf = 0xFC00FC00u;
+  static __device__ __forceinline__ float load(const __half* p) { return __half2float(*p); }
+  static __device__ __forceinline__ void store(__half* p, float v) { *p = __float2half_rn(v); }
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&v)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  static __device__ __forceinline__ float widen_max(uint32_t w) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(f.x), "f"(f.y));
+    return d;
+  }
+};
+template <>
+struct Elem<float> {
+  static constexpr int kUnit = 4;
+  static constexpr uint32_t kNegInf = 0xFF800000u;
+  static __device__ __forceinline__ float load(const float* p) { return *p; }
+  static __device__ __forceinline__ void store(float* p, float v) { *p = v; }
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&v)[4]) {
+    v[0] = __uint_as_float(q.x);
+    v[1] = __uint_as_float(q.y);
+    v[2] = __uint_as_float(q.z);
+    v[3] = __uint_as_float(q.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&v)[4]) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
+    return __float_as_uint(d);
+  }
+  static __device__ __forceinline__ float widen_max(uint32_t w) { return __uint_as_float(w); }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// A row cut for 16-byte access: `head` elements before the first 16-byte
+// boundary, `units` whole units, the rest behind them. The (fewer than two
+// units of) elements outside whole units are the row's ragged ones.
+template <typename T>
+struct Row {
+  const T* z;
+  int head, units, ragged;
+  __device__ __forceinline__ Row(const T* p, int V) : z(p) {
+    constexpr int E = Elem<T>::kUnit;
+    const int to_boundary = (int)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T));
+    head = min(V, to_boundary);
+    units = (V - head) / E;
+    ragged = V - units * E;
+  }
+  __device__ __forceinline__ const uint4* unit_ptr() const { return reinterpret_cast<const uint4*>(z + head); }
+  __device__ __forceinline__ int ragged_index(int i) const {
+    return i < head ? i : units * Elem<T>::kUnit + i;
+  }
+};
+
+// Running statistics of the elements a thread has seen.
+struct Acc {
+  float m = -INFINITY, s = 0.f, a = 0.f;
+  // Takes the maximum up to `mx` and returns the finite value to subtract.
+  template <bool ENT>
+  __device__ __forceinline__ float raise(float mx, float c) {
+    const float mn = max_nan(m, mx);
+    const float x = (m - mn) * c;
+    const float f = (m == mn) ? 1.f : ex2(x);
+    if (ENT) a = f * (a + s * fmaxf(x, -1e30f));  // s is 0 where x is -inf
+    s *= f;
+    m = mn;
+    return mn == -INFINITY ? 0.f : mn;
+  }
+  template <bool ENT>
+  __device__ __forceinline__ void add(float z, float ms, float c) {
+    const float x = (z - ms) * c;
+    const float e = ex2(x);
+    s += e;
+    if (ENT) a = fmaf(e, fmaxf(x, -256.f), a);  // 2^-256 is 0: a masked entry adds 0, not 0 * inf
+  }
+  // Joins another thread's statistics.
+  template <bool ENT>
+  __device__ __forceinline__ void join(float m2, float s2, float a2, float c) {
+    const float mn = max_nan(m, m2);
+    const float x1 = (m - mn) * c, x2 = (m2 - mn) * c;
+    const float f1 = (m == mn) ? 1.f : ex2(x1), f2 = (m2 == mn) ? 1.f : ex2(x2);
+    if (ENT) {
+      const float y1 = (m == mn) ? 0.f : fmaxf(x1, -1e30f), y2 = (m2 == mn) ? 0.f : fmaxf(x2, -1e30f);
+      a = f1 * (a + s * y1) + f2 * (a2 + s2 * y2);
+    }
+    s = s * f1 + s2 * f2;
+    m = mn;
+  }
+};
+
+__device__ __forceinline__ uint4 load_unit(const uint4* p) {
+  uint4 q;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+               : "l"(p));
+  return q;
+}
+
+// Masks the elements of unit `u` whose bit is set (bit = u * E + j).
+template <typename T>
+__device__ __forceinline__ void mask_unit(uint4& q, const uint8_t* bits, int u) {
+  constexpr int E = Elem<T>::kUnit;
+  uint32_t b = E == 8 ? bits[u] : (bits[u >> 1] >> ((u & 1) * 4)) & 15u;
+  if (b == 0) return;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&q);
+  if (E == 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = (b >> (2 * i)) & 1u, hi = (b >> (2 * i + 1)) & 1u;
+      const uint32_t keep = (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
+      w[i] = (w[i] & keep) | (Elem<T>::kNegInf & ~keep);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if ((b >> i) & 1u) w[i] = Elem<T>::kNegInf;
+  }
+}
+
+// Statistics of the units [u0, u1) of a row over the threads of a block,
+// four 16-byte loads in flight per thread.
+template <typename T, int NT, bool ENT, bool MASK>
+__device__ __forceinline__ void stream_units(const uint4* p, int u0, int u1, float c, Acc& acc, const uint8_t* bits) {
+  constexpr int UN = 4, E = Elem<T>::kUnit;
+  for (int u = u0 + (int)threadIdx.x; u < u1; u += UN * NT) {
+    uint4 q[UN];
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      if (u + i * NT < u1) {
+        q[i] = load_unit(p + u + i * NT);
+      } else {
+        q[i] = make_uint4(Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf);
+      }
+    }
+    if (MASK) {
+#pragma unroll
+      for (int i = 0; i < UN; ++i)
+        if (u + i * NT < u1) mask_unit<T>(q[i], bits, u + i * NT - u0);
+    }
+    uint32_t mx = Elem<T>::max2(Elem<T>::max2(q[0].x, q[0].y), Elem<T>::max2(q[0].z, q[0].w));
+#pragma unroll
+    for (int i = 1; i < UN; ++i)
+      mx = Elem<T>::max2(mx, Elem<T>::max2(Elem<T>::max2(q[i].x, q[i].y), Elem<T>::max2(q[i].z, q[i].w)));
+    const float ms = acc.raise<ENT>(Elem<T>::widen_max(mx), c);
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      if (u + i * NT < u1) {
+        float v[E];
+        Elem<T>::unpack(q[i], v);
+#pragma unroll
+        for (int j = 0; j < E; ++j) acc.add<ENT>(v[j], ms, c);
+      }
+    }
+  }
+}
+
+// Joins the statistics of a block's threads; every thread returns with them.
+template <int NT, bool ENT>
+__device__ __forceinline__ Acc block_join(Acc acc, float c, float (*sm)[3]) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, acc.m, o);
+    const float s2 = __shfl_xor_sync(0xffffffffu, acc.s, o);
+    const float a2 = ENT ? __shfl_xor_sync(0xffffffffu, acc.a, o) : 0.f;
+    acc.join<ENT>(m2, s2, a2, c);
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) {
+    sm[warp][0] = acc.m;
+    sm[warp][1] = acc.s;
+    sm[warp][2] = acc.a;
+  }
+  __syncthreads();
+  constexpr int NW = NT / 32;
+  Acc r;
+  const int w = lane & (NW - 1);
+  r.m = sm[w][0];
+  r.s = sm[w][1];
+  r.a = sm[w][2];
+#pragma unroll
+  for (int o = NW / 2; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, r.m, o);
+    const float s2 = __shfl_xor_sync(0xffffffffu, r.s, o);
+    const float a2 = ENT ? __shfl_xor_sync(0xffffffffu, r.a, o) : 0.f;
+    r.join<ENT>(m2, s2, a2, c);
+  }
+  return r;
+}
+
+// Writes a row's units [u0, u1) and, for the first segment, its ragged elements: out = f(z, index).
+template <typename T, int NT, typename F>
+__device__ __forceinline__ void map_row(const Row<T>& row, T* out, int u0, int u1, int ragged, const F& f) {
+  constexpr int UN = 4, E = Elem<T>::kUnit;
+  const bool same = ((reinterpret_cast<uintptr_t>(row.z) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  if ((int)threadIdx.x < ragged) {
+    const int idx = row.ragged_index(threadIdx.x);
+    Elem<T>::store(out + idx, f(Elem<T>::load(row.z + idx), idx));
+  }
+  const uint4* p = row.unit_ptr();
+  for (int u = u0 + (int)threadIdx.x; u < u1; u += UN * NT) {
+    uint4 q[UN];
+#pragma unroll
+    for (int i = 0; i < UN; ++i)
+      if (u + i * NT < u1) q[i] = load_unit(p + u + i * NT);
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      if (u + i * NT < u1) {
+        const int idx = row.head + (u + i * NT) * E;
+        float v[E];
+        Elem<T>::unpack(q[i], v);
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = f(v[j], idx + j);
+        if (same) {
+          *reinterpret_cast<uint4*>(out + idx) = Elem<T>::pack(v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < E; ++j) Elem<T>::store(out + idx + j, v[j]);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int NT>
+__device__ __forceinline__ void zero_row(const Row<T>& out, int u0, int u1, int ragged) {
+  T* o = const_cast<T*>(out.z);
+  if ((int)threadIdx.x < ragged) Elem<T>::store(o + out.ragged_index(threadIdx.x), 0.f);
+  uint4* p = const_cast<uint4*>(out.unit_ptr());
+  for (int u = u0 + (int)threadIdx.x; u < u1; u += NT) p[u] = make_uint4(0, 0, 0, 0);
+}
+
+// Units of segment `seg` of `nseg`; the first segment also takes the ragged elements.
+__device__ __forceinline__ void segment(int units, int seg, int nseg, int& u0, int& u1) {
+  const int per = (units + nseg - 1) / nseg;
+  u0 = min(units, seg * per);
+  u1 = min(units, u0 + per);
+}
+
+// ------------------------------------------------------------------ host
+
+template <typename T>
+struct Tag {
+  using type = T;
+};
+
+template <typename F>
+void for_logits_type(at::ScalarType dtype, F&& f) {
+  switch (dtype) {
+    case at::kBFloat16: f(Tag<__nv_bfloat16>{}); break;
+    case at::kHalf: f(Tag<__half>{}); break;
+    case at::kFloat: f(Tag<float>{}); break;
+    default: KB_CHECK(false, "logits must be bf16, fp16 or fp32");
+  }
+}
+
+void check_rows(const at::Tensor& t, const char* name, int64_t rows, int64_t cols, at::ScalarType dtype,
+                const at::Tensor& like) {
+  const std::string n(name);
+  KB_CHECK(t.is_cuda() && t.device() == like.device(), n + " must be on the logits' device");
+  KB_CHECK(t.scalar_type() == dtype, n + " has the wrong dtype");
+  KB_CHECK(t.is_contiguous() && t.numel() == rows * cols, n + " must be contiguous with one entry per row and column");
+}
+
+// logits [rows, >= vocab] with unit inner stride; returns the row count.
+int64_t check_logits(const at::Tensor& logits, int64_t vocab, double temperature, const char* name) {
+  const std::string n(name);
+  check_cuda_tensor(logits, name);
+  KB_CHECK(logits.dim() == 2, n + " must be [rows, vocab]");
+  KB_CHECK(vocab >= 1 && vocab <= logits.size(1), n + " has fewer columns than the vocabulary");
+  KB_CHECK(vocab <= (1 << 19), "vocabularies of more than 524288 entries are not supported");
+  KB_CHECK(logits.size(1) == 1 || logits.stride(1) == 1, n + " must have unit inner stride");
+  KB_CHECK(logits.size(0) <= 0x7FFFFFFF / 16, n + " has too many rows");
+  KB_CHECK(reinterpret_cast<uintptr_t>(logits.data_ptr()) % logits.element_size() == 0, n + " is misaligned");
+  KB_CHECK(temperature >= 1e-4 && temperature <= 1e4, "temperature must lie in [1e-4, 1e4]");
+  return logits.size(0);
+}
+
+void check_out(const at::Tensor& out, const at::Tensor& logits, int64_t vocab) {
+  KB_CHECK(out.is_cuda() && out.device() == logits.device() && out.scalar_type() == logits.scalar_type(),
+           "out must have the logits' device and dtype");
+  KB_CHECK(out.dim() == 2 && out.size(0) == logits.size(0) && out.size(1) >= vocab, "out must be [rows, vocab]");
+  KB_CHECK(out.size(1) == 1 || out.stride(1) == 1, "out must have unit inner stride");
+  KB_CHECK(out.size(0) <= 1 || out.stride(0) >= vocab, "rows of out overlap");
+}
+
+int row_segments(int64_t rows, int64_t vocab, int64_t elem, int threads, int device) {
+  const int64_t units = vocab * elem / 16;
+  const int64_t most = std::max<int64_t>(1, units / (2 * threads));
+  const int64_t want = (4 * (int64_t)num_sms(device) + rows - 1) / rows;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({most, want, 64}));
+}
+
+}  // namespace
+}  // namespace kb

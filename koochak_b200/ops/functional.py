@@ -9,14 +9,18 @@ out-of-memory surfaces as ``torch.OutOfMemoryError``.
 from __future__ import annotations
 
 import math
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 import torch.nn.functional as F
 
-from ._ext import native
+from ._ext import native, use_native
 
 ACT_NONE, ACT_GELU, ACT_GELU_BWD = 0, 1, 2
+
+# Alternatives of token_logprobs, or teacher slots of topk_distillation, per row.
+MAX_TOP_K = 128
+MAX_LIST_VOCAB = 1 << 19
 
 
 # ----------------------------------------------------------------- GEMM
@@ -186,6 +190,306 @@ def cross_entropy_forward(logits, target, vocab, ignore_index=-100):
 def cross_entropy_backward_(logits, target, lse, gscale, vocab, ignore_index=-100):
     native().cross_entropy_backward(logits, target.reshape(-1).contiguous(), lse, gscale, int(vocab), int(ignore_index))
     return logits
+
+
+# ------------------------------------------- per-token losses over a vocabulary
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` returns; every tensor has the logits' leading shape.
+
+    ``logprobs`` (None without tokens) and ``entropy`` carry gradients;
+    ``top_logprobs`` and ``top_ids`` (both ``[..., top_k]``, None for
+    ``top_k=0``) do not.
+    """
+
+    logprobs: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_logprobs: Optional[torch.Tensor]
+    top_ids: Optional[torch.Tensor]
+
+
+def _vocab_rows(logits: torch.Tensor, name: str) -> torch.Tensor:
+    """``logits`` as [rows, vocab] with unit inner stride (a view where the strides allow it)."""
+
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{name}: logits must be [..., vocab] with at least one column")
+    if logits.shape[-1] > MAX_LIST_VOCAB:
+        raise ValueError(f"{name}: vocabularies of more than {MAX_LIST_VOCAB} entries are not supported")
+    if logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"{name}: logits must be bf16, fp16 or fp32, got {logits.dtype}")
+    rows = logits.numel() // logits.shape[-1]
+    z = logits.reshape(rows, logits.shape[-1])
+    return z if z.stride(1) == 1 or z.shape[1] == 1 else z.contiguous()
+
+
+def _check_temperature(temperature: float, name: str) -> None:
+    if not 1e-4 <= temperature <= 1e4:
+        raise ValueError(f"{name}: temperature must lie in [1e-4, 1e4], got {temperature}")
+
+
+def _row_gradient(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if g is None else g.float().reshape(-1).contiguous()
+
+
+def _like_rows(z: torch.Tensor) -> torch.Tensor:
+    """An uninitialised [rows, vocab] tensor whose rows start where ``z``'s do modulo 16 bytes, if z's rows do not
+    overlap."""
+
+    rows, vocab = z.shape
+    ld = z.stride(0) if rows > 1 and vocab <= z.stride(0) <= vocab + 1024 else vocab
+    return torch.empty((rows, ld), device=z.device, dtype=z.dtype)[:, :vocab]
+
+
+def token_logprobs_forward(logits, tokens, *, top_k: int = 0, temperature: float = 1.0, ignore_index: int = -100):
+    """Returns (logprobs, entropy, stats, top_logprobs, top_ids) of 2-D ``logits`` (unit inner stride).
+
+    ``stats`` is what ``token_logprobs_backward`` needs; ``logprobs`` is None
+    without ``tokens``, the last two for ``top_k=0``.
+    """
+
+    rows, vocab = logits.shape
+    dev = logits.device
+    entropy = torch.empty(rows, device=dev, dtype=torch.float32)
+    stats = torch.empty((rows, native().TOKEN_LOGPROBS_STATS), device=dev, dtype=torch.float32)
+    logprobs = torch.empty(rows, device=dev, dtype=torch.float32) if tokens is not None else None
+    top_logprobs = torch.empty((rows, top_k), device=dev, dtype=torch.float32) if top_k else None
+    top_ids = torch.empty((rows, top_k), device=dev, dtype=torch.int64) if top_k else None
+    native().token_logprobs_forward(logits, tokens, logprobs, entropy, stats, top_logprobs, top_ids, int(vocab),
+                                    float(temperature), int(ignore_index))
+    return logprobs, entropy, stats, top_logprobs, top_ids
+
+
+def token_logprobs_backward(logits, tokens, stats, entropy, dlogprobs, dentropy, *, temperature: float = 1.0,
+                            ignore_index: int = -100, out: Optional[torch.Tensor] = None):
+    """Gradient of the logits from those of ``logprobs`` and ``entropy`` (fp32 rows, or None).
+
+    ``out=logits`` overwrites the logits with their gradient. Rows whose
+    gradients both are zero, and ignored rows, get zeros without being read.
+    """
+
+    out = _like_rows(logits) if out is None else out
+    native().token_logprobs_backward(logits, tokens, stats, entropy, dlogprobs, dentropy, out, int(logits.shape[1]),
+                                     float(temperature), int(ignore_index))
+    return out
+
+
+class _TokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top_k, temperature, ignore_index):
+        z = _vocab_rows(logits, "token_logprobs")
+        logprobs, entropy, stats, top_logprobs, top_ids = token_logprobs_forward(
+            z, tokens, top_k=top_k, temperature=temperature, ignore_index=ignore_index)
+        ctx.save_for_backward(logits, tokens, stats, entropy)
+        ctx.meta = (temperature, ignore_index)
+        ctx.set_materialize_grads(False)
+        if top_k:
+            ctx.mark_non_differentiable(top_logprobs, top_ids)
+        return logprobs, entropy, top_logprobs, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlogprobs, dentropy, _dtop, _dids):
+        logits, tokens, stats, entropy = ctx.saved_tensors
+        if dlogprobs is None and dentropy is None:
+            return None, None, None, None, None
+        temperature, ignore_index = ctx.meta
+        dz = token_logprobs_backward(_vocab_rows(logits, "token_logprobs"), tokens, stats, entropy,
+                                     _row_gradient(dlogprobs), _row_gradient(dentropy), temperature=temperature,
+                                     ignore_index=ignore_index)
+        return dz.view(logits.shape), None, None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, top_k: int = 0,
+                   temperature: float = 1.0, ignore_index: int = -100) -> TokenLogprobs:
+    """Log probabilities of given tokens, entropies and the most likely alternatives, in one pass over the logits.
+
+    ``logits`` is ``[..., vocab]`` in bf16, fp16 or fp32 (any row stride),
+    ``tokens`` ``[...]`` (int64; None when only entropy and alternatives are
+    wanted). With ``p = softmax(logits / temperature)``: ``logprobs`` is
+    ``log p[token]``, ``entropy`` ``-sum p log p`` in nats, ``top_ids`` the
+    ``top_k`` (at most 128) largest logits in descending order, equal logits
+    by their index, and ``top_logprobs`` their log probabilities. All are fp32
+    but the ids. The results of a row with ``tokens == ignore_index`` are
+    zeros and ids of -1; a token outside the vocabulary has a NaN log
+    probability. Logits of -inf are never produced (they add nothing to the
+    entropy); a row of -inf only, or with a NaN or +inf, gives NaN. NaN logits
+    rank above all others.
+    """
+
+    name = "token_logprobs"
+    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    z = _vocab_rows(logits, name)
+    _check_temperature(temperature, name)
+    if not 0 <= top_k <= min(MAX_TOP_K, vocab):
+        raise ValueError(f"{name}: top_k must lie in [0, {min(MAX_TOP_K, vocab)}], got {top_k}")
+    if tokens is not None:
+        if tokens.shape != lead or tokens.dtype != torch.int64 or tokens.device != logits.device:
+            raise ValueError(f"{name}: tokens must be int64 of shape {tuple(lead)} on {logits.device}")
+        tokens = tokens.reshape(-1).contiguous()
+    if not use_native(logits):
+        res = token_logprobs_ref(z, tokens, top_k=top_k, temperature=temperature, ignore_index=ignore_index)
+    else:
+        res = _TokenLogprobsFn.apply(logits, tokens, int(top_k), float(temperature), int(ignore_index))
+    logprobs, entropy, top_logprobs, top_ids = res
+    return TokenLogprobs(None if logprobs is None else logprobs.view(lead), entropy.view(lead),
+                         None if top_logprobs is None else top_logprobs.view(*lead, top_k),
+                         None if top_ids is None else top_ids.view(*lead, top_k))
+
+
+def token_logprobs_ref(logits, tokens, *, top_k: int = 0, temperature: float = 1.0, ignore_index: int = -100):
+    """2-D logits, 1-D tokens; (logprobs, entropy, top_logprobs, top_ids) in fp32 (fp64 for fp64 logits)."""
+
+    zf = logits if logits.dtype == torch.float64 else logits.float()
+    logp = torch.log_softmax(zf / temperature, dim=-1)
+    masked = torch.isneginf(zf) & torch.isfinite(logp.detach().amax(-1, keepdim=True))
+    entropy = -torch.where(masked, 0.0, logp.exp() * logp.masked_fill(masked, 0.0)).sum(-1)
+    counted = torch.ones_like(entropy, dtype=torch.bool) if tokens is None else tokens != ignore_index
+    logprobs = top_logprobs = top_ids = None
+    if tokens is not None:
+        inside = (tokens >= 0) & (tokens < logits.shape[1])
+        got = logp.gather(1, torch.where(inside, tokens, 0)[:, None])[:, 0]
+        logprobs = torch.where(counted, torch.where(inside, got, math.nan), 0.0)
+    if top_k:
+        ids = zf.detach().sort(dim=-1, descending=True, stable=True).indices[:, :top_k]
+        top_logprobs = torch.where(counted[:, None], logp.detach().gather(1, ids), 0.0)
+        top_ids = torch.where(counted[:, None], ids, -1)
+    return logprobs, torch.where(counted, entropy, 0.0), top_logprobs, top_ids
+
+
+def topk_distillation_forward(logits, teacher_ids, teacher_logits, *, temperature: float = 1.0, tail: bool = False):
+    """Returns (loss rows, stats for the backward pass) of 2-D ``logits`` and ``[rows, k]`` teachers."""
+
+    rows, vocab = logits.shape
+    loss = torch.empty(rows, device=logits.device, dtype=torch.float32)
+    stats = torch.empty((rows, native().TOPK_DISTILLATION_STATS), device=logits.device, dtype=torch.float32)
+    native().topk_distillation_forward(logits, teacher_ids, teacher_logits, loss, stats, int(vocab),
+                                       float(temperature), bool(tail))
+    return loss, stats
+
+
+def topk_distillation_backward(logits, teacher_ids, teacher_logits, stats, *, row_scale=None, scale=None,
+                               temperature: float = 1.0, tail: bool = False, out: Optional[torch.Tensor] = None):
+    """Gradient of ``sum(row_scale * loss) * scale`` (fp32 rows and scalar on the device; None is one).
+
+    ``out=logits`` overwrites the logits with their gradient. Rows of scale
+    zero, and rows without slots, get zeros without being read.
+    """
+
+    out = _like_rows(logits) if out is None else out
+    native().topk_distillation_backward(logits, teacher_ids, teacher_logits, stats, row_scale, scale, out,
+                                        int(logits.shape[1]), float(temperature), bool(tail))
+    return out
+
+
+class _TopkDistillationFn(torch.autograd.Function):
+    """Loss rows, or with ``weight`` their weighted sum."""
+
+    @staticmethod
+    def forward(ctx, logits, ids, teacher, weight, temperature, tail):
+        z = _vocab_rows(logits, "topk_distillation")
+        loss, stats = topk_distillation_forward(z, ids, teacher, temperature=temperature, tail=tail)
+        ctx.save_for_backward(logits, ids, teacher, weight, stats)
+        ctx.meta = (temperature, tail)
+        if weight is None:
+            return loss
+        return torch.where(weight == 0, 0.0, loss * weight).sum()
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        logits, ids, teacher, weight, stats = ctx.saved_tensors
+        temperature, tail = ctx.meta
+        g = _row_gradient(dloss)
+        dz = topk_distillation_backward(_vocab_rows(logits, "topk_distillation"), ids, teacher, stats,
+                                        row_scale=g if weight is None else weight,
+                                        scale=None if weight is None else g, temperature=temperature, tail=tail)
+        return dz.view(logits.shape), None, None, None, None, None
+
+
+def topk_distillation(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
+                      temperature: float = 1.0, tail: bool = False, weight: Optional[torch.Tensor] = None,
+                      reduction: str = "none") -> torch.Tensor:
+    """KL divergence of a student's distribution from a teacher known by its top logits.
+
+    ``logits`` is ``[..., vocab]`` (bf16, fp16 or fp32, any row stride), the
+    teacher's ``teacher_ids`` (int64) and ``teacher_logits`` (floating) are
+    ``[..., k]`` with 1 to 128 slots. Ids outside the vocabulary are empty
+    slots, so rows may hold fewer; ids of a row should differ (equal ones
+    count as separate slots). With ``p = softmax(logits / temperature)``:
+
+    * ``tail=False``: ``q = softmax(teacher_logits / temperature)`` over the
+      row's slots; the loss is ``sum q (log q - log p[id])``.
+    * ``tail=True``: ``teacher_logits`` are log probabilities at this
+      temperature (``token_logprobs(...).top_logprobs``), ``q`` their
+      exponentials, and the teacher's remaining mass ``1 - sum q`` is compared
+      with the student's mass outside the listed tokens as one more slot
+      (where the student has none, the loss is infinite and that slot adds
+      nothing to the gradient).
+
+    Rows without slots have loss and gradient zero. ``reduction="none"``
+    returns fp32 losses ``[...]``; ``"sum"`` returns their sum weighted by
+    ``weight`` (``[...]``, ones when None), where rows of weight zero are left
+    out altogether. The gradient reaches the logits only; it is not scaled by
+    the temperature's square.
+    """
+
+    name = "topk_distillation"
+    lead = logits.shape[:-1]
+    z = _vocab_rows(logits, name)
+    _check_temperature(temperature, name)
+    if reduction not in ("none", "sum"):
+        raise ValueError(f"{name}: reduction must be 'none' or 'sum', got {reduction!r}")
+    if teacher_ids.dim() != logits.dim() or teacher_ids.shape[:-1] != lead or teacher_ids.dtype != torch.int64:
+        raise ValueError(f"{name}: teacher_ids must be int64 of shape {(*lead, 'k')}")
+    if teacher_logits.shape != teacher_ids.shape or not teacher_logits.is_floating_point():
+        raise ValueError(f"{name}: teacher_logits must be floating, of teacher_ids' shape")
+    if not 1 <= teacher_ids.shape[-1] <= MAX_TOP_K:
+        raise ValueError(f"{name}: 1 to {MAX_TOP_K} teacher slots per row, got {teacher_ids.shape[-1]}")
+    if weight is not None and (reduction != "sum" or weight.shape != lead):
+        raise ValueError(f"{name}: weight goes with reduction='sum' and has shape {tuple(lead)}")
+    for other in (teacher_ids, teacher_logits, weight):
+        if other is not None and other.device != logits.device:
+            raise ValueError(f"{name}: all tensors must be on {logits.device}")
+    k = teacher_ids.shape[-1]
+    ids = teacher_ids.reshape(-1, k).contiguous()
+    teacher = teacher_logits.detach().reshape(-1, k).float().contiguous()
+    if reduction == "sum" and weight is None:
+        weight = torch.ones(lead, device=logits.device, dtype=torch.float32)
+    weight = None if weight is None else _row_gradient(weight.detach())
+    if not use_native(logits):
+        loss = topk_distillation_ref(z, ids, teacher, temperature=temperature, tail=tail)
+        if weight is not None:
+            return torch.where(weight == 0, 0.0, loss * weight).sum()
+    else:
+        loss = _TopkDistillationFn.apply(logits, ids, teacher, weight, float(temperature), bool(tail))
+    return loss if reduction == "sum" else loss.view(lead)
+
+
+def topk_distillation_ref(logits, teacher_ids, teacher_logits, *, temperature: float = 1.0, tail: bool = False):
+    """2-D logits and ``[rows, k]`` teachers; loss rows in fp32 (fp64 for fp64 logits)."""
+
+    zf = logits if logits.dtype == torch.float64 else logits.float()
+    logp = torch.log_softmax(zf / temperature, dim=-1)
+    valid = (teacher_ids >= 0) & (teacher_ids < logits.shape[1])
+    at = torch.where(valid, teacher_ids, 0)
+    t = torch.where(valid, teacher_logits.to(zf.dtype), -math.inf)
+    if tail:
+        q, logq = t.exp(), t
+    else:
+        t = t / temperature
+        high = t.amax(-1, keepdim=True)
+        e = (t - torch.where(high == -math.inf, 0.0, high)).exp()
+        total = e.sum(-1, keepdim=True)
+        q = torch.where(total == 0, 0.0, e / total)
+        logq = q.log()
+    loss = torch.where(q == 0, 0.0, q * (logq - logp.gather(1, at)).masked_fill(q == 0, 0.0)).sum(-1)
+    if tail:
+        listed = torch.zeros_like(logp.detach()).scatter_add_(1, at, valid.to(logp.dtype)) > 0
+        rest = (1.0 - q.sum(-1)).clamp_min(0.0)
+        log_rest = torch.logsumexp(logp.masked_fill(listed, -math.inf), -1)
+        loss = loss + torch.where(rest == 0, 0.0, rest * (rest.log() - log_rest).masked_fill(rest == 0, 0.0))
+    return torch.where(valid.any(-1), loss, 0.0)
 
 
 def bias_grad(g: torch.Tensor) -> torch.Tensor:

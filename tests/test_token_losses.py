@@ -1,0 +1,649 @@
+"""Log probabilities with entropy and alternatives, and distillation from top logits, against 64-bit definitions.
+
+The CPU tests check the reference forms (values, gradients by differences,
+refusals); the GPU tests compare the kernels with the reference forms in
+fp64 on the same inputs.
+
+Tolerances. A log probability is ln 2 ((z - m) c - log2 S): the product
+carries three fp32 roundings (2^-24 each, relative), the sum S of exponentials
+accurate to 2^-22 adds 2^-22 to its logarithm, and the last subtraction rounds
+once more, so an error of |log p| 2^-22 + 2^-20 is allowed. The entropy adds
+sum p log p whose terms each carry the error of p (2^-22, and 2^-24 |x| of the
+exponent) and of the logarithm: (H + log V) 2^-20 + 2^-19. Gradients are sums
+of two products of p with rows' factors of size G: p is off by 2^-22 and by
+2^-24 times an exponent below 128 where it matters (p > 2^-128), relative, so
+G 2^-17 covers p <= 1, plus half a step of the logits' type.
+"""
+
+import math
+
+import pytest
+import torch
+
+from koochak_b200.ops import functional as kf
+
+DEV = "cuda"
+gpu = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+IGNORE = -100
+
+
+@pytest.fixture(autouse=True)
+def _status_clean(request):
+    yield
+    if "gpu" in request.keywords and torch.cuda.is_available():
+        from koochak_b200.ops import check_status
+
+        torch.cuda.synchronize()
+        check_status()
+
+
+def _half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _logits(rows, vocab, dtype, layout="padded", seed=0, device=DEV, sigma=2.0):
+    """[rows, vocab] logits with some likely tokens; ``layout`` decides strides and alignment."""
+
+    gen = torch.Generator().manual_seed(seed)
+    z = torch.randn(rows, vocab, generator=gen) * sigma
+    n = min(8, vocab)
+    ids = torch.stack([torch.randperm(vocab, generator=gen)[:n] for _ in range(rows)]) if rows else \
+        torch.zeros(0, n, dtype=torch.int64)
+    z.scatter_add_(1, ids, torch.full((rows, n), 6.0))
+    z = z.to(device, dtype)
+    if layout == "contiguous":
+        return z
+    if layout == "padded":
+        ld = (vocab + 63) // 64 * 64
+        buf = torch.full((rows, ld), math.nan, device=device, dtype=dtype)
+    elif layout == "offset":  # rows start off every 16-byte boundary, by another distance each
+        buf = torch.full((rows, vocab + 5), math.nan, device=device, dtype=dtype)[:, 1:]
+    elif layout == "columns":  # inner stride is not one
+        buf = torch.full((vocab, rows), math.nan, device=device, dtype=dtype).t()
+    else:
+        raise AssertionError(layout)
+    buf = buf[:, :vocab]
+    buf.copy_(z)
+    return buf
+
+
+def _close(got, want, tol, what):
+    got, want = got.double().cpu(), want.double().cpu()
+    assert got.shape == want.shape, what
+    same = (got == want) | (got.isnan() & want.isnan())
+    err = torch.where(same, 0.0, (got - want).abs())
+    bad = ~(err <= (tol.double().cpu() if isinstance(tol, torch.Tensor) else tol))
+    assert not bad.any(), f"{what}: {bad.sum()} off, {got[bad][:4]} for {want[bad][:4]}"
+
+
+def _logprob_tol(want):
+    return torch.nan_to_num(want.abs(), nan=0.0, posinf=0.0) * 2.0**-22 + 2.0**-20
+
+
+def _check_logprobs(z, tokens, top_k=0, temperature=1.0, grads=True, seed=0):
+    vocab = z.shape[-1]
+    rows = z.numel() // vocab
+    z = z.detach().requires_grad_(grads)
+    res = kf.token_logprobs(z, tokens, top_k=top_k, temperature=temperature, ignore_index=IGNORE)
+    ref_z = z.detach().cpu().double().reshape(rows, vocab).requires_grad_(grads)
+    flat = None if tokens is None else tokens.cpu().reshape(-1)
+    logp, ent, tlp, tid = kf.token_logprobs_ref(ref_z, flat, top_k=top_k, temperature=temperature,
+                                                ignore_index=IGNORE)
+    lead = z.shape[:-1]
+    assert res.entropy.shape == lead and res.entropy.dtype == torch.float32
+    if tokens is None:
+        assert res.logprobs is None
+    else:
+        _close(res.logprobs.detach().reshape(-1), logp.detach(), _logprob_tol(logp.detach()), "logprobs")
+    tol = (ent.detach().nan_to_num(0.0).abs() + math.log(vocab)) * 2.0**-20 + 2.0**-19
+    _close(res.entropy.detach().reshape(-1), ent.detach(), tol, "entropy")
+    if top_k:
+        assert torch.equal(res.top_ids.cpu().reshape(rows, top_k), tid)
+        _close(res.top_logprobs.reshape(rows, top_k), tlp, _logprob_tol(tlp), "top_logprobs")
+    if not grads:
+        return res
+    gen = torch.Generator().manual_seed(seed + 1)
+    dlp, dh = torch.randn(rows, generator=gen), torch.randn(rows, generator=gen) * 0.3
+    outs, gs = [res.entropy.reshape(-1)], [dh.to(z.device)]
+    ref_outs, ref_gs = [ent], [dh.double()]
+    if tokens is not None:
+        outs, gs = outs + [res.logprobs.reshape(-1)], gs + [dlp.to(z.device)]
+        ref_outs, ref_gs = ref_outs + [logp], ref_gs + [dlp.double()]
+    (dz,) = torch.autograd.grad(outs, z, gs)
+    (want,) = torch.autograd.grad(ref_outs, ref_z, ref_gs)
+    assert dz.shape == z.shape and dz.dtype == z.dtype
+    size = (dlp.abs() + dh.abs() * (ent.detach().nan_to_num(0.0) + 1.0)).double() / temperature
+    tol = size[:, None] * 2.0**-17 + want.nan_to_num(0.0).abs() * _half_step(z.dtype) * (1 + 2.0**-10)
+    tol = tol + torch.finfo(z.dtype).tiny * _half_step(z.dtype) * 2
+    _close(dz.reshape(rows, vocab), want, tol, "dlogits")
+    return res
+
+
+def _tokens(rows, vocab, device=DEV, seed=0, ignored=True):
+    gen = torch.Generator().manual_seed(seed + 7)
+    t = torch.randint(0, vocab, (rows,), generator=gen)
+    if ignored and rows > 2:
+        t[::5] = IGNORE
+    return t.to(device)
+
+
+# ------------------------------------------------------------------- CPU
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+def test_reference_logprobs_and_gradient_by_differences(temperature):
+    torch.manual_seed(0)
+    z = torch.randn(3, 11, dtype=torch.float64, requires_grad=True)
+    tokens = torch.tensor([2, IGNORE, 10])
+
+    def f(x):
+        lp, ent, _, _ = kf.token_logprobs_ref(x, tokens, temperature=temperature, ignore_index=IGNORE)
+        return lp, ent
+
+    p = torch.softmax(z / temperature, -1)
+    lp, ent = f(z)
+    assert torch.allclose(lp[0], p[0, 2].log()) and lp[1] == 0 and ent[1] == 0
+    assert torch.allclose(ent[2], -(p[2] * p[2].log()).sum())
+    assert torch.autograd.gradcheck(f, (z,))
+    (g,) = torch.autograd.grad((lp[0] * 0.5 + ent[0] * 0.25), z)
+    hot = torch.zeros(11, dtype=torch.float64)
+    hot[2] = 1
+    want = (0.5 * (hot - p[0]) - 0.25 * p[0] * (p[0].log() + ent[0])) / temperature
+    assert torch.allclose(g[0], want) and not g[1].any()
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_reference_distillation_and_gradient_by_differences(tail):
+    torch.manual_seed(1)
+    z = torch.randn(4, 9, dtype=torch.float64, requires_grad=True)
+    ids = torch.tensor([[1, 5, 8], [0, -1, 3], [-1, -1, 99], [2, 2, 4]])
+    t = torch.log_softmax(torch.randn(4, 4, dtype=torch.float64), -1)[:, :3]
+    temperature = 1.5
+
+    def f(x):
+        return kf.topk_distillation_ref(x, ids, t, temperature=temperature, tail=tail)
+
+    loss = f(z)
+    assert loss[2] == 0 and torch.autograd.gradcheck(f, (z,))
+    p = torch.softmax(z.detach() / temperature, -1)
+    q = t[0].exp() if tail else torch.softmax(t[0] / temperature, -1)
+    want = (q * (q.log() - p[0, ids[0]].log())).sum()
+    if tail:
+        rest, p_rest = 1 - q.sum(), 1 - p[0, ids[0]].sum()
+        want = want + rest * (rest / p_rest).log()
+    assert torch.allclose(loss[0], want)
+    (g,) = torch.autograd.grad(loss[0], z)
+    dz = p[0].clone() if tail else p[0] * q.sum()
+    dz[ids[0]] -= q
+    if tail:
+        off = torch.ones(9, dtype=torch.bool)
+        off[ids[0]] = False
+        dz[off] -= rest * p[0][off] / p_rest
+    assert torch.allclose(g[0], dz / temperature)
+
+
+def test_reference_masks():
+    z = torch.randn(4, 6, dtype=torch.float64)
+    z[0, 1:4] = -math.inf
+    z[1] = -math.inf
+    z[2] = torch.finfo(torch.float32).min
+    lp, ent, tlp, tid = kf.token_logprobs_ref(z, torch.tensor([1, 1, 1, 7]), top_k=5)
+    keep = z[0, [0, 4, 5]].softmax(-1)
+    assert lp[0] == -math.inf and torch.allclose(ent[0], -(keep * keep.log()).sum())
+    assert tid[0, 3:].tolist() == [1, 2] and tlp[0, 3] == -math.inf
+    assert lp[1].isnan() and ent[1].isnan()
+    assert torch.allclose(ent[2], torch.tensor(math.log(6), dtype=torch.float64)) and tid[2].tolist() == [0, 1, 2, 3, 4]
+    assert lp[3].isnan() and ent[3].isfinite()  # token outside the vocabulary
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_refusals(device):
+    z = torch.randn(3, 40, device=device)
+    tok = torch.zeros(3, dtype=torch.int64, device=device)
+    ids = torch.zeros(3, 4, dtype=torch.int64, device=device)
+    t = torch.zeros(3, 4, device=device)
+    for bad in (dict(top_k=-1), dict(top_k=41), dict(temperature=0.0), dict(temperature=math.nan),
+                dict(temperature=-1.0), dict(temperature=math.inf)):
+        with pytest.raises(ValueError):
+            kf.token_logprobs(z, tok, **bad)
+    with pytest.raises(ValueError):
+        kf.token_logprobs(z.new_zeros(2, 300), tok[:2], top_k=129)
+    with pytest.raises(ValueError):
+        kf.token_logprobs(z, tok[:2])
+    with pytest.raises(ValueError):
+        kf.token_logprobs(z, tok.int())
+    with pytest.raises(TypeError):
+        kf.token_logprobs(z.double(), tok)
+    with pytest.raises(ValueError):
+        kf.token_logprobs(z[:, :0], tok)
+    with pytest.raises(ValueError):
+        kf.token_logprobs(z.new_zeros(1, 1).expand(1, (1 << 19) + 1), tok[:1])
+    with pytest.raises(ValueError):
+        kf.topk_distillation(z, ids, t, reduction="mean")
+    with pytest.raises(ValueError):
+        kf.topk_distillation(z, ids, t, weight=torch.ones(3, device=device))
+    with pytest.raises(ValueError):
+        kf.topk_distillation(z, ids, t, weight=torch.ones(2, device=device), reduction="sum")
+    with pytest.raises(ValueError):
+        kf.topk_distillation(z, ids.int(), t)
+    with pytest.raises(ValueError):
+        kf.topk_distillation(z, ids, t[:, :3])
+    with pytest.raises(ValueError):
+        kf.topk_distillation(z, ids, ids)
+    with pytest.raises(ValueError):
+        kf.topk_distillation(z, ids[:, :0], t[:, :0])
+    with pytest.raises(ValueError):
+        kf.topk_distillation(z, ids.repeat(1, 40), t.repeat(1, 40))
+    with pytest.raises(ValueError):
+        kf.topk_distillation(z, ids, t, temperature=0)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_leading_shapes_and_empty_batches(device):
+    z = _logits(6, 50, torch.float32, "contiguous", device=device).view(2, 3, 50)
+    tok = _tokens(6, 50, device, ignored=False).view(2, 3)
+    res = kf.token_logprobs(z, tok, top_k=3)
+    assert res.logprobs.shape == (2, 3) and res.top_ids.shape == (2, 3, 3)
+    loss = kf.topk_distillation(z, res.top_ids, res.top_logprobs, tail=True)
+    assert loss.shape == (2, 3)
+    # A student that is its own teacher: 2^-19 covers the roundings of q and p against one another.
+    assert loss.abs().max() < 2.0**-19
+    one = kf.token_logprobs(z[0, 0], tok[0, 0], top_k=2)
+    assert one.logprobs.shape == () and one.top_ids.shape == (2,)
+    for empty in (z[:0], z[:, :0]):
+        lead = empty.shape[:-1]
+        e = kf.token_logprobs(empty, tok.new_zeros(lead), top_k=2)
+        assert e.logprobs.shape == lead and e.top_ids.shape == (*lead, 2)
+        assert kf.topk_distillation(empty, tok.new_zeros(*lead, 4), z.new_zeros(*lead, 4)).shape == lead
+        assert kf.topk_distillation(empty, tok.new_zeros(*lead, 4), z.new_zeros(*lead, 4), reduction="sum") == 0
+
+
+# ------------------------------------------------------- log probabilities
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,layout", [
+    (1, 1, "contiguous"), (3, 2, "contiguous"), (2, 7, "offset"), (5, 129, "offset"), (4, 1000, "padded"),
+    (7, 1001, "contiguous"), (6, 4099, "offset"), (3, 8193, "columns"), (5, 32000, "padded"), (4, 50257, "contiguous"),
+    (300, 4099, "contiguous"), (2, 131072, "padded"), (1, 524288, "padded"),
+])
+def test_logprobs_shapes(dtype, rows, vocab, layout):
+    z = _logits(rows, vocab, dtype, layout)
+    _check_logprobs(z, _tokens(rows, vocab), top_k=min(5, vocab))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [128, 1000, 4100, 4500, 50257])
+@pytest.mark.parametrize("top_k", [1, 2, 31, 33, 128])
+def test_alternatives(dtype, vocab, top_k):
+    _check_logprobs(_logits(5, vocab, dtype, "contiguous", seed=top_k), None, top_k=top_k, grads=False)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("temperature", [0.05, 0.7, 3.0, 100.0])
+def test_logprobs_temperature(dtype, temperature):
+    z = _logits(6, 5000, dtype)
+    # Logits up to about 16 / 0.05: the log probabilities grow with 1 / T, and their error with them.
+    _check_logprobs(z, _tokens(6, 5000), top_k=7, temperature=temperature)
+
+
+def _hard_rows(vocab, dtype, device):
+    """Rows where selection and sums can go wrong: ties, masks, order in memory, extremes."""
+
+    low = torch.finfo(dtype).min
+    gen = torch.Generator().manual_seed(3)
+    r = torch.randn(vocab, generator=gen)
+    asc = torch.linspace(-9, 9, vocab)
+    rows = [
+        torch.zeros(vocab),                                        # every value the same
+        asc, asc.flip(0),                                          # sorted in memory
+        torch.where(torch.arange(vocab) % 2 == 0, 0.0, -0.0),      # zeros of both signs are ties
+        torch.where(torch.arange(vocab) < vocab - 3, -math.inf, r),    # fewer tokens left than alternatives
+        torch.where(torch.arange(vocab) == vocab // 2, 1.0, -math.inf),  # one token left
+        torch.full((vocab,), low),                                 # masked by the lowest value throughout
+        torch.where(torch.arange(vocab) % 7 == 3, r, low),
+        torch.round(r),                                            # few distinct values
+        torch.where(torch.arange(vocab) < 150, 5.0 + r, r - 9.0),  # the likely ones side by side
+        torch.where(torch.arange(vocab) % 512 == 5, 4.0 + r, r),   # ... or in one thread's share
+        torch.where(torch.arange(vocab) % 4096 < 8, 4.0 + r, r),
+        r * 1e-3, r.clamp(-1, 1) * 1000,
+    ]
+    return torch.stack(rows).to(dtype).to(device)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [200, 3001, 40001])
+@pytest.mark.parametrize("top_k", [3, 128])
+def test_hard_rows(dtype, vocab, top_k):
+    z = _hard_rows(vocab, dtype, DEV)
+    _check_logprobs(z, _tokens(len(z), vocab, ignored=False), top_k=top_k)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_without_distribution(dtype):
+    """-inf throughout, a NaN or +inf: NaN results, as the definitions give; NaN ranks first."""
+
+    z = _logits(4, 5003, dtype, "contiguous")
+    z[0] = -math.inf
+    z[1, 4000] = math.nan
+    z[2, 17] = math.inf
+    res = kf.token_logprobs(z.requires_grad_(), _tokens(4, 5003, ignored=False), top_k=4)
+    assert res.logprobs[:3].isnan().all() and res.entropy[:3].isnan().all()
+    assert res.logprobs[3].isfinite() and res.entropy[3].isfinite()
+    assert res.top_ids[0].tolist() == [0, 1, 2, 3] and res.top_ids[1, 0] == 4000 and res.top_ids[2, 0] == 17
+    assert res.top_logprobs[3].isfinite().all()
+    (dz,) = torch.autograd.grad(res.logprobs.sum(), z)
+    assert dz[:3].isnan().any(1).all() and dz[3].isfinite().all()
+
+
+@gpu
+def test_rows_left_out_are_not_read():
+    """Ignored rows and rows of zero gradient give zeros whatever they hold; tokens outside the vocabulary give NaN."""
+
+    z = _logits(4, 999, torch.bfloat16, "contiguous")
+    z[0], z[1] = math.nan, math.nan
+    z = z.requires_grad_()
+    tok = torch.tensor([IGNORE, 5, 999, -3], device=DEV)
+    res = kf.token_logprobs(z, tok, top_k=2)
+    assert res.logprobs[0] == 0 and res.entropy[0] == 0 and res.top_ids[0].tolist() == [-1, -1]
+    assert res.logprobs[2].isnan() and res.logprobs[3].isnan() and res.entropy[2:].isfinite().all()
+    (dz,) = torch.autograd.grad(res.logprobs, z, torch.tensor([1.0, 0.0, 1.0, 0.0], device=DEV), retain_graph=True)
+    assert not dz[0].any() and not dz[1].any() and dz[2].isnan().all() and not dz[3].any()
+    (dz,) = torch.autograd.grad(res.entropy[3], z)
+    assert dz[3].isfinite().all() and dz[3].any() and not dz[:3].any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_in_place_gradients(dtype):
+    """The low-level backward calls may overwrite the logits; other columns and rows stay as they were."""
+
+    rows, vocab = 37, 1003
+    buf = torch.full((rows + 1, 1024), 7.0, device=DEV, dtype=dtype)
+    buf[:rows, :vocab] = _logits(rows, vocab, dtype, "contiguous")
+    tok = _tokens(rows, vocab)
+    for in_place in (lambda z, out: kf.token_logprobs_backward(
+            z, tok, *_lp_saved(z, tok), torch.ones(rows, device=DEV), torch.ones(rows, device=DEV),
+            ignore_index=IGNORE, out=out), lambda z, out: _kd_backward(z, out)):
+        apart = in_place(buf[:rows, :vocab], None)
+        b = buf.clone()
+        z = b[:rows, :vocab]
+        assert in_place(z, z) is z
+        assert torch.equal(z, apart)
+        assert (b[rows] == 7).all() and (b[:, vocab:] == 7).all()
+
+
+def _lp_saved(z, tok):
+    _, entropy, stats, _, _ = kf.token_logprobs_forward(z, tok, ignore_index=IGNORE)
+    return stats, entropy
+
+
+def _kd_backward(z, out):
+    ids, t = _teacher(z.shape[0], z.shape[1], 9, tail=True)
+    _, stats = kf.topk_distillation_forward(z, ids, t, tail=True)
+    return kf.topk_distillation_backward(z, ids, t, stats, tail=True, out=out)
+
+
+# ------------------------------------------------------------ distillation
+
+
+def _teacher(rows, vocab, k, tail, seed=0, ragged=True, device=DEV):
+    gen = torch.Generator().manual_seed(seed + 11)
+    ids = torch.stack([torch.randperm(vocab, generator=gen)[:k] if k <= vocab else
+                       torch.randint(0, vocab, (k,), generator=gen) for _ in range(rows)])
+    t = torch.randn(rows, k + 1, generator=gen) * 2
+    t = torch.log_softmax(t, -1)[:, :k] if tail else t[:, :k]
+    if ragged and k > 2:
+        ids[:, 1] = -1
+        ids[::3, 2] = vocab + 5
+    if ragged and rows > 3:
+        ids[3] = -1
+    return ids.to(device), t.contiguous().to(device)
+
+
+def _check_distill(z, ids, t, tail, temperature=1.0, weight=None, scale=1.0, seed=0):
+    rows, vocab = z.shape
+    z = z.detach().requires_grad_()
+    zr = z.detach().cpu().double().requires_grad_()
+    want = kf.topk_distillation_ref(zr, ids.cpu(), t.cpu(), temperature=temperature, tail=tail)
+    gen = torch.Generator().manual_seed(seed + 5)
+    if weight is None:
+        loss = kf.topk_distillation(z, ids, t, temperature=temperature, tail=tail)
+        g = torch.randn(rows, generator=gen)
+        (dz,) = torch.autograd.grad(loss, z, g.to(z.device))
+        (dr,) = torch.autograd.grad(want, zr, g.double())
+        got = loss.detach()
+    else:
+        g = weight.cpu() * scale
+        total = kf.topk_distillation(z, ids, t, temperature=temperature, tail=tail, weight=weight, reduction="sum")
+        (dz,) = torch.autograd.grad(total, z, torch.tensor(scale, device=z.device))
+        (dr,) = torch.autograd.grad(want, zr, g.double())
+        want = torch.where(weight.cpu() == 0, 0.0, want.detach() * weight.cpu().double())
+        got, want = total.detach()[None], want.sum()[None]
+        wsum = weight.abs().sum().item()
+    # The loss is a mean (sum q <= 1 + rounding) of differences of log q and log p, each as exact as a log probability.
+    lp = torch.log_softmax(zr.detach() / temperature, -1)
+    size = torch.where(lp.isinf(), 0.0, lp).abs().amax(-1).nan_to_num(0.0).max().item() + 16
+    tol = size * 2.0**-20 * (1.0 if weight is None else wsum)
+    _close(got, want.detach(), tol, "loss")
+    # dz = g / T (Q p - q [- q_rest p / p_rest]): three numbers of at most 1, each accurate to 2^-18.
+    tol = g.abs().double()[:, None] / temperature * 2.0**-16 + dr.nan_to_num(0.0).abs() * _half_step(z.dtype) * 1.01
+    _close(dz, dr, tol + torch.finfo(z.dtype).tiny * _half_step(z.dtype) * 2, "dlogits")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("rows,vocab,k,layout", [
+    (1, 1, 1, "contiguous"), (2, 7, 7, "offset"), (5, 129, 3, "offset"), (4, 1000, 128, "padded"),
+    (7, 1001, 16, "contiguous"), (6, 4099, 33, "offset"), (3, 8193, 5, "columns"), (5, 32000, 64, "padded"),
+    (4, 50257, 128, "contiguous"), (300, 4099, 8, "contiguous"), (1, 131072, 100, "padded"), (1, 524288, 20, "padded"),
+])
+def test_distillation_shapes(dtype, tail, rows, vocab, k, layout):
+    z = _logits(rows, vocab, dtype, layout)
+    ids, t = _teacher(rows, vocab, k, tail)
+    _check_distill(z, ids, t, tail, temperature=1.0 if tail else 2.0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("rows,vocab,layout", [(1, 777, "contiguous"), (37, 1001, "offset"), (9, 50257, "padded"),
+                                               (333, 5000, "padded"), (3, 131072, "contiguous")])
+@pytest.mark.parametrize("scale", [1.0, 0.375])
+def test_distillation_weighted_sum(dtype, tail, rows, vocab, layout, scale):
+    z = _logits(rows, vocab, dtype, layout)
+    ids, t = _teacher(rows, vocab, 12, tail)
+    weight = torch.rand(rows, device=DEV) + 0.1
+    weight[rows // 2::4] = 0
+    z[rows // 2::4] = math.nan  # rows of weight zero are left out
+    zc = z.clone()
+    zc[rows // 2::4] = 0
+    z0 = z.detach().requires_grad_()
+    a = kf.topk_distillation(z0, ids, t, tail=tail, weight=weight, reduction="sum")
+    (da,) = torch.autograd.grad(a, z0)
+    assert a.isfinite() and da.isfinite().all() and not da[rows // 2::4].any()
+    _check_distill(zc, ids, t, tail, weight=weight, scale=scale)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tail", [False, True])
+def test_distillation_repeated_and_masked(dtype, tail):
+    """The same id twice, every id of the vocabulary, teachers of -inf, student masks on and off the list."""
+
+    vocab, k = 301, 40
+    z = _logits(8, vocab, dtype, "offset")
+    ids, t = _teacher(8, vocab, k, tail, ragged=False)
+    ids[0, 5], ids[0, 7] = ids[0, 1], ids[0, 1]
+    ids[1] = 300
+    ids[2, 1:] = -1
+    t[3, 4:] = -math.inf
+    z[4, ids[4, 3:].sort().values[0]] = -math.inf
+    z[5].index_fill_(0, torch.arange(vocab, device=DEV)[~torch.isin(torch.arange(vocab, device=DEV), ids[5])],
+                     -math.inf)
+    off = torch.arange(vocab, device=DEV)[~torch.isin(torch.arange(vocab, device=DEV), ids[6])]
+    z[6].index_fill_(0, off[::2], torch.finfo(dtype).min)
+    rows = [0, 2, 3, 4, 6] if tail else list(range(8))
+    if tail:  # row 5 has no student mass off the list, row 1 lists one token 40 times: infinite or above one
+        inf = kf.topk_distillation(z, ids, t, tail=True)
+        assert inf[5] == math.inf
+    _check_distill(z[rows], ids[rows], t[rows], tail)
+    if not tail:
+        t[7] = -math.inf
+        assert kf.topk_distillation(z, ids, t)[7] == 0
+    small = _logits(2, 6, dtype, "contiguous")
+    all_ids = torch.arange(6, device=DEV).repeat(2, 1)
+    q = torch.log_softmax(torch.randn(2, 6, device=DEV), -1) + 1e-3  # sums to a little over one: no rest
+    if tail:
+        _check_distill(small, all_ids, q, True)
+
+
+@gpu
+def test_distillation_rows_without_slots_are_not_read():
+    z = torch.full((3, 500), math.nan, device=DEV, dtype=torch.float16)
+    z[1] = 1.0
+    ids = torch.tensor([[-1, 500], [3, -1], [-7, 1 << 40]], device=DEV)
+    z = z.requires_grad_()
+    for tail in (False, True):
+        loss = kf.topk_distillation(z, ids, torch.zeros(3, 2, device=DEV) - 0.5, tail=tail)
+        (dz,) = torch.autograd.grad(loss.sum(), z)
+        assert loss[0] == 0 and loss[2] == 0 and loss[1] > 0
+        assert not dz[0].any() and not dz[2].any() and dz[1].isfinite().all()
+
+
+@gpu
+def test_student_mass_far_below_fp32():
+    """The rest's probability is a sum of its own: exact where one minus the listed mass would be zero."""
+
+    z = torch.full((2, 1000), -60.0, device=DEV)
+    z[:, :4] = torch.tensor([1.0, 0.5, 0.0, -0.5])
+    ids = torch.arange(4, device=DEV).repeat(2, 1)
+    t = torch.log(torch.tensor([0.5, 0.2, 0.15, 0.1], device=DEV)).repeat(2, 1)
+    _check_distill(z, ids, t, True)
+
+
+# ----------------------------------------------------------------- together
+
+
+@gpu
+def test_teacher_to_student_run():
+    """Alternatives of a teacher feed a student's loss; gradient descent on the student's logits follows the formula."""
+
+    rows, vocab, k = 64, 5003, 32
+    teacher = _logits(rows, vocab, torch.bfloat16, "padded", seed=1)
+    tok = _tokens(rows, vocab)
+    got = kf.token_logprobs(teacher, tok, top_k=k, ignore_index=IGNORE)
+    student = _logits(rows, vocab, torch.float32, "contiguous", seed=2)
+    _check_distill(student, got.top_ids, got.top_logprobs, True)
+    s = student.requires_grad_()
+    loss = kf.topk_distillation(s, got.top_ids, got.top_logprobs, tail=True)
+    assert (loss[tok == IGNORE] == 0).all()  # ignored rows came back with empty slots
+    (g,) = torch.autograd.grad(loss.sum(), s)
+    after = kf.topk_distillation(s.detach() - 1e-2 * g, got.top_ids, got.top_logprobs, tail=True)
+    assert (after <= loss).all()
+
+
+@gpu
+def test_broadcast_gradients_and_reuse():
+    """Expanded upstream gradients, two losses on one set of logits, and backward twice."""
+
+    z = _logits(20, 3001, torch.float32, "contiguous").requires_grad_()
+    tok = _tokens(20, 3001, ignored=False)
+    ids, t = _teacher(20, 3001, 6, False)
+    res = kf.token_logprobs(z, tok)
+    loss = kf.topk_distillation(z, ids, t, weight=torch.ones(20, device=DEV), reduction="sum")
+    total = res.logprobs.sum() + 0.5 * res.entropy.mean() + loss
+    total.backward(retain_graph=True)
+    once = z.grad.clone()
+    total.backward()
+    # Accumulating equal fp32 gradients twice is a doubling, which is exact.
+    assert torch.equal(z.grad, 2 * once)
+    zr = z.detach().cpu().double().requires_grad_()
+    lp, ent, _, _ = kf.token_logprobs_ref(zr, tok.cpu())
+    kd = kf.topk_distillation_ref(zr, ids.cpu(), t.cpu())
+    (lp.sum() + 0.5 * ent.mean() + kd.sum()).backward()
+    _close(once, zr.grad, 3 * 2.0**-16, "sum of gradients")
+
+
+@gpu
+def test_other_stream_and_graph():
+    """Work is enqueued on the caller's stream, and forward with backward can be captured and replayed."""
+
+    z = _logits(33, 4099, torch.bfloat16, "padded")
+    tok = _tokens(33, 4099)
+    ids, t = _teacher(33, 4099, 10, True)
+    w = torch.rand(33, device=DEV)
+
+    def step(x):
+        x = x.detach().requires_grad_()
+        res = kf.token_logprobs(x, tok, top_k=5)
+        a, = torch.autograd.grad(res.logprobs.sum() + res.entropy.sum(), x)
+        loss = kf.topk_distillation(x, ids, t, tail=True, weight=w, reduction="sum")
+        b, = torch.autograd.grad(loss, x)
+        return [res.logprobs.detach(), res.entropy.detach(), res.top_ids, a, loss.detach(), b]
+
+    want = step(z)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(z)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    static = z.clone()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(static)
+        graphs.append((g, out))
+    other = _logits(33, 4099, torch.bfloat16, "padded", seed=9)
+    for data in (z, other):
+        static.copy_(data)
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        again = step(static)  # the same rows at the same alignment: sums are cut at 16-byte boundaries
+        for _, out in graphs:
+            assert all(torch.equal(x, y) for x, y in zip(out, again))
+
+
+@gpu
+def test_repeatable():
+    z = _logits(500, 32000, torch.bfloat16)
+    tok = _tokens(500, 32000)
+    first = kf.token_logprobs(z, tok, top_k=40)
+    for _ in range(3):
+        again = kf.token_logprobs(z, tok, top_k=40)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+    ids, t = first.top_ids, first.top_logprobs
+    one = kf.topk_distillation(z, ids, t, tail=True)
+    assert torch.equal(one, kf.topk_distillation(z, ids, t, tail=True))
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """The last rows of a logits buffer of more than 2^32 bytes and more than 2^31 elements."""
+
+    rows, vocab = 17000, 131072
+    if torch.cuda.get_device_properties(0).total_memory < 40 << 30:
+        pytest.skip("needs 20 GB")
+    z = torch.zeros(rows, vocab, device=DEV, dtype=torch.bfloat16)
+    z[-3:] = _logits(3, vocab, torch.bfloat16, "contiguous")
+    tok = torch.full((rows,), IGNORE, device=DEV)
+    tok[-3:] = torch.tensor([5, 70000, 131071], device=DEV)
+    res = kf.token_logprobs(z, tok, top_k=9)
+    small = kf.token_logprobs(z[-3:].clone(), tok[-3:], top_k=9)
+    for a, b in zip(res, small):
+        assert torch.equal(a[-3:], b)
+    assert not res.logprobs[:-3].any()
+    ids, t = res.top_ids, res.top_logprobs
+    loss, stats = kf.topk_distillation_forward(z, ids, t, tail=True)
+    d = kf.topk_distillation_backward(z, ids, t, stats, tail=True, out=z)
+    assert not d[:-3].any() and d[-3:].any(1).all()
