@@ -7,7 +7,7 @@
 namespace kb {
 namespace {
 
-constexpr int kCand = 2048;  // candidates held while the alternatives are selected
+constexpr int kCand = 1024;  // candidates held while the alternatives are selected
 constexpr int kStats = 2;    // floats kept per row for the backward pass: m, log2 S
 
 // ----------------------------------------------------------- alternatives
@@ -26,102 +26,138 @@ __device__ __forceinline__ unsigned long long key_of(uint32_t order, int index) 
   return ((unsigned long long)order << 32) | (uint32_t)~index;
 }
 
+constexpr int kHits = 512;  // units looked at element by element
+
+template <int NT>
 struct SelectShared {
-  unsigned long long cand[kCand];
-  unsigned long long sorted[kMaxList];
-  uint32_t wmin[32], wmax[32];
-  int count, listed;
-  int warp_sum[32];
-  uint16_t tids[1024];
+  static constexpr int kGroups = NT <= 256 ? 16 : 8;  // maxima kept per thread: batch b counts to group b % kGroups
+  union alignas(16) {
+    float group_max[kGroups][NT];
+    unsigned long long cand[kCand];
+  };
+  union {
+    uint16_t list[kGroups * NT];
+    int sums[kCand];  // ranks, or counts per warp
+  };
+  uint4 hit[kHits];
+  int hit_unit[kHits];
+  uint32_t warp_key[NT / 32], warp_top[NT / 32];
+  int count, listed, hits;
 };
 
-// The k largest keys of a block's elements, sorted, in sh.sorted (padded with
-// 0 where the block has fewer).
+// Calls emit(i, key) for the k largest keys of a block's elements, i their
+// places in descending order (fewer where the block has fewer elements).
 //
-// Selection without a second pass over the row: every thread knows the
-// maximum of its own elements. If t is the k-th largest of the thread maxima,
-// at least k elements are >= t, so only the threads whose maximum is >= t
-// (about k of them) hold elements of the answer. t is found by bisection on
-// the integer order, one vote of the block per step; it may stop early at a
-// slightly lower t. The elements of those threads are read again (from L2)
-// by the whole block and those >= t are ranked by counting.
+// Selection without a second pass over the row: the statistics' pass keeps
+// the maximum of each thread, and of each group of a thread's batches.
+// 1. With r = k / warps, rounded up, let t be the least of the warps' r-th
+//    largest thread maxima: at least k elements are >= t.
+// 2. One warp bisects t among those groups' maxima until not many more than k
+//    are left. All k largest elements are >= t still, and lie in these groups.
+// 3. Those groups are read again (from L2), first for the units with an
+//    element >= t, then for the elements, which are ranked by counting.
 // Ties and rows sorted in memory can make the candidates overflow; then the
 // k-th value is bisected over the row itself and ties are taken in index order.
-template <typename T, int NT>
-__device__ void select_top(const Row<T>& row, int u0, int u1, int ragged, float mine, int k, SelectShared& sh) {
-  constexpr int E = Elem<T>::kUnit;
+template <typename T, int NT, typename Emit>
+__device__ void select_top(const Row<T>& row, int u0, int u1, int ragged, float mine, int k, SelectShared<NT>& sh,
+                           const Emit& emit) {
+  constexpr int E = Elem<T>::kUnit, NW = NT / 32, kGroups = SelectShared<NT>::kGroups;
+  static_assert(NW <= 32 && NT * kGroups <= 65536, "list entries are 16 bits wide");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n_units = u1 - u0;
-  const int total = n_units * E + ragged;
-  const int want = min(k, total);
+  const int want = min(k, n_units * E + ragged);
   const bool has = tid < n_units || tid < ragged;
   const uint32_t key = has ? order_of(mine) : 0u;
-  const uint32_t wmin = __reduce_min_sync(0xffffffffu, key), wmax = __reduce_max_sync(0xffffffffu, key);
-  if (lane == 0) {
-    sh.wmin[warp] = wmin;
-    sh.wmax[warp] = wmax;
+  {
+    // The warp's r-th largest: take the maximum out until r are gone.
+    const int r = (want + NW - 1) / NW;
+    uint32_t rest = key, top = 0;
+    int gone = 0;
+    while (gone < r) {
+      top = __reduce_max_sync(0xffffffffu, rest);
+      if (lane == 0 && gone == 0) sh.warp_top[warp] = top;
+      gone = top == 0 ? r : gone + __popc(__ballot_sync(0xffffffffu, rest == top));
+      rest = rest == top ? 0u : rest;
+    }
+    if (lane == 0) sh.warp_key[warp] = top;
   }
   if (tid == 0) {
     sh.count = 0;
     sh.listed = 0;
+    sh.hits = 0;
   }
-  for (int i = tid; i < k; i += NT) sh.sorted[i] = 0;
   __syncthreads();
-  uint32_t lo = 0xFFFFFFFFu, top = 0u;
-  for (int w = 0; w < NT / 32; ++w) {
-    lo = min(lo, sh.wmin[w]);
-    top = max(top, sh.wmax[w]);
+  // 0: some warp has fewer elements, all stay
+  uint32_t t = max(__reduce_min_sync(0xffffffffu, sh.warp_key[lane & (NW - 1)]), 1u);
+  const uint32_t top = __reduce_max_sync(0xffffffffu, sh.warp_top[lane & (NW - 1)]);
+  const int batches = (n_units + kBatch * NT - 1) / (kBatch * NT);
+  if (key >= t) {
+    for (int g = 0; g < min(batches, kGroups); ++g)
+      if (tid + g * kBatch * NT < n_units && order_of(sh.group_max[g][tid]) >= t)
+        sh.list[atomicAdd(&sh.listed, 1)] = (uint16_t)(g * NT + tid);
   }
-  // count(key >= lo) >= want, count(key > hi) < want; with fewer threads than `want` every element stays.
-  if (want > NT) lo = 0;
-  uint32_t hi = want > NT ? 0u : top;
-  const int enough = want + (want >> 2) + 4;
-  while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo) / 2 + 1;
-    const int n = __syncthreads_count(key >= mid);
-    if (n >= want) {
-      lo = mid;
-      if (n <= enough) break;
-    } else {
-      hi = mid - 1;
-    }
-  }
-  const uint32_t t = max(lo, 1u);
-  if (key >= t) sh.tids[atomicAdd(&sh.listed, 1)] = (uint16_t)tid;
   __syncthreads();
-  const int per = (n_units + NT - 1) / NT + 1;  // a thread's units, and one ragged element
-  const int tasks = sh.listed * per;
-  const uint4* p = row.unit_ptr();
-  for (int i = tid; i < tasks; i += NT) {
-    const int who = sh.tids[i / per], j = i % per;
-    if (j == per - 1) {
-      if (who < ragged) {
-        const int idx = row.ragged_index(who);
-        const uint32_t o = order_of(Elem<T>::load(row.z + idx));
-        if (o >= t) {
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kCand) sh.cand[at] = key_of(o, idx);
+  const int listed = sh.listed;
+  constexpr int kOwn = 16;  // maxima per lane in step 2
+  if (listed > want + want / 8 + 2 && listed <= 32 * kOwn) {
+    if (warp == 0) {
+      uint32_t own[kOwn];
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        const int at = i * 32 + lane;
+        own[i] = 0;
+        if (at < listed) own[i] = order_of(sh.group_max[sh.list[at] / NT][sh.list[at] % NT]);
+      }
+      uint32_t lo = t, hi = top;  // count(>= lo) >= want, count(> hi) < want
+      while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2 + 1;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+          if (i * 32 < listed) n += __popc(__ballot_sync(0xffffffffu, own[i] >= mid));
+        if (n >= want) {
+          lo = mid;
+          if (n <= want + want / 8 + 2) break;
+        } else {
+          hi = mid - 1;
         }
       }
-    } else {
-      const int u = u0 + who + j * NT;
-      if (u < u1) {
+      if (lane == 0) sh.warp_key[0] = lo;
+    }
+    __syncthreads();
+    t = sh.warp_key[0];
+  }
+  auto push = [&](uint32_t o, int idx) {
+    if (o >= t) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kCand) sh.cand[at] = key_of(o, idx);
+    }
+  };
+  const uint4* p = row.unit_ptr();
+  for (int first = 0; first < batches; first += kGroups) {
+    for (int i = tid; i < listed * kBatch; i += NT) {
+      const int entry = sh.list[i / kBatch];
+      const int u = u0 + entry % NT + ((entry / NT + first) * kBatch + i % kBatch) * NT;
+      if (u < u1 && order_of(sh.group_max[entry / NT][entry % NT]) >= t) {
         const uint4 q = load_unit(p + u);
-        float v[E];
-        Elem<T>::unpack(q, v);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t o = order_of(v[e]);
-          if (o >= t) {
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kCand) sh.cand[at] = key_of(o, row.head + u * E + e);
+        const float mx = Elem<T>::widen_max(Elem<T>::max2(Elem<T>::max2(q.x, q.y), Elem<T>::max2(q.z, q.w)));
+        if (order_of(mx) >= t) {
+          const int at = atomicAdd(&sh.hits, 1);
+          if (at < kHits) {
+            sh.hit[at] = q;
+            sh.hit_unit[at] = u;
           }
         }
       }
     }
   }
   __syncthreads();
-  int n = sh.count;
+  const int hits = min(sh.hits, kHits);
+  if (tid < ragged) push(order_of(Elem<T>::load(row.z + row.ragged_index(tid))), row.ragged_index(tid));
+  for (int i = tid; i < hits * E; i += NT)
+    push(order_of(Elem<T>::load(reinterpret_cast<const T*>(sh.hit) + i)), row.head + sh.hit_unit[i / E] * E + i % E);
+  __syncthreads();
+  int n = sh.hits > kHits ? kCand + 1 : sh.count;
   __syncthreads();
   if (n > kCand) {
     // The want-th value over all elements: count(>= lo) >= want and count(> hi) < want throughout.
@@ -175,12 +211,12 @@ __device__ void select_top(const Row<T>& row, int u0, int u1, int ragged, float 
       const bool in = idx < unit_end || (idx >= tail && idx < end);
       const bool tie = in && order_of(Elem<T>::load(row.z + idx)) == a;
       const uint32_t vote = __ballot_sync(0xffffffffu, tie);
-      if (lane == 0) sh.warp_sum[warp] = __popc(vote);
+      if (lane == 0) sh.sums[warp] = __popc(vote);
       __syncthreads();
       int before = taken, sum = 0;
       for (int w = 0; w < NT / 32; ++w) {
-        if (w < warp) before += sh.warp_sum[w];
-        sum += sh.warp_sum[w];
+        if (w < warp) before += sh.sums[w];
+        sum += sh.sums[w];
       }
       const int at = before + __popc(vote & ((1u << lane) - 1u));
       if (tie && at < want) sh.cand[at] = key_of(a, idx);
@@ -217,67 +253,134 @@ __device__ void select_top(const Row<T>& row, int u0, int u1, int ragged, float 
   for (int i = tid; i < n; i += NT) {
     const unsigned long long ki = sh.cand[i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += sh.cand[j] > ki;
-    if (rank < want) sh.sorted[rank] = ki;
+    int j = 0;
+#pragma unroll 4
+    for (; j + 1 < n; j += 2) {
+      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&sh.cand[j]);
+      rank += (two.x > ki) + (two.y > ki);
+    }
+    if (j < n) rank += sh.cand[j] > ki;
+    if (rank < want) emit(rank, ki);
   }
-  __syncthreads();
 }
 
 // --------------------------------------------------- log probabilities
 
-// One block per row: statistics in one pass, then the alternatives.
-template <typename T, int NT, bool TOPK>
-__global__ void __launch_bounds__(NT) logprob_forward_kernel(const T* __restrict__ logits, long long ld, int V,
-                                                             const int64_t* __restrict__ tokens, int64_t ignore_index,
-                                                             float c, float inv_t, int k, float* __restrict__ logprobs,
-                                                             float* __restrict__ entropy, float* __restrict__ stats,
-                                                             float* __restrict__ top_logprobs,
-                                                             int64_t* __restrict__ top_ids) {
-  const int row_i = blockIdx.x, tid = threadIdx.x;
+// A block per row, or with SPLIT a cluster of blocks that share it: statistics
+// in one pass, then the alternatives. The blocks of a cluster select their own
+// alternatives, and the first block merges the sorted lists.
+template <typename T, int NT, bool TOPK, bool SPLIT>
+__global__ void __launch_bounds__(NT)
+    logprob_forward_kernel(const T* __restrict__ logits, long long ld, int V, const int64_t* __restrict__ tokens,
+                           int64_t ignore_index, float c, float inv_t, int k, float* __restrict__ logprobs,
+                           float* __restrict__ entropy, float* __restrict__ stats, float* __restrict__ top_logprobs,
+                           int64_t* __restrict__ top_ids) {
+  namespace cg = cooperative_groups;
+  const int tid = threadIdx.x;
+  int part = 0, parts = 1;
+  if constexpr (SPLIT) {
+    part = (int)cg::this_cluster().block_rank();
+    parts = (int)cg::this_cluster().num_blocks();
+  }
+  const long long row_i = SPLIT ? blockIdx.x / parts : blockIdx.x;
   const int64_t token = tokens ? tokens[row_i] : 0;
   if (tokens && token == ignore_index) {
-    if (tid == 0) {
-      logprobs[row_i] = 0.f;
-      entropy[row_i] = 0.f;
-      stats[kStats * (long long)row_i] = 0.f;
-      stats[kStats * (long long)row_i + 1] = 0.f;
-    }
-    if (TOPK) {
-      for (int i = tid; i < k; i += NT) {
-        top_logprobs[(long long)row_i * k + i] = 0.f;
-        top_ids[(long long)row_i * k + i] = -1;
+    if (part == 0) {
+      if (tid == 0) {
+        logprobs[row_i] = 0.f;
+        entropy[row_i] = 0.f;
+        stats[kStats * row_i] = 0.f;
+        stats[kStats * row_i + 1] = 0.f;
+      }
+      for (int i = tid; TOPK && i < k; i += NT) {
+        top_logprobs[row_i * k + i] = 0.f;
+        top_ids[row_i * k + i] = -1;
       }
     }
     return;
   }
-  const Row<T> row(logits + (long long)row_i * ld, V);
-  Acc acc;
-  if (tid < row.ragged) {
-    const float v = Elem<T>::load(row.z + row.ragged_index(tid));
-    const float ms = acc.raise<true>(v, c);
-    acc.add<true>(v, ms, c);
+  const Row<T> row(logits + row_i * ld, V);
+  int u0, u1;
+  segment(row.units, part, parts, u0, u1);
+  const int ragged = part == 0 ? row.ragged : 0;
+  Run<true> run;
+  float mine = -INFINITY;
+  if (tid < 32) {  // fewer than two units of ragged elements
+    mine = tid < ragged ? Elem<T>::load(row.z + row.ragged_index(tid)) : -INFINITY;
+    run.add_one(mine, c);
   }
-  stream_units<T, NT, true, false>(row.unit_ptr(), 0, row.units, c, acc, nullptr);
-  __shared__ float join_sm[32][3];
-  const Acc all = block_join<NT, true>(acc, c, join_sm);
+  __shared__ Acc join_sm[NT / 32], result;
+  __shared__ std::conditional_t<TOPK, SelectShared<NT>, int> sh;
+  stream_units<T, NT, true, false>(row.unit_ptr(), u0, u1, c, run, nullptr, [&](int batch, float mx) {
+    if constexpr (TOPK) {
+      mine = max_nan(mine, mx);
+      float& kept = sh.group_max[batch % sh.kGroups][tid];
+      kept = batch < sh.kGroups ? mx : max_nan(kept, mx);
+    }
+  });
+  Acc all = block_join<NT, true>(run, c, join_sm);
+  if constexpr (SPLIT) {
+    __shared__ unsigned long long sorted[TOPK ? kMaxList : 1];
+    if (tid == 0) result = all;
+    if constexpr (TOPK) {
+      for (int i = tid; i < k; i += NT) sorted[i] = 0;  // below every key
+      select_top<T, NT>(row, u0, u1, ragged, mine, k, sh,
+                        [&](int place, unsigned long long key) { sorted[place] = key; });
+    }
+    cg::this_cluster().sync();
+    if (part == 0) {
+      if (tid < 32) {
+        all = *cg::this_cluster().map_shared_rank(&result, (tid & 7) < parts ? tid & 7 : 0);
+        if ((tid & 7) >= parts) all = Acc();
+        all = join_lanes<8, true>(all, c);
+      }
+      if constexpr (TOPK) {
+        for (int i = tid; i < parts * k; i += NT) sh.cand[i] = *cg::this_cluster().map_shared_rank(&sorted[i % k], i / k);
+      }
+    }
+    cg::this_cluster().sync();  // the other blocks' shared memory is not needed any more
+    if (part != 0) return;
+  }
   // Log probabilities are taken in units of z / T, not of c z: (lowest - m) c would overflow.
-  const float log2s = log2f(all.s), ln_s = kLn2 * log2s;
   if (tid == 0) {
+    const float log2s = log2f(all.s);
     if (tokens) {
       const bool inside = token >= 0 && token < V;
-      logprobs[row_i] = inside ? (Elem<T>::load(row.z + token) - all.m) * inv_t - ln_s : NAN;
+      logprobs[row_i] = inside ? (Elem<T>::load(row.z + token) - all.m) * inv_t - kLn2 * log2s : NAN;
     }
     entropy[row_i] = kLn2 * (log2s - all.a / all.s);
-    stats[kStats * (long long)row_i] = all.m;
-    stats[kStats * (long long)row_i + 1] = log2s;
+    stats[kStats * row_i] = all.m;
+    stats[kStats * row_i + 1] = log2s;
+    if (TOPK) {
+      result.m = all.m;
+      result.s = kLn2 * log2s;
+    }
   }
   if constexpr (TOPK) {
-    __shared__ SelectShared sh;
-    select_top<T, NT>(row, 0, row.units, row.ragged, acc.m, k, sh);
-    for (int i = tid; i < k; i += NT) {
-      const unsigned long long key = sh.sorted[i];
-      top_ids[(long long)row_i * k + i] = (int64_t)(uint32_t)~(uint32_t)key;
-      top_logprobs[(long long)row_i * k + i] = (value_of((uint32_t)(key >> 32)) - all.m) * inv_t - ln_s;
+    auto emit = [&](int place, unsigned long long key) {
+      top_ids[row_i * k + place] = (int64_t)(uint32_t)~(uint32_t)key;
+      top_logprobs[row_i * k + place] = (value_of((uint32_t)(key >> 32)) - result.m) * inv_t - result.s;
+    };
+    if constexpr (SPLIT) {
+      __syncthreads();
+      // A key's place is its place in its own list and the number of larger keys in the others.
+      for (int i = tid; i < parts * k; i += NT) {
+        const unsigned long long key = sh.cand[i];
+        int place = i % k;
+        for (int other = 0; other < parts; ++other) {
+          if (other == i / k) continue;
+          int lo = 0, hi = k;  // keys before lo are larger, from hi on smaller
+          while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (sh.cand[other * k + mid] > key) lo = mid + 1;
+            else hi = mid;
+          }
+          place += lo;
+        }
+        if (key != 0 && place < k) emit(place, key);
+      }
+    } else {
+      select_top<T, NT>(row, u0, u1, ragged, mine, k, sh, emit);
     }
   }
 }
@@ -290,28 +393,45 @@ __global__ void __launch_bounds__(NT)
                             const int64_t* __restrict__ tokens, int64_t ignore_index, float c, float inv_t,
                             const float* __restrict__ stats, const float* __restrict__ entropy,
                             const float* __restrict__ dlogprobs, const float* __restrict__ dentropy) {
-  const int row_i = blockIdx.x;
+  const long long row_i = gridDim.x - 1 - blockIdx.x;  // last rows first: the forward pass left them in L2
   const int64_t token = tokens ? tokens[row_i] : -1;
   float g = dlogprobs ? dlogprobs[row_i] : 0.f;
   const float gh = dentropy ? dentropy[row_i] : 0.f;
   int u0, u1;
   if ((tokens && token == ignore_index) || (g == 0.f && gh == 0.f)) {
-    const Row<T> row(out + (long long)row_i * ld_out, V);
+    const Row<T> row(out + row_i * ld_out, V);
     segment(row.units, blockIdx.y, gridDim.y, u0, u1);
     zero_row<T, NT>(row, u0, u1, blockIdx.y == 0 ? row.ragged : 0);
     return;
   }
   if (token < 0 || token >= V) g = g == 0.f ? 0.f : NAN;  // its log probability is NaN too
-  const Row<T> row(logits + (long long)row_i * ld, V);
+  const Row<T> row(logits + row_i * ld, V);
   segment(row.units, blockIdx.y, gridDim.y, u0, u1);
-  const float m = stats[kStats * (long long)row_i], log2s = stats[kStats * (long long)row_i + 1];
+  const float m = stats[kStats * row_i], log2s = stats[kStats * row_i + 1];
   const float a = -(g + gh * entropy[row_i]) * inv_t, b = -gh * kLn2 * inv_t, hot = g * inv_t;
   const int at = (int)token;
-  map_row<T, NT>(row, out + (long long)row_i * ld_out, u0, u1, blockIdx.y == 0 ? row.ragged : 0, [&](float z, int j) {
-    const float y = (z - m) * c - log2s;
-    const float d = ex2(y) * fmaf(b, fmaxf(y, -256.f), a);
-    return j == at ? d + hot : d;
-  });
+  T* o = out + row_i * ld_out;
+  const int ragged = blockIdx.y == 0 ? row.ragged : 0;
+  const F2 minus_m = pair(-m, -m), cc = pair(c, c), ml = pair(-log2s, -log2s), aa = pair(a, a), bb = pair(b, b);
+  auto given = [&](F2 d, int j) {
+    if ((unsigned)(at - j) < 2u) {
+      const float2 s = split(d);
+      d = at == j ? pair(s.x + hot, s.y) : pair(s.x, s.y + hot);
+    }
+    return d;
+  };
+  if (b == 0.f) {
+    map_row<T, NT>(row, o, u0, u1, ragged, [&](F2 z, int j) {
+      const float2 y = split(fma2(add2(z, minus_m), cc, ml));
+      return given(mul2(pair(ex2(y.x), ex2(y.y)), aa), j);
+    });
+  } else {
+    map_row<T, NT>(row, o, u0, u1, ragged, [&](F2 z, int j) {
+      float2 y = split(fma2(add2(z, minus_m), cc, ml));
+      const F2 p = pair(ex2(y.x), ex2(y.y));
+      return given(mul2(p, fma2(bb, pair(fmaxf(y.x, -256.f), fmaxf(y.y, -256.f)), aa)), j);  // 0 (-inf) is 0 here
+    });
+  }
 }
 
 }  // namespace
@@ -346,13 +466,17 @@ void token_logprobs_forward(const at::Tensor& logits, const c10::optional<at::Te
   int64_t* ti = top_ids ? top_ids->data_ptr<int64_t>() : nullptr;
   for_logits_type(logits.scalar_type(), [&](auto tag) {
     using T = typename decltype(tag)::type;
-    auto launch = [&](auto kern, int nt) {
-      kern<<<(unsigned)rows, nt, 0, s>>>((const T*)logits.data_ptr(), logits.stride(0), (int)vocab, tok, ignore_index,
-                                         c, (float)(1.0 / temperature), k, lp, entropy.data_ptr<float>(), stats.data_ptr<float>(), tl, ti);
+    auto launch = [&](auto kern, int nt, int parts) {
+      launch_rows(kern, rows, nt, parts, 0, s, (const T*)logits.data_ptr(), (long long)logits.stride(0), (int)vocab, tok,
+                  ignore_index, c, (float)(1.0 / temperature), k, lp, entropy.data_ptr<float>(),
+                  stats.data_ptr<float>(), tl, ti);
     };
-    const bool small = vocab * (int64_t)sizeof(T) <= 8192;
-    if (small) k ? launch(logprob_forward_kernel<T, 128, true>, 128) : launch(logprob_forward_kernel<T, 128, false>, 128);
-    else k ? launch(logprob_forward_kernel<T, 512, true>, 512) : launch(logprob_forward_kernel<T, 512, false>, 512);
+    const int nt = getenv("KB_NT") ? atoi(getenv("KB_NT")) : 256;
+    const int parts = row_parts(rows, vocab * (int64_t)sizeof(T), logits.get_device());
+    if (parts > 1) k ? launch(logprob_forward_kernel<T, 256, true, true>, 256, parts) : launch(logprob_forward_kernel<T, 256, false, true>, 256, parts);
+    else if (nt == 128) k ? launch(logprob_forward_kernel<T, 128, true, false>, 128, 1) : launch(logprob_forward_kernel<T, 128, false, false>, 128, 1);
+    else if (nt == 256) k ? launch(logprob_forward_kernel<T, 256, true, false>, 256, 1) : launch(logprob_forward_kernel<T, 256, false, false>, 256, 1);
+    else k ? launch(logprob_forward_kernel<T, 512, true, false>, 512, 1) : launch(logprob_forward_kernel<T, 512, false, false>, 512, 1);
   });
   KB_LAUNCHED();
 }

@@ -14,10 +14,12 @@
 #pragma once
 
 #include <ATen/ATen.h>
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "host_utils.h"
 
@@ -135,6 +137,34 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
+// Pairs of fp32 values in one 64-bit register: one instruction per two elements.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pair(float a, float b) {
+  F2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 split(F2 v) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+  return d;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
 // A row cut for 16-byte access: `head` elements before the first 16-byte
 // boundary, `units` whole units, the rest behind them. The (fewer than two
 // units of) elements outside whole units are the row's ragged ones.
@@ -155,28 +185,12 @@ struct Row {
   }
 };
 
-// Running statistics of the elements a thread has seen.
+constexpr int kBatch = 4;  // units of a thread's batch of loads
+
+// Statistics of a set of elements: maximum, S and A (see above).
 struct Acc {
   float m = -INFINITY, s = 0.f, a = 0.f;
-  // Takes the maximum up to `mx` and returns the finite value to subtract.
-  template <bool ENT>
-  __device__ __forceinline__ float raise(float mx, float c) {
-    const float mn = max_nan(m, mx);
-    const float x = (m - mn) * c;
-    const float f = (m == mn) ? 1.f : ex2(x);
-    if (ENT) a = f * (a + s * fmaxf(x, -1e30f));  // s is 0 where x is -inf
-    s *= f;
-    m = mn;
-    return mn == -INFINITY ? 0.f : mn;
-  }
-  template <bool ENT>
-  __device__ __forceinline__ void add(float z, float ms, float c) {
-    const float x = (z - ms) * c;
-    const float e = ex2(x);
-    s += e;
-    if (ENT) a = fmaf(e, fmaxf(x, -256.f), a);  // 2^-256 is 0: a masked entry adds 0, not 0 * inf
-  }
-  // Joins another thread's statistics.
+  // Joins another set's statistics.
   template <bool ENT>
   __device__ __forceinline__ void join(float m2, float s2, float a2, float c) {
     const float mn = max_nan(m, m2);
@@ -191,12 +205,80 @@ struct Acc {
   }
 };
 
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float d;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
+  return d;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Running statistics of a warp's elements. The maximum is the warp's, so it
+// rarely grows and the lanes' sums need no rescaling when they are joined;
+// each lane holds its sums as two halves.
+template <bool ENT>
+struct Run {
+  float m = -INFINITY, ms = 0.f;  // maximum, and the finite value to subtract
+  F2 s = 0, a = 0;
+  // Takes the maximum up to the lanes' `wide`; called by whole warps.
+  __device__ __forceinline__ void raise(float wide, float c) {
+    if (!__any_sync(0xffffffffu, !(wide <= m))) return;
+    const float mn = max_nan(m, warp_max_nan(wide));
+    const float x = (m - mn) * c;
+    const float f = (m == mn) ? 1.f : ex2(x);
+    const F2 ff = pair(f, f);
+    if (ENT) {
+      const float y = fmaxf(x, -1e30f);  // the sum is 0 where x is -inf
+      a = mul2(ff, fma2(s, pair(y, y), a));
+    }
+    s = mul2(s, ff);
+    m = mn;
+    ms = mn == -INFINITY ? 0.f : mn;
+  }
+  __device__ __forceinline__ void add(F2 z, F2 minus_ms, F2 c) {
+    const F2 x = mul2(add2(z, minus_ms), c);
+    const float2 xs = split(x);
+    const F2 e = pair(ex2(xs.x), ex2(xs.y));
+    s = add2(s, e);
+    if (ENT) a = fma2(e, x, a);
+  }
+  // The same for A alone, with 2^-inf (-inf) = 0.
+  __device__ __forceinline__ void add_masked(F2 z, F2 minus_ms, F2 c) {
+    const float2 xs = split(mul2(add2(z, minus_ms), c));
+    a = fma2(pair(ex2(xs.x), ex2(xs.y)), pair(fmaxf(xs.x, -256.f), fmaxf(xs.y, -256.f)), a);
+  }
+  // One element per lane (-inf for none); called by whole warps.
+  __device__ __forceinline__ void add_one(float z, float c) {
+    raise(z, c);
+    const float x = (z - ms) * c, e = ex2(x);
+    s = add2(s, pair(e, 0.f));
+    if (ENT) a = fma2(pair(e, 0.f), pair(fmaxf(x, -256.f), 0.f), a);
+  }
+  // The warp's statistics, in every lane.
+  __device__ __forceinline__ Acc total() const {
+    Acc r;
+    r.m = m;
+    const float2 ss = split(s), aa = split(a);
+    r.s = warp_sum(ss.x + ss.y);
+    r.a = ENT ? warp_sum(aa.x + aa.y) : 0.f;
+    return r;
+  }
+};
+
 __device__ __forceinline__ uint4 load_unit(const uint4* p) {
   uint4 q;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
                : "l"(p));
   return q;
+}
+
+__device__ __forceinline__ void store_unit(uint4* p, const uint4& q) {
+  asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w)
+               : "memory");
 }
 
 // Masks the elements of unit `u` whose bit is set (bit = u * E + j).
@@ -220,12 +302,21 @@ __device__ __forceinline__ void mask_unit(uint4& q, const uint8_t* bits, int u) 
   }
 }
 
-// Statistics of the units [u0, u1) of a row over the threads of a block,
-// four 16-byte loads in flight per thread.
-template <typename T, int NT, bool ENT, bool MASK>
-__device__ __forceinline__ void stream_units(const uint4* p, int u0, int u1, float c, Acc& acc, const uint8_t* bits) {
-  constexpr int UN = 4, E = Elem<T>::kUnit;
-  for (int u = u0 + (int)threadIdx.x; u < u1; u += UN * NT) {
+// Statistics of the units [u0, u1) of a row over the threads of a block, in
+// batches of four 16-byte loads per thread (unit u0 + tid + (4 b + i) NT is the
+// i-th of batch b); batch_max(b, m) gets each batch's maximum. Per element: widening, half a packed
+// maximum, and in pairs a subtraction, a product, two 2^x and one or two sums.
+// Clamping the masked entries' exponents would cost one more instruction per
+// element; instead a batch whose A came out NaN (0 times -inf) takes its A again.
+template <typename T, int NT, bool ENT, bool MASK, typename G>
+__device__ __forceinline__ void stream_units(const uint4* p, int u0, int u1, float c, Run<ENT>& run,
+                                             const uint8_t* bits, const G& batch_max) {
+  static_assert(!(ENT && MASK), "the masked form takes no entropy");
+  constexpr int UN = kBatch, E = Elem<T>::kUnit;
+  const F2 cc = pair(c, c);
+  int batch = 0;
+  for (int base = u0 + (int)(threadIdx.x & ~31u); base < u1; base += UN * NT, ++batch) {  // whole warps
+    const int u = base + (int)(threadIdx.x & 31);
     uint4 q[UN];
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
@@ -244,60 +335,84 @@ __device__ __forceinline__ void stream_units(const uint4* p, int u0, int u1, flo
 #pragma unroll
     for (int i = 1; i < UN; ++i)
       mx = Elem<T>::max2(mx, Elem<T>::max2(Elem<T>::max2(q[i].x, q[i].y), Elem<T>::max2(q[i].z, q[i].w)));
-    const float ms = acc.raise<ENT>(Elem<T>::widen_max(mx), c);
+    const float wide = Elem<T>::widen_max(mx);
+    batch_max(batch, wide);
+    run.raise(wide, c);
+    const F2 mm = pair(-run.ms, -run.ms);
+    const F2 a_before = run.a;
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
       if (u + i * NT < u1) {
         float v[E];
         Elem<T>::unpack(q[i], v);
 #pragma unroll
-        for (int j = 0; j < E; ++j) acc.add<ENT>(v[j], ms, c);
+        for (int j = 0; j < E; j += 2) run.add(pair(v[j], v[j + 1]), mm, cc);
+      }
+    }
+    if (ENT) {
+      const float2 aa = split(run.a);
+      if (!(aa.x + aa.y == aa.x + aa.y)) {
+        run.a = a_before;
+#pragma unroll 1
+        for (int i = 0; i < UN; ++i) {
+          if (u + i * NT < u1) {
+            float v[E];
+            Elem<T>::unpack(load_unit(p + u + i * NT), v);
+#pragma unroll
+            for (int j = 0; j < E; j += 2) run.add_masked(pair(v[j], v[j + 1]), mm, cc);
+          }
+        }
       }
     }
   }
 }
 
-// Joins the statistics of a block's threads; every thread returns with them.
-template <int NT, bool ENT>
-__device__ __forceinline__ Acc block_join(Acc acc, float c, float (*sm)[3]) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, acc.m, o);
-    const float s2 = __shfl_xor_sync(0xffffffffu, acc.s, o);
-    const float a2 = ENT ? __shfl_xor_sync(0xffffffffu, acc.a, o) : 0.f;
-    acc.join<ENT>(m2, s2, a2, c);
-  }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) {
-    sm[warp][0] = acc.m;
-    sm[warp][1] = acc.s;
-    sm[warp][2] = acc.a;
-  }
-  __syncthreads();
-  constexpr int NW = NT / 32;
+// Joins statistics held by the first N lanes of a warp (N a power of two); every lane returns with them.
+template <int N, bool ENT>
+__device__ __forceinline__ Acc join_lanes(Acc v, float c) {
   Acc r;
-  const int w = lane & (NW - 1);
-  r.m = sm[w][0];
-  r.s = sm[w][1];
-  r.a = sm[w][2];
+  const bool mine = (int)(threadIdx.x & 31) < N;
+  r.m = warp_max_nan(mine ? v.m : -INFINITY);
+  const float x = (v.m - r.m) * c, f = v.m == r.m ? 1.f : ex2(x);
+  float s = mine ? v.s * f : 0.f, a = 0.f;
+  if (ENT) a = mine ? f * (v.a + v.s * (v.m == r.m ? 0.f : fmaxf(x, -1e30f))) : 0.f;
 #pragma unroll
-  for (int o = NW / 2; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, r.m, o);
-    const float s2 = __shfl_xor_sync(0xffffffffu, r.s, o);
-    const float a2 = ENT ? __shfl_xor_sync(0xffffffffu, r.a, o) : 0.f;
-    r.join<ENT>(m2, s2, a2, c);
+  for (int o = N / 2; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (ENT) a += __shfl_xor_sync(0xffffffffu, a, o);
   }
+  r.s = __shfl_sync(0xffffffffu, s, 0);
+  r.a = ENT ? __shfl_sync(0xffffffffu, a, 0) : 0.f;
   return r;
 }
 
-// Writes a row's units [u0, u1) and, for the first segment, its ragged elements: out = f(z, index).
+// Joins the statistics of a block's warps; the first warp returns with them.
+template <int NT, bool ENT>
+__device__ __forceinline__ Acc block_join(const Run<ENT>& run, float c, Acc* sm) {
+  const Acc w = run.total();
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = w;
+  __syncthreads();
+  Acc r;
+  if (threadIdx.x < 32) r = join_lanes<NT / 32, ENT>(sm[threadIdx.x & (NT / 32 - 1)], c);
+  return r;
+}
+
+// Units of part `i` of `n`; the first part also takes the ragged elements.
+__device__ __forceinline__ void segment(int units, int i, int n, int& u0, int& u1) {
+  const int per = (units + n - 1) / n;
+  u0 = min(units, i * per);
+  u1 = min(units, u0 + per);
+}
+
+// Writes a row's units [u0, u1) and, for the first segment, its ragged
+// elements: out = f(two elements, the index of the first).
 template <typename T, int NT, typename F>
 __device__ __forceinline__ void map_row(const Row<T>& row, T* out, int u0, int u1, int ragged, const F& f) {
   constexpr int UN = 4, E = Elem<T>::kUnit;
   const bool same = ((reinterpret_cast<uintptr_t>(row.z) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
   if ((int)threadIdx.x < ragged) {
     const int idx = row.ragged_index(threadIdx.x);
-    Elem<T>::store(out + idx, f(Elem<T>::load(row.z + idx), idx));
+    Elem<T>::store(out + idx, split(f(pair(Elem<T>::load(row.z + idx), 0.f), idx)).x);
   }
   const uint4* p = row.unit_ptr();
   for (int u = u0 + (int)threadIdx.x; u < u1; u += UN * NT) {
@@ -312,9 +427,13 @@ __device__ __forceinline__ void map_row(const Row<T>& row, T* out, int u0, int u
         float v[E];
         Elem<T>::unpack(q[i], v);
 #pragma unroll
-        for (int j = 0; j < E; ++j) v[j] = f(v[j], idx + j);
+        for (int j = 0; j < E; j += 2) {
+          const float2 d = split(f(pair(v[j], v[j + 1]), idx + j));
+          v[j] = d.x;
+          v[j + 1] = d.y;
+        }
         if (same) {
-          *reinterpret_cast<uint4*>(out + idx) = Elem<T>::pack(v);
+          store_unit(reinterpret_cast<uint4*>(out + idx), Elem<T>::pack(v));
         } else {
 #pragma unroll
           for (int j = 0; j < E; ++j) Elem<T>::store(out + idx + j, v[j]);
@@ -329,14 +448,7 @@ __device__ __forceinline__ void zero_row(const Row<T>& out, int u0, int u1, int 
   T* o = const_cast<T*>(out.z);
   if ((int)threadIdx.x < ragged) Elem<T>::store(o + out.ragged_index(threadIdx.x), 0.f);
   uint4* p = const_cast<uint4*>(out.unit_ptr());
-  for (int u = u0 + (int)threadIdx.x; u < u1; u += NT) p[u] = make_uint4(0, 0, 0, 0);
-}
-
-// Units of segment `seg` of `nseg`; the first segment also takes the ragged elements.
-__device__ __forceinline__ void segment(int units, int seg, int nseg, int& u0, int& u1) {
-  const int per = (units + nseg - 1) / nseg;
-  u0 = min(units, seg * per);
-  u1 = min(units, u0 + per);
+  for (int u = u0 + (int)threadIdx.x; u < u1; u += NT) store_unit(p + u, make_uint4(0, 0, 0, 0));
 }
 
 // ------------------------------------------------------------------ host
@@ -384,6 +496,30 @@ void check_out(const at::Tensor& out, const at::Tensor& logits, int64_t vocab) {
   KB_CHECK(out.dim() == 2 && out.size(0) == logits.size(0) && out.size(1) >= vocab, "out must be [rows, vocab]");
   KB_CHECK(out.size(1) == 1 || out.stride(1) == 1, "out must have unit inner stride");
   KB_CHECK(out.size(0) <= 1 || out.stride(0) >= vocab, "rows of out overlap");
+}
+
+// Blocks that share a row: clusters of up to 8 where rows alone leave the device idle, of at least 16 KB each.
+int row_parts(int64_t rows, int64_t row_bytes, int device) {
+  int parts = 1;
+  while (parts < 8 && rows * parts * 2 <= 2 * (int64_t)num_sms(device) && row_bytes >= parts * 2 * 16384) parts *= 2;
+  return parts;
+}
+
+template <typename... P, typename... A>
+void launch_rows(void (*kern)(P...), int64_t rows, int threads, int parts, size_t smem, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * parts));
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)parts;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
+  KB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...));
 }
 
 int row_segments(int64_t rows, int64_t vocab, int64_t elem, int threads, int device) {

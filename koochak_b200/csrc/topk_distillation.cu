@@ -34,17 +34,6 @@ __device__ __forceinline__ bool read_slots(const T* z, int V, const int64_t* ids
   return __syncthreads_or(any);
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-__device__ __forceinline__ float warp_max_nan(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-
 // What a row's gradient needs besides its logits:
 // dz_j = g (coef 2^((z_j - ms) c)) off the list, g (Q p_j - sum of its q) on it, p_j = 2^((z_j - m) c) inv_s.
 struct KdStats {
@@ -125,7 +114,7 @@ __global__ void __launch_bounds__(NT)
                            float* __restrict__ stats) {
   extern __shared__ __align__(16) uint8_t bits[];
   __shared__ ListShared sh;
-  __shared__ float join_sm[32][3];
+  __shared__ Acc join_sm[NT / 32];
   constexpr int E = Elem<T>::kUnit;
   const int tid = threadIdx.x;
   const long long row_i = blockIdx.x;
@@ -140,7 +129,7 @@ __global__ void __launch_bounds__(NT)
     if (tid < kStats) stats[row_i * kStats + tid] = 0.f;
     return;
   }
-  Acc acc;
+  Run<false> run;
   if (TAIL) {
     // Bit u * E + j for element j of unit u, ragged elements behind the units.
     for (int i = tid; i < K; i += NT) {
@@ -153,16 +142,13 @@ __global__ void __launch_bounds__(NT)
     }
     __syncthreads();
   }
-  if (tid < row.ragged) {
+  if (tid < 32) {  // fewer than two units of ragged elements
     const int bit = row.units * E + tid;
-    if (!TAIL || !((bits[bit >> 3] >> (bit & 7)) & 1u)) {
-      const float v = Elem<T>::load(row.z + row.ragged_index(tid));
-      const float ms = acc.raise<false>(v, c);
-      acc.add<false>(v, ms, c);
-    }
+    const bool in = tid < row.ragged && (!TAIL || !((bits[bit >> 3] >> (bit & 7)) & 1u));
+    run.add_one(in ? Elem<T>::load(row.z + row.ragged_index(tid)) : -INFINITY, c);
   }
-  stream_units<T, NT, false, TAIL>(row.unit_ptr(), 0, row.units, c, acc, bits);
-  const Acc all = block_join<NT, false>(acc, c, join_sm);
+  stream_units<T, NT, false, TAIL>(row.unit_ptr(), 0, row.units, c, run, bits, [](int, float) {});
+  const Acc all = block_join<NT, false>(run, c, join_sm);
   if (tid < 32) {
     const KdStats r = distill_row<TAIL>(all, c, inv_t, K, sh);
     if (tid == 0) {
@@ -204,7 +190,7 @@ __global__ void __launch_bounds__(NT)
                             const float* __restrict__ scale) {
   constexpr int E = Elem<T>::kUnit;
   __shared__ ListShared sh;
-  const long long row_i = blockIdx.x;
+  const long long row_i = gridDim.x - 1 - blockIdx.x;  // last rows first: the forward pass left them in L2
   const float* s = stats + row_i * kStats;
   const float w = row_scale ? row_scale[row_i] : 1.f;
   T* o = out + row_i * ld_out;
@@ -230,7 +216,11 @@ __global__ void __launch_bounds__(NT)
   for (int i = threadIdx.x; i < K; i += NT) sh.q[i] = ex2((sh.t[i] - r.t_max) * (TAIL ? kLog2e : c)) * r.inv_e;
   const float dense = g * r.coef;
   const int ragged = blockIdx.y == 0 ? row.ragged : 0;
-  map_row<T, NT>(row, o, u0, u1, ragged, [&](float z, int) { return dense * ex2((z - r.ms) * c); });
+  const F2 minus_m = pair(-r.ms, -r.ms), cc = pair(c, c), dd = pair(dense, dense);
+  map_row<T, NT>(row, o, u0, u1, ragged, [&](F2 z, int) {
+    const float2 x = split(mul2(add2(z, minus_m), cc));
+    return mul2(pair(ex2(x.x), ex2(x.y)), dd);
+  });
   __syncthreads();
   write_listed<T, NT, TAIL>(o, sh, K, c, g, r, row.head + u0 * E, row.head + u1 * E, blockIdx.y == 0, row.head,
                             row.head + row.units * E);
@@ -265,8 +255,9 @@ void topk_distillation_forward(const at::Tensor& logits, const at::Tensor& ids, 
                                             ids.data_ptr<int64_t>(), teacher.data_ptr<float>(), k, c,
                                             (float)(1.0 / temperature), loss.data_ptr<float>(), stats.data_ptr<float>());
     };
-    const bool small = vocab * (int64_t)sizeof(T) <= 8192;
-    if (small) tail ? launch(distill_forward_kernel<T, 128, true>, 128) : launch(distill_forward_kernel<T, 128, false>, 128);
+    const int nt = getenv("KB_NT") ? atoi(getenv("KB_NT")) : 512;
+    if (nt == 128) tail ? launch(distill_forward_kernel<T, 128, true>, 128) : launch(distill_forward_kernel<T, 128, false>, 128);
+    else if (nt == 256) tail ? launch(distill_forward_kernel<T, 256, true>, 256) : launch(distill_forward_kernel<T, 256, false>, 256);
     else tail ? launch(distill_forward_kernel<T, 512, true>, 512) : launch(distill_forward_kernel<T, 512, false>, 512);
   });
   KB_LAUNCHED();

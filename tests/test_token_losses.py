@@ -640,8 +640,13 @@ def test_offsets_beyond_32_bits():
     tok[-3:] = torch.tensor([5, 70000, 131071], device=DEV)
     res = kf.token_logprobs(z, tok, top_k=9)
     small = kf.token_logprobs(z[-3:].clone(), tok[-3:], top_k=9)
-    for a, b in zip(res, small):
-        assert torch.equal(a[-3:], b)
+    # Few rows are shared by several blocks, so their sums are added in another order: each of the two results is within
+    # its tolerance of the exact value, and they are within twice that of one another. The alternatives are equal.
+    assert torch.equal(res.top_ids[-3:], small.top_ids)
+    for a, b in ((res.logprobs, small.logprobs), (res.top_logprobs, small.top_logprobs)):
+        _close(a[-3:], b, 2 * _logprob_tol(b.double()), "log probabilities")
+    tol = 2 * ((small.entropy.double() + math.log(vocab)) * 2.0**-20 + 2.0**-19)
+    _close(res.entropy[-3:], small.entropy, tol, "entropy")
     assert not res.logprobs[:-3].any()
     ids, t = res.top_ids, res.top_logprobs
     loss, stats = kf.topk_distillation_forward(z, ids, t, tail=True)
