@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(NT)
   }
   __shared__ Acc join_sm[NT / 32], result;
   __shared__ std::conditional_t<TOPK, SelectShared<NT>, int> sh;
-  stream_units<T, NT, true, false>(row.unit_ptr(), u0, u1, c, run, nullptr, [&](int batch, float mx) {
+  stream_units<T, NT, true, false>(FromMemory{row.unit_ptr()}, u0, u1, c, run, nullptr, [&](int batch, float mx) {
     if constexpr (TOPK) {
       mine = max_nan(mine, mx);
       float& kept = sh.group_max[batch % sh.kGroups][tid];
@@ -466,17 +466,15 @@ void token_logprobs_forward(const at::Tensor& logits, const c10::optional<at::Te
   int64_t* ti = top_ids ? top_ids->data_ptr<int64_t>() : nullptr;
   for_logits_type(logits.scalar_type(), [&](auto tag) {
     using T = typename decltype(tag)::type;
-    auto launch = [&](auto kern, int nt, int parts) {
-      launch_rows(kern, rows, nt, parts, 0, s, (const T*)logits.data_ptr(), (long long)logits.stride(0), (int)vocab, tok,
-                  ignore_index, c, (float)(1.0 / temperature), k, lp, entropy.data_ptr<float>(),
-                  stats.data_ptr<float>(), tl, ti);
-    };
-    const int nt = getenv("KB_NT") ? atoi(getenv("KB_NT")) : 256;
-    const int parts = row_parts(rows, vocab * (int64_t)sizeof(T), logits.get_device());
-    if (parts > 1) k ? launch(logprob_forward_kernel<T, 256, true, true>, 256, parts) : launch(logprob_forward_kernel<T, 256, false, true>, 256, parts);
-    else if (nt == 128) k ? launch(logprob_forward_kernel<T, 128, true, false>, 128, 1) : launch(logprob_forward_kernel<T, 128, false, false>, 128, 1);
-    else if (nt == 256) k ? launch(logprob_forward_kernel<T, 256, true, false>, 256, 1) : launch(logprob_forward_kernel<T, 256, false, false>, 256, 1);
-    else k ? launch(logprob_forward_kernel<T, 512, true, false>, 512, 1) : launch(logprob_forward_kernel<T, 512, false, false>, 512, 1);
+    const RowLaunch how = row_launch(rows, vocab * (int64_t)sizeof(T), logits.get_device());
+    for_bool(k > 0, [&](auto top_tag) {
+      for_row_launch(how, [&](auto nt_tag, auto split_tag) {
+        constexpr int NT = decltype(nt_tag)::value;
+        launch_rows(logprob_forward_kernel<T, NT, decltype(top_tag)::value, decltype(split_tag)::value>, rows, NT,
+                    how.parts, 0, s, (const T*)logits.data_ptr(), logits.stride(0), (int)vocab, tok, ignore_index, c,
+                    (float)(1.0 / temperature), k, lp, entropy.data_ptr<float>(), stats.data_ptr<float>(), tl, ti);
+      });
+    });
   });
   KB_LAUNCHED();
 }

@@ -302,14 +302,21 @@ __device__ __forceinline__ void mask_unit(uint4& q, const uint8_t* bits, int u) 
   }
 }
 
+// Where a row's units come from: memory, or units [u0, ..) staged in shared memory.
+struct FromMemory {
+  const uint4* p;
+  __device__ __forceinline__ void begin(int) const {}
+  __device__ __forceinline__ uint4 load(int u) const { return load_unit(p + u); }
+};
+
 // Statistics of the units [u0, u1) of a row over the threads of a block, in
 // batches of four 16-byte loads per thread (unit u0 + tid + (4 b + i) NT is the
 // i-th of batch b); batch_max(b, m) gets each batch's maximum. Per element: widening, half a packed
 // maximum, and in pairs a subtraction, a product, two 2^x and one or two sums.
 // Clamping the masked entries' exponents would cost one more instruction per
 // element; instead a batch whose A came out NaN (0 times -inf) takes its A again.
-template <typename T, int NT, bool ENT, bool MASK, typename G>
-__device__ __forceinline__ void stream_units(const uint4* p, int u0, int u1, float c, Run<ENT>& run,
+template <typename T, int NT, bool ENT, bool MASK, typename Src, typename G>
+__device__ __forceinline__ void stream_units(const Src& src, int u0, int u1, float c, Run<ENT>& run,
                                              const uint8_t* bits, const G& batch_max) {
   static_assert(!(ENT && MASK), "the masked form takes no entropy");
   constexpr int UN = kBatch, E = Elem<T>::kUnit;
@@ -317,19 +324,23 @@ __device__ __forceinline__ void stream_units(const uint4* p, int u0, int u1, flo
   int batch = 0;
   for (int base = u0 + (int)(threadIdx.x & ~31u); base < u1; base += UN * NT, ++batch) {  // whole warps
     const int u = base + (int)(threadIdx.x & 31);
+    const bool whole = base + (UN - 1) * NT + 32 <= u1;
+    src.begin(batch);
     uint4 q[UN];
+    if (whole) {
 #pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      if (u + i * NT < u1) {
-        q[i] = load_unit(p + u + i * NT);
-      } else {
+      for (int i = 0; i < UN; ++i) q[i] = src.load(u + i * NT);
+    } else {
+#pragma unroll
+      for (int i = 0; i < UN; ++i) {
         q[i] = make_uint4(Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf);
+        if (u + i * NT < u1) q[i] = src.load(u + i * NT);
       }
     }
     if (MASK) {
 #pragma unroll
       for (int i = 0; i < UN; ++i)
-        if (u + i * NT < u1) mask_unit<T>(q[i], bits, u + i * NT - u0);
+        if (u + i * NT < u1) mask_unit<T>(q[i], bits, u + i * NT);
     }
     uint32_t mx = Elem<T>::max2(Elem<T>::max2(q[0].x, q[0].y), Elem<T>::max2(q[0].z, q[0].w));
 #pragma unroll
@@ -342,7 +353,7 @@ __device__ __forceinline__ void stream_units(const uint4* p, int u0, int u1, flo
     const F2 a_before = run.a;
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
-      if (u + i * NT < u1) {
+      if (whole || base + i * NT < u1) {  // lanes behind the end hold -inf
         float v[E];
         Elem<T>::unpack(q[i], v);
 #pragma unroll
@@ -357,7 +368,7 @@ __device__ __forceinline__ void stream_units(const uint4* p, int u0, int u1, flo
         for (int i = 0; i < UN; ++i) {
           if (u + i * NT < u1) {
             float v[E];
-            Elem<T>::unpack(load_unit(p + u + i * NT), v);
+            Elem<T>::unpack(src.load(u + i * NT), v);
 #pragma unroll
             for (int j = 0; j < E; j += 2) run.add_masked(pair(v[j], v[j + 1]), mm, cc);
           }
@@ -404,43 +415,55 @@ __device__ __forceinline__ void segment(int units, int i, int n, int& u0, int& u
   u1 = min(units, u0 + per);
 }
 
-// Writes a row's units [u0, u1) and, for the first segment, its ragged
-// elements: out = f(two elements, the index of the first).
+// Writes a thread's batch of units u, u + NT, ...: out = f(two elements, the index of the first). `loaded` is called
+// once the batch is in registers.
+template <typename T, int NT, typename Src, typename F, typename L>
+__device__ __forceinline__ void map_batch(const Row<T>& row, const Src& src, T* out, bool same, int u, int u1,
+                                          const F& f, const L& loaded) {
+  constexpr int E = Elem<T>::kUnit;
+  uint4 q[kBatch];
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i)
+    if (u + i * NT < u1) q[i] = src.load(u + i * NT);
+  loaded();
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    if (u + i * NT < u1) {
+      const int idx = row.head + (u + i * NT) * E;
+      float v[E];
+      Elem<T>::unpack(q[i], v);
+#pragma unroll
+      for (int j = 0; j < E; j += 2) {
+        const float2 d = split(f(pair(v[j], v[j + 1]), idx + j));
+        v[j] = d.x;
+        v[j + 1] = d.y;
+      }
+      if (same) {
+        store_unit(reinterpret_cast<uint4*>(out + idx), Elem<T>::pack(v));
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) Elem<T>::store(out + idx + j, v[j]);
+      }
+    }
+  }
+}
+
+// Whether a row and its gradient lie alike to 16-byte boundaries.
+template <typename T>
+__device__ __forceinline__ bool same_boundaries(const T* z, const T* out) {
+  return ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+}
+
+// The same for the units [u0, u1) of a row and, for the first segment, its ragged elements.
 template <typename T, int NT, typename F>
 __device__ __forceinline__ void map_row(const Row<T>& row, T* out, int u0, int u1, int ragged, const F& f) {
-  constexpr int UN = 4, E = Elem<T>::kUnit;
-  const bool same = ((reinterpret_cast<uintptr_t>(row.z) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  const bool same = same_boundaries(row.z, out);
   if ((int)threadIdx.x < ragged) {
     const int idx = row.ragged_index(threadIdx.x);
     Elem<T>::store(out + idx, split(f(pair(Elem<T>::load(row.z + idx), 0.f), idx)).x);
   }
-  const uint4* p = row.unit_ptr();
-  for (int u = u0 + (int)threadIdx.x; u < u1; u += UN * NT) {
-    uint4 q[UN];
-#pragma unroll
-    for (int i = 0; i < UN; ++i)
-      if (u + i * NT < u1) q[i] = load_unit(p + u + i * NT);
-#pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      if (u + i * NT < u1) {
-        const int idx = row.head + (u + i * NT) * E;
-        float v[E];
-        Elem<T>::unpack(q[i], v);
-#pragma unroll
-        for (int j = 0; j < E; j += 2) {
-          const float2 d = split(f(pair(v[j], v[j + 1]), idx + j));
-          v[j] = d.x;
-          v[j + 1] = d.y;
-        }
-        if (same) {
-          store_unit(reinterpret_cast<uint4*>(out + idx), Elem<T>::pack(v));
-        } else {
-#pragma unroll
-          for (int j = 0; j < E; ++j) Elem<T>::store(out + idx + j, v[j]);
-        }
-      }
-    }
-  }
+  const FromMemory src{row.unit_ptr()};
+  for (int u = u0 + (int)threadIdx.x; u < u1; u += kBatch * NT) map_batch<T, NT>(row, src, out, same, u, u1, f, [] {});
 }
 
 template <typename T, int NT>
@@ -498,11 +521,36 @@ void check_out(const at::Tensor& out, const at::Tensor& logits, int64_t vocab) {
   KB_CHECK(out.size(0) <= 1 || out.stride(0) >= vocab, "rows of out overlap");
 }
 
-// Blocks that share a row: clusters of up to 8 where rows alone leave the device idle, of at least 16 KB each.
-int row_parts(int64_t rows, int64_t row_bytes, int device) {
-  int parts = 1;
-  while (parts < 8 && rows * parts * 2 <= 2 * (int64_t)num_sms(device) && row_bytes >= parts * 2 * 16384) parts *= 2;
-  return parts;
+// Threads per row of the statistics' passes. Small blocks leave less of the device idle at a row's end (V = 50257 bf16,
+// 16384 rows: 264 us with 128 threads, 282 with 256, 337 with 512) as long as there are rows enough to fill it; rows
+// above 128 KB take 256 (V = 131072 fp32, 4096 rows: 313 against 333 us). Few rows are shared by clusters of blocks
+// of at least 16 KB each.
+struct RowLaunch {
+  int threads, parts;
+};
+RowLaunch row_launch(int64_t rows, int64_t row_bytes, int device) {
+  const int64_t fill = 1536 * (int64_t)num_sms(device);
+  RowLaunch how{row_bytes > 128 * 1024 ? 256 : 128, 1};
+  while (how.threads < 512 && rows * how.threads < fill && row_bytes >= 32 * how.threads) how.threads *= 2;
+  if (how.threads < 512 || rows * 512 >= fill || row_bytes < 32768) return how;
+  how.threads = 256;
+  while (how.parts < 8 && rows * how.parts * 256 < fill && row_bytes >= how.parts * 2 * 16384) how.parts *= 2;
+  return how;
+}
+
+template <int N>
+using Int = std::integral_constant<int, N>;
+template <typename F>
+void for_bool(bool b, F&& f) {
+  if (b) f(std::true_type{});
+  else f(std::false_type{});
+}
+template <typename F>
+void for_row_launch(const RowLaunch& how, F&& f) {
+  if (how.parts > 1) f(Int<256>{}, std::true_type{});
+  else if (how.threads == 128) f(Int<128>{}, std::false_type{});
+  else if (how.threads == 256) f(Int<256>{}, std::false_type{});
+  else f(Int<512>{}, std::false_type{});
 }
 
 template <typename... P, typename... A>

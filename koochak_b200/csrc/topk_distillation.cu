@@ -2,11 +2,13 @@
 // student's distribution from the teacher's, and its gradient.
 #include <torch/csrc/utils/pybind.h>
 
+#include "sm100.cuh"
 #include "token_losses.cuh"
 
 namespace kb {
 namespace {
 
+constexpr int kChunks = 32;  // bulk copies a block stages its units with, at most
 constexpr int kStats = 8;  // floats kept per row for the backward pass: KdStats, the last 0 for a row without slots
 
 // --------------------------------------------------------- distillation
@@ -37,21 +39,47 @@ __device__ __forceinline__ bool read_slots(const T* z, int V, const int64_t* ids
 // What a row's gradient needs besides its logits:
 // dz_j = g (coef 2^((z_j - ms) c)) off the list, g (Q p_j - sum of its q) on it, p_j = 2^((z_j - m) c) inv_s.
 struct KdStats {
-  float ms, coef, m, inv_s, t_max, inv_e, mass, loss;
+  float ms, coef, m, inv_s, t_max, inv_e, mass;
+};
+__device__ __forceinline__ void store_stats(float* s, const KdStats& r) {
+  s[0] = r.ms;
+  s[1] = r.coef;
+  s[2] = r.m;
+  s[3] = r.inv_s;
+  s[4] = r.t_max;
+  s[5] = r.inv_e;
+  s[6] = r.mass;
+  s[7] = 1.f;
+}
+
+// What a row's list alone decides: the normaliser of q, its sum, the rest, and (TAIL) the student's maximum and sum
+// over the distinct listed tokens.
+struct ListStats {
+  float t_max, inv_e, q_sum, q_rest, z_max, z_sum;
 };
 
-// Loss of one row, by one warp, from the statistics of the streamed elements
-// (all of them, or with TAIL those off the list).
+// By one warp.
 template <bool TAIL>
-__device__ __forceinline__ KdStats distill_row(const Acc& str, float c, float inv_t, int K, const ListShared& sh) {
+__device__ __forceinline__ ListStats list_stats(float c, int K, const ListShared& sh) {
   const int lane = threadIdx.x & 31;
-  KdStats r;
-  float q_sum = 0.f;
+  ListStats r{0.f, 1.f, 0.f, 0.f, -INFINITY, 0.f};
   if (TAIL) {
-    r.t_max = 0.f;
-    r.inv_e = 1.f;
-    for (int i = lane; i < K; i += 32) q_sum += ex2(sh.t[i] * kLog2e);
-    q_sum = warp_sum(q_sum);
+    float q_sum = 0.f, zm = -INFINITY, s = 0.f;
+    for (int i = lane; i < K; i += 32) {
+      q_sum += ex2(sh.t[i] * kLog2e);
+      if (sh.id[i] >= 0) zm = max_nan(zm, sh.z[i]);
+    }
+    r.q_sum = warp_sum(q_sum);
+    r.q_rest = r.q_sum > 1.f ? 0.f : 1.f - r.q_sum;
+    r.z_max = warp_max_nan(zm);
+    const float zs = r.z_max == -INFINITY ? 0.f : r.z_max;
+    for (int i = lane; i < K; i += 32) {
+      bool counts = sh.id[i] >= 0;
+      if (sh.repeated)
+        for (int j = 0; j < i; ++j) counts &= sh.id[j] != sh.id[i];
+      if (counts) s += ex2((sh.z[i] - zs) * c);
+    }
+    r.z_sum = warp_sum(s);
   } else {
     float tm = -INFINITY, e = 0.f;
     for (int i = lane; i < K; i += 32) tm = max_nan(tm, sh.t[i]);
@@ -60,26 +88,39 @@ __device__ __forceinline__ KdStats distill_row(const Acc& str, float c, float in
     for (int i = lane; i < K; i += 32) e += ex2((sh.t[i] - r.t_max) * c);
     e = warp_sum(e);
     r.inv_e = e == 0.f ? 0.f : 1.f / e;
-    q_sum = e == 0.f ? 0.f : 1.f;
+    r.q_sum = e == 0.f ? 0.f : 1.f;
   }
-  const float q_rest = TAIL ? (q_sum > 1.f ? 0.f : 1.f - q_sum) : 0.f;
+  return r;
+}
+
+// From the statistics of the streamed elements (all of them, or with TAIL those off the list).
+template <bool TAIL>
+__device__ __forceinline__ KdStats row_stats(const Acc& str, const ListStats& list, float c) {
   Acc all = str;
+  if (TAIL) all.join<false>(list.z_max, list.z_sum, 0.f, c);
+  KdStats r;
+  r.t_max = list.t_max;
+  r.inv_e = list.inv_e;
+  r.m = all.m;
+  r.inv_s = 1.f / all.s;
+  // Where the student has no mass off the list, a rest is an infinite constant: it has no gradient.
+  r.mass = TAIL && str.s != 0.f ? list.q_sum + list.q_rest : list.q_sum;
+  r.coef = r.mass * r.inv_s;
   if (TAIL) {
-    float zm = -INFINITY;
-    for (int i = lane; i < K; i += 32)
-      if (sh.id[i] >= 0) zm = max_nan(zm, sh.z[i]);
-    zm = warp_max_nan(zm);
-    const float zs = zm == -INFINITY ? 0.f : zm;
-    float s = 0.f;
-    for (int i = lane; i < K; i += 32) {
-      bool counts = sh.id[i] >= 0;
-      if (sh.repeated)
-        for (int j = 0; j < i; ++j) counts &= sh.id[j] != sh.id[i];
-      if (counts) s += ex2((sh.z[i] - zs) * c);
-    }
-    s = warp_sum(s);
-    all.join<false>(zm, s, 0.f, c);
+    const float down = str.m == all.m ? 0.f : str.m - all.m;
+    r.coef = str.s == 0.f ? 0.f : r.coef * ex2(down * c) - list.q_rest / str.s;
   }
+  r.ms = str.m == -INFINITY ? 0.f : str.m;
+  return r;
+}
+
+// The row's loss, by one warp.
+template <bool TAIL>
+__device__ __forceinline__ float row_loss(const Acc& str, const ListStats& list, const KdStats& r, float c, float inv_t,
+                                          int K, const ListShared& sh) {
+  const int lane = threadIdx.x & 31;
+  Acc all = str;
+  if (TAIL) all.join<false>(list.z_max, list.z_sum, 0.f, c);
   // In units of z / T, not of c z: (lowest - m) c would overflow.
   const float ln_s = kLn2 * log2f(all.s), ln_inv_e = TAIL ? 0.f : kLn2 * log2f(r.inv_e);
   float loss = 0.f;
@@ -90,140 +131,406 @@ __device__ __forceinline__ KdStats distill_row(const Acc& str, float c, float in
     if (q != 0.f) loss += q * (lq - ((sh.z[i] - all.m) * inv_t - ln_s));
   }
   loss = warp_sum(loss);
-  r.m = all.m;
-  r.inv_s = 1.f / all.s;
-  // Where the student has no mass off the list, a rest is an infinite constant: it has no gradient.
-  r.mass = TAIL && str.s != 0.f ? q_sum + q_rest : q_sum;
-  if (TAIL) {
+  if (TAIL && list.q_rest != 0.f) {
     const float down = str.m == all.m ? 0.f : str.m - all.m;
-    if (q_rest != 0.f) loss += q_rest * (kLn2 * (log2f(q_rest) - log2f(str.s)) - down * inv_t + ln_s);
-    r.coef = str.s == 0.f ? 0.f : r.mass * ex2(down * c) * r.inv_s - q_rest / str.s;
-  } else {
-    r.coef = r.mass * r.inv_s;
+    loss += list.q_rest * (kLn2 * (log2f(list.q_rest) - log2f(str.s)) - down * inv_t + ln_s);
   }
-  r.ms = str.m == -INFINITY ? 0.f : str.m;
-  r.loss = loss;
-  return r;
+  return loss;
 }
 
-// One block per row. Off-list elements are told by a bit per element in shared memory (TAIL).
-template <typename T, int NT, bool TAIL>
-__global__ void __launch_bounds__(NT)
-    distill_forward_kernel(const T* __restrict__ logits, long long ld, int V, const int64_t* __restrict__ ids,
-                           const float* __restrict__ teacher, int K, float c, float inv_t, float* __restrict__ loss,
-                           float* __restrict__ stats) {
-  extern __shared__ __align__(16) uint8_t bits[];
-  __shared__ ListShared sh;
-  __shared__ Acc join_sm[NT / 32];
+// A bit per element: u * E + j for element j of unit u, the ragged elements behind the units.
+template <typename T>
+__device__ __forceinline__ int bit_of(const Row<T>& row, int id) {
+  const int body = row.units * Elem<T>::kUnit;
+  return id < row.head ? body + id : id < row.head + body ? id - row.head : id;
+}
+// Sets a bit; whether it was set before.
+__device__ __forceinline__ bool mark(uint8_t* bits, int bit) {
+  return (atomicOr(reinterpret_cast<uint32_t*>(bits) + (bit >> 5), 1u << (bit & 31)) >> (bit & 31)) & 1u;
+}
+__device__ __forceinline__ void unmark(uint8_t* bits, int bit) { reinterpret_cast<uint32_t*>(bits)[bit >> 5] = 0; }
+__device__ __forceinline__ bool marked(const uint8_t* bits, int bit) { return (bits[bit >> 3] >> (bit & 7)) & 1u; }
+
+// Gradient of the listed elements among units [u0, u1) and, if asked, the ragged ones: sums the q of slots that name
+// the same token.
+template <typename T>
+__device__ __forceinline__ void write_listed(const Row<T>& row, T* out, int u0, int u1, bool ragged_too, int K, float c,
+                                             float g, const KdStats& r, const ListShared& sh, int first, int step) {
   constexpr int E = Elem<T>::kUnit;
-  const int tid = threadIdx.x;
-  const long long row_i = blockIdx.x;
-  const Row<T> row(logits + row_i * ld, V);
-  if (tid == 0) sh.repeated = 0;
-  if (TAIL) {
-    uint32_t* w = reinterpret_cast<uint32_t*>(bits);
-    for (int i = tid; i < (V + 31) / 32; i += NT) w[i] = 0;
-  }
-  if (!read_slots<T, NT>(row.z, V, ids + row_i * K, teacher + row_i * K, K, sh)) {
-    if (tid == 0) loss[row_i] = 0.f;
-    if (tid < kStats) stats[row_i * kStats + tid] = 0.f;
-    return;
-  }
-  Run<false> run;
-  if (TAIL) {
-    // Bit u * E + j for element j of unit u, ragged elements behind the units.
-    for (int i = tid; i < K; i += NT) {
-      const int id = sh.id[i];
-      if (id < 0) continue;
-      const int body = row.units * E;
-      const int bit = id < row.head ? body + id : id < row.head + body ? id - row.head : id;
-      const uint32_t old = atomicOr(reinterpret_cast<uint32_t*>(bits) + (bit >> 5), 1u << (bit & 31));
-      if ((old >> (bit & 31)) & 1u) sh.repeated = 1;
-    }
-    __syncthreads();
-  }
-  if (tid < 32) {  // fewer than two units of ragged elements
-    const int bit = row.units * E + tid;
-    const bool in = tid < row.ragged && (!TAIL || !((bits[bit >> 3] >> (bit & 7)) & 1u));
-    run.add_one(in ? Elem<T>::load(row.z + row.ragged_index(tid)) : -INFINITY, c);
-  }
-  stream_units<T, NT, false, TAIL>(row.unit_ptr(), 0, row.units, c, run, bits, [](int, float) {});
-  const Acc all = block_join<NT, false>(run, c, join_sm);
-  if (tid < 32) {
-    const KdStats r = distill_row<TAIL>(all, c, inv_t, K, sh);
-    if (tid == 0) {
-      loss[row_i] = r.loss;
-      float* s = stats + row_i * kStats;
-      s[0] = r.ms;
-      s[1] = r.coef;
-      s[2] = r.m;
-      s[3] = r.inv_s;
-      s[4] = r.t_max;
-      s[5] = r.inv_e;
-      s[6] = r.mass;
-      s[7] = 1.f;
-    }
-  }
-}
-
-// Gradient of the listed elements of a segment: sums the q of slots that name the same token.
-template <typename T, int NT, bool TAIL>
-__device__ __forceinline__ void write_listed(T* out, const ListShared& sh, int K, float c, float g, const KdStats& r,
-                                             int lo, int hi, bool ragged_too, int body_lo, int body_hi) {
-  for (int i = threadIdx.x; i < K; i += NT) {
+  for (int i = first; i < K; i += step) {
     const int id = sh.id[i];
     if (id < 0) continue;
-    const bool in_body = id >= body_lo && id < body_hi;
-    if (in_body ? !(id >= lo && id < hi) : !ragged_too) continue;
-    float q = 0.f;
-    for (int j = 0; j < K; ++j)
-      if (sh.id[j] == id) q += sh.q[j];
+    const int at = id - row.head;
+    const bool in_body = at >= 0 && at < row.units * E;
+    if (in_body ? !(at >= u0 * E && at < u1 * E) : !ragged_too) continue;
+    float q = sh.q[i];
+    if (sh.repeated) {
+      q = 0.f;
+      for (int j = 0; j < K; ++j)
+        if (sh.id[j] == id) q += sh.q[j];
+    }
     Elem<T>::store(out + id, g * (r.mass * (ex2((sh.z[i] - r.m) * c) * r.inv_s) - q));
   }
 }
 
+// Gradient of a row's units [u0, u1): the dense part in one pass, then the listed elements over it.
 template <typename T, int NT, bool TAIL>
-__global__ void __launch_bounds__(NT)
-    distill_backward_kernel(const T* logits, long long ld, T* out, long long ld_out, int V,
-                            const int64_t* __restrict__ ids, const float* __restrict__ teacher, int K, float c,
-                            float inv_t, const float* __restrict__ stats, const float* __restrict__ row_scale,
-                            const float* __restrict__ scale) {
-  constexpr int E = Elem<T>::kUnit;
-  __shared__ ListShared sh;
-  const long long row_i = gridDim.x - 1 - blockIdx.x;  // last rows first: the forward pass left them in L2
-  const float* s = stats + row_i * kStats;
-  const float w = row_scale ? row_scale[row_i] : 1.f;
-  T* o = out + row_i * ld_out;
-  int u0, u1;
-  if (s[7] == 0.f || w == 0.f) {
-    const Row<T> row(o, V);
-    segment(row.units, blockIdx.y, gridDim.y, u0, u1);
-    zero_row<T, NT>(row, u0, u1, blockIdx.y == 0 ? row.ragged : 0);
-    return;
-  }
-  const Row<T> row(logits + row_i * ld, V);
-  segment(row.units, blockIdx.y, gridDim.y, u0, u1);
-  KdStats r;
-  r.ms = s[0];
-  r.coef = s[1];
-  r.m = s[2];
-  r.inv_s = s[3];
-  r.t_max = s[4];
-  r.inv_e = s[5];
-  r.mass = s[6];
-  const float g = w * (scale ? *scale : 1.f) * inv_t;
-  read_slots<T, NT>(row.z, V, ids + row_i * K, teacher + row_i * K, K, sh);
+__device__ __forceinline__ void write_gradient(const Row<T>& row, T* out, int u0, int u1, int ragged, int K, float c,
+                                               float g, const KdStats& r, ListShared& sh) {
   for (int i = threadIdx.x; i < K; i += NT) sh.q[i] = ex2((sh.t[i] - r.t_max) * (TAIL ? kLog2e : c)) * r.inv_e;
   const float dense = g * r.coef;
-  const int ragged = blockIdx.y == 0 ? row.ragged : 0;
   const F2 minus_m = pair(-r.ms, -r.ms), cc = pair(c, c), dd = pair(dense, dense);
-  map_row<T, NT>(row, o, u0, u1, ragged, [&](F2 z, int) {
+  map_row<T, NT>(row, out, u0, u1, ragged, [&](F2 z, int) {
     const float2 x = split(mul2(add2(z, minus_m), cc));
     return mul2(pair(ex2(x.x), ex2(x.y)), dd);
   });
   __syncthreads();
-  write_listed<T, NT, TAIL>(o, sh, K, c, g, r, row.head + u0 * E, row.head + u1 * E, blockIdx.y == 0, row.head,
-                            row.head + row.units * E);
+  write_listed<T>(row, out, u0, u1, ragged > 0, K, c, g, r, sh, threadIdx.x, NT);
+}
+
+// Loss of each row, times its weight: a block per row, or with SPLIT a cluster of blocks that share it. Off-list
+// elements are told by a bit per element in shared memory (TAIL).
+template <typename T, int NT, bool TAIL, bool SPLIT>
+__global__ void __launch_bounds__(NT)
+    distill_forward_kernel(const T* __restrict__ logits, long long ld, int V, const int64_t* __restrict__ ids,
+                           const float* __restrict__ teacher, int K, float c, float inv_t,
+                           const float* __restrict__ weight, float* __restrict__ loss, float* __restrict__ stats) {
+  namespace cg = cooperative_groups;
+  extern __shared__ __align__(16) uint8_t bits[];
+  __shared__ ListShared sh;
+  __shared__ Acc join_sm[NT / 32], result;
+  constexpr int E = Elem<T>::kUnit;
+  const int tid = threadIdx.x;
+  int part = 0, parts = 1;
+  if constexpr (SPLIT) {
+    part = (int)cg::this_cluster().block_rank();
+    parts = (int)cg::this_cluster().num_blocks();
+  }
+  const long long row_i = SPLIT ? blockIdx.x / parts : blockIdx.x;
+  const Row<T> row(logits + row_i * ld, V);
+  int u0, u1;
+  segment(row.units, part, parts, u0, u1);
+  const int ragged = part == 0 ? row.ragged : 0;
+  const float w = weight ? weight[row_i] : 1.f;
+  if (tid == 0) sh.repeated = 0;
+  if (TAIL) {
+    uint32_t* words = reinterpret_cast<uint32_t*>(bits);
+    for (int i = tid; i < (V + 31) / 32; i += NT) words[i] = 0;
+  }
+  const bool some = w != 0.f && read_slots<T, NT>(row.z, V, ids + row_i * K, teacher + row_i * K, K, sh);
+  if (!some) {
+    if (part == 0 && tid == 0) loss[row_i] = 0.f;
+    if (part == 0 && tid < kStats) stats[row_i * kStats + tid] = 0.f;
+    return;
+  }
+  Run<false> run;
+  if (TAIL) {
+    for (int i = tid; i < K; i += NT)
+      if (sh.id[i] >= 0 && mark(bits, bit_of(row, sh.id[i]))) sh.repeated = 1;
+    __syncthreads();
+  }
+  if (tid < 32) {  // fewer than two units of ragged elements
+    const bool in = tid < ragged && (!TAIL || !marked(bits, row.units * E + tid));
+    run.add_one(in ? Elem<T>::load(row.z + row.ragged_index(tid)) : -INFINITY, c);
+  }
+  stream_units<T, NT, false, TAIL>(FromMemory{row.unit_ptr()}, u0, u1, c, run, bits, [](int, float) {});
+  Acc all = block_join<NT, false>(run, c, join_sm);
+  if constexpr (SPLIT) {
+    if (tid == 0) result = all;
+    cg::this_cluster().sync();
+    if (part == 0 && tid < 32) {
+      all = *cg::this_cluster().map_shared_rank(&result, (tid & 7) < parts ? tid & 7 : 0);
+      all = join_lanes<8, false>((tid & 7) < parts ? all : Acc(), c);
+    }
+    cg::this_cluster().sync();  // the parts' statistics are read
+  }
+  if (part == 0 && tid < 32) {
+    const ListStats list = list_stats<TAIL>(c, K, sh);
+    const KdStats r = row_stats<TAIL>(all, list, c);
+    const float l = row_loss<TAIL>(all, list, r, c, inv_t, K, sh);
+    if (tid == 0) {
+      loss[row_i] = w * l;
+      store_stats(stats + row_i * kStats, r);
+    }
+  }
+}
+
+// A row's units [0, ..) staged in shared memory.
+struct FromStage {
+  const uint4* stage;
+  uint64_t* full;
+  uint32_t parity;
+  volatile int* abort_flag;
+  int* status;
+  // Waits for the batch's chunk; a copy that does not arrive is recorded, and the host raises on it.
+  __device__ __forceinline__ void begin(int batch) const {
+    mbar_wait(&full[batch], parity, abort_flag, status, kStatusTimeoutRowStage);
+  }
+  __device__ __forceinline__ uint4 load(int u) const { return stage[u]; }
+};
+
+// Loss and gradient of each row in one go: the logits are read from memory once and the gradient written once.
+//
+// A persistent block stages a row in shared memory by bulk copies, a chunk per barrier. Its streaming warps take the
+// statistics in a first pass and write the gradient in a second; a chunk that all of them have left behind is filled
+// with the block's next row at once. One more warp serves them: it issues the copies, joins the statistics, and does
+// all work on the lists (the next row's list is fetched, marked and summed during this row's second pass, and the
+// listed elements are written after the dense gradient). Two blocks share an SM, so that one stores and fetches while
+// the other is between its passes.
+// Reading the row twice through L2 instead took 849 us on 16384 x 50257 bf16, more than two kernels (815 us): too many
+// rows are in flight for L2 to hold them.
+constexpr int kOwn = kMaxList / 32;  // slots per lane of the serving warp
+
+struct GradShared {
+  ListShared list[2];
+  KdStats stats;
+  float weight[2];
+  int some[2];
+  uint64_t full[kChunks], empty[kChunks], ready, joined, solved, done;
+  int abort_flag;
+};
+
+template <typename T, int NT, bool TAIL>
+__global__ void __launch_bounds__(NT + 32, 1024 / NT)
+    distill_grad_kernel(const T* logits, long long ld, T* out, long long ld_out, int V, long long rows,
+                        const int64_t* __restrict__ ids, const float* __restrict__ teacher, int K, float c, float inv_t,
+                        const float* __restrict__ weight, float* __restrict__ loss, float* __restrict__ stats,
+                        int stage_units, int* status) {
+  extern __shared__ __align__(128) uint8_t dynamic[];
+  constexpr int E = Elem<T>::kUnit, NW = NT / 32, kChunk = kBatch * NT;  // units of a batch of the streaming warps
+  uint4* stage = reinterpret_cast<uint4*>(dynamic);
+  uint8_t* bits = dynamic + 16 * (size_t)stage_units;
+  __shared__ GradShared sh;
+  __shared__ Acc sums[NW];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int chunks = (stage_units + kChunk - 1) / kChunk;
+  if (tid == 0) {
+    for (int i = 0; i < chunks; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], NW);
+    }
+    mbar_init(&sh.ready, 1);
+    mbar_init(&sh.joined, NW);
+    mbar_init(&sh.solved, 1);
+    mbar_init(&sh.done, NW);
+    sh.abort_flag = 0;
+    fence_barrier_init();
+  }
+  for (int i = tid; i < (V + 31) / 32; i += NT + 32) reinterpret_cast<uint32_t*>(bits)[i] = 0;
+  __syncthreads();
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    mbar_wait(bar, parity & 1u, &sh.abort_flag, status, kStatusTimeoutRowStage);
+  };
+  // Rows so far, and rows with slots: `full` and `empty` complete once per row with slots, the other barriers once per
+  // row, each only after everyone who waits on it has seen the row before: ready(n + 1) follows joined(n), joined and
+  // done(n + 1) follow solved(n + 1), and that follows done(n).
+  uint32_t count = 0, staged = 0;
+
+  if (tid < NT) {
+    for (long long r = blockIdx.x; r < rows; r += gridDim.x, ++count) {
+      const Row<T> row(logits + r * ld, V);
+      T* o = out + r * ld_out;
+      const float rag = tid < row.ragged ? Elem<T>::load(row.z + row.ragged_index(tid)) : -INFINITY;
+      wait(&sh.ready, count);
+      const float g = sh.weight[count & 1] * inv_t;
+      if (!sh.some[count & 1]) {
+        if (lane == 0) mbar_arrive(&sh.joined);
+        wait(&sh.solved, count);
+        const Row<T> to(o, V);
+        zero_row<T, NT>(to, 0, to.units, to.ragged);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.done);
+        continue;
+      }
+      Run<false> run;
+      const FromStage src{stage, sh.full, staged & 1u, &sh.abort_flag, status};
+      if (tid < 32) run.add_one(TAIL && tid < row.ragged && marked(bits, row.units * E + tid) ? -INFINITY : rag, c);
+      stream_units<T, NT, false, TAIL>(src, 0, row.units, c, run, bits, [](int, float) {});
+      const Acc mine = run.total();
+      if (lane == 0) {
+        sums[tid >> 5] = mine;
+        mbar_arrive(&sh.joined);
+      }
+      wait(&sh.solved, count);
+      const F2 minus_m = pair(-sh.stats.ms, -sh.stats.ms), cc = pair(c, c);
+      const F2 dd = pair(g * sh.stats.coef, g * sh.stats.coef);
+      auto gradient = [&](F2 v, int) {
+        const float2 x = split(mul2(add2(v, minus_m), cc));
+        return mul2(pair(ex2(x.x), ex2(x.y)), dd);
+      };
+      const bool same = same_boundaries(row.z, o);
+      for (int i = 0; i < chunks; ++i) {
+        map_batch<T, NT>(row, src, o, same, i * kChunk + tid, row.units, gradient, [&] {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.empty[i]);
+        });
+      }
+      if (tid < row.ragged) Elem<T>::store(o + row.ragged_index(tid), split(gradient(pair(rag, 0.f), 0)).x);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.done);
+      ++staged;
+    }
+    return;
+  }
+
+  // The serving warp. Slots lane, lane + 32, ... of the row that comes next:
+  int64_t given[kOwn];
+  float t[kOwn], z[kOwn], w = 0.f;
+  auto ask = [&](long long r) {
+    w = r < rows ? (weight ? weight[r] : 1.f) : 0.f;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const bool in = r < rows && i * 32 + lane < K;
+      given[i] = in ? ids[r * K + i * 32 + lane] : -1;
+      t[i] = in ? teacher[r * K + i * 32 + lane] : 0.f;
+    }
+  };
+  auto valid = [&](int i) { return given[i] >= 0 && given[i] < V; };
+  auto ask_logits = [&](long long r) {
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) z[i] = valid(i) ? Elem<T>::load(logits + r * ld + given[i]) : 0.f;
+  };
+  auto any_slot = [&] {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) any |= valid(i);
+    return __any_sync(0xffffffffu, any) && w != 0.f;
+  };
+  // Gives the row out to the streaming warps: its list, marks and what the list alone decides.
+  auto prepare = [&](const Row<T>& row, uint32_t n, bool some) {
+    ListShared& list = sh.list[n & 1];
+    ListStats ls{};
+    if (some) {
+      if (lane == 0) list.repeated = 0;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        if (i * 32 + lane < K) {
+          const int id = valid(i) ? (int)given[i] : -1;
+          list.id[i * 32 + lane] = id;
+          list.t[i * 32 + lane] = valid(i) ? t[i] : -INFINITY;
+          list.z[i * 32 + lane] = z[i];
+          if (id >= 0 && mark(bits, bit_of(row, id))) list.repeated = 1;
+        }
+      }
+      __syncwarp();
+      ls = list_stats<TAIL>(c, K, list);
+    }
+    if (lane == 0) {
+      sh.some[n & 1] = some;
+      sh.weight[n & 1] = w;
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.ready);
+    return ls;
+  };
+  uint32_t fetched = 0;  // rows whose copies were issued
+  auto fetch = [&](const Row<T>& row, int i) {  // chunk i of a row; every barrier completes once per row
+    if (fetched > 0) wait(&sh.empty[i], fetched - 1);
+    if (lane == 0) {
+      const int n = min(kChunk, row.units - i * kChunk);
+      if (n > 0) {
+        mbar_arrive_expect_tx(&sh.full[i], (uint32_t)n * 16);
+        bulk_load_1d(stage + i * kChunk, row.unit_ptr() + i * kChunk, (uint32_t)n * 16, &sh.full[i]);
+      } else {
+        mbar_arrive(&sh.full[i]);
+      }
+    }
+    __syncwarp();
+  };
+  ask(blockIdx.x);
+  bool some = any_slot();
+  if (some) {
+    for (int i = 0; i < chunks; ++i) fetch(Row<T>(logits + blockIdx.x * ld, V), i);
+    ++fetched;
+  }
+  ask_logits(blockIdx.x);
+  ListStats list = prepare(Row<T>(logits + blockIdx.x * ld, V), 0, some);
+  float w_now = w;
+  ask(blockIdx.x + (long long)gridDim.x);
+  for (long long r = blockIdx.x; r < rows; r += gridDim.x, ++count) {
+    const long long next = r + gridDim.x;
+    const Row<T> row(logits + r * ld, V), next_row(logits + (next < rows ? next : r) * ld, V);
+    ListShared& now = sh.list[count & 1];
+    const bool some_next = any_slot();
+    ask_logits(next);
+    KdStats k;
+    Acc all;
+    wait(&sh.joined, count);
+    if (some) {
+      all = join_lanes<NW, false>(sums[lane & (NW - 1)], c);
+      k = row_stats<TAIL>(all, list, c);
+      if (lane == 0) sh.stats = k;
+    }
+    if (lane == 0) mbar_arrive(&sh.solved);
+    // The streaming warps are in the second pass, or write zeros.
+    const ListStats list_now = list;
+    if (some_next && chunks > 0) fetch(next_row, 0);
+    if (some) {
+      for (int i = lane; i < K; i += 32)
+        if (now.id[i] >= 0) unmark(bits, bit_of(row, now.id[i]));
+      __syncwarp();
+    }
+    const float w_next = w;
+    if (next < rows) list = prepare(next_row, count + 1, some_next);
+    ask(next + gridDim.x);
+    if (some_next) {
+      for (int i = 1; i < chunks; ++i) fetch(next_row, i);
+      ++fetched;
+    }
+    if (some) {
+      const float l = row_loss<TAIL>(all, list_now, k, c, inv_t, K, now);
+      if (lane == 0) {
+        loss[r] = w_now * l;
+        store_stats(stats + r * kStats, k);
+      }
+      for (int i = lane; i < K; i += 32) now.q[i] = ex2((now.t[i] - k.t_max) * (TAIL ? kLog2e : c)) * k.inv_e;
+    }
+    wait(&sh.done, count);
+    if (some) {
+      __syncwarp();
+      write_listed<T>(row, out + r * ld_out, 0, row.units, true, K, c, w_now * inv_t, k, now, lane, 32);
+      ++staged;
+    } else if (lane < kStats) {
+      stats[r * kStats + lane] = 0.f;
+      if (lane == 0) loss[r] = 0.f;
+    }
+    __syncwarp();
+    some = some_next;
+    w_now = w_next;
+  }
+}
+
+// Gradient from the statistics the forward pass left; with `unless_one` nothing is done where the scale is one.
+template <typename T, int NT, bool TAIL>
+__global__ void __launch_bounds__(NT)
+    distill_backward_kernel(const T* logits, long long ld, T* out, long long ld_out, int V, long long rows,
+                            const int64_t* __restrict__ ids, const float* __restrict__ teacher, int K, float c,
+                            float inv_t, const float* __restrict__ stats, const float* __restrict__ row_scale,
+                            const float* __restrict__ scale, bool unless_one) {
+  __shared__ ListShared sh;
+  const float factor = scale ? *scale : 1.f;
+  if (unless_one && factor == 1.f) return;
+  for (long long i = blockIdx.x; i < rows; i += gridDim.x) {
+    const long long row_i = rows - 1 - i;  // last rows first: the forward pass left them in L2
+    const float* s = stats + row_i * kStats;
+    const float w = row_scale ? row_scale[row_i] : 1.f;
+    T* o = out + row_i * ld_out;
+    int u0, u1;
+    if (s[7] == 0.f || w == 0.f) {
+      const Row<T> row(o, V);
+      segment(row.units, blockIdx.y, gridDim.y, u0, u1);
+      zero_row<T, NT>(row, u0, u1, blockIdx.y == 0 ? row.ragged : 0);
+      continue;
+    }
+    const Row<T> row(logits + row_i * ld, V);
+    segment(row.units, blockIdx.y, gridDim.y, u0, u1);
+    const KdStats r{s[0], s[1], s[2], s[3], s[4], s[5], s[6]};
+    if (threadIdx.x == 0) sh.repeated = 1;  // not known here
+    read_slots<T, NT>(row.z, V, ids + row_i * K, teacher + row_i * K, K, sh);
+    write_gradient<T, NT, TAIL>(row, o, u0, u1, blockIdx.y == 0 ? row.ragged : 0, K, c, w * factor * inv_t, r, sh);
+    __syncthreads();  // the list is read before the next row's replaces it
+  }
 }
 
 int check_teacher(const at::Tensor& ids, const at::Tensor& teacher, int64_t rows, const at::Tensor& logits) {
@@ -235,38 +542,75 @@ int check_teacher(const at::Tensor& ids, const at::Tensor& teacher, int64_t rows
 }
 }  // namespace
 
+void topk_distillation_backward(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher,
+                                const at::Tensor& stats, const c10::optional<at::Tensor>& row_scale,
+                                const c10::optional<at::Tensor>& scale, const at::Tensor& out, int64_t vocab,
+                                double temperature, bool tail, bool unless_one);
+
+// With `out`, the gradient of the weighted sum of losses is written too (it may be the logits themselves).
 void topk_distillation_forward(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher,
-                               at::Tensor& loss, at::Tensor& stats, int64_t vocab, double temperature, bool tail) {
+                               const c10::optional<at::Tensor>& weight, at::Tensor& loss, at::Tensor& stats,
+                               const c10::optional<at::Tensor>& out, int64_t vocab, double temperature, bool tail) {
   const int64_t rows = check_logits(logits, vocab, temperature, "logits");
   const int k = check_teacher(ids, teacher, rows, logits);
+  if (weight) check_rows(*weight, "weight", rows, 1, at::kFloat, logits);
   check_rows(loss, "loss", rows, 1, at::kFloat, logits);
   check_rows(stats, "stats", rows, kStats, at::kFloat, logits);
+  if (out) check_out(*out, logits, vocab);
   if (rows == 0) return;
+  const int64_t bits = tail ? (vocab + 31) / 32 * 4 : 0;
+  const int device = logits.get_device();
+  // Loss and gradient in one kernel where a row fits into half an SM's shared memory and the rows fill the device.
+  const int64_t units = vocab * logits.element_size() / 16, staged = (units * 16 + 127) / 128 * 128 + (vocab + 31) / 32 * 4;
+  const bool together = out && staged <= 108 * 1024 && rows >= num_sms(device);
+  if (out && !together) {
+    topk_distillation_forward(logits, ids, teacher, weight, loss, stats, c10::nullopt, vocab, temperature, tail);
+    topk_distillation_backward(logits, ids, teacher, stats, weight, c10::nullopt, *out, vocab, temperature, tail, false);
+    return;
+  }
   const c10::cuda::CUDAGuard guard(logits.device());
   cudaStream_t s = c10::cuda::getCurrentCUDAStream().stream();
-  const float c = (float)(1.4426950408889634 / temperature);
-  const size_t bits = tail ? (size_t)((vocab + 31) / 32 * 4) : 0;
+  const float c = (float)(1.4426950408889634 / temperature), inv_t = (float)(1.0 / temperature);
+  const float* w = weight ? weight->data_ptr<float>() : nullptr;
   for_logits_type(logits.scalar_type(), [&](auto tag) {
     using T = typename decltype(tag)::type;
-    auto launch = [&](auto kern, int nt) {
-      if (bits > 32 * 1024)
-        KB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bits));
-      kern<<<(unsigned)rows, nt, bits, s>>>((const T*)logits.data_ptr(), logits.stride(0), (int)vocab,
-                                            ids.data_ptr<int64_t>(), teacher.data_ptr<float>(), k, c,
-                                            (float)(1.0 / temperature), loss.data_ptr<float>(), stats.data_ptr<float>());
-    };
-    const int nt = getenv("KB_NT") ? atoi(getenv("KB_NT")) : 512;
-    if (nt == 128) tail ? launch(distill_forward_kernel<T, 128, true>, 128) : launch(distill_forward_kernel<T, 128, false>, 128);
-    else if (nt == 256) tail ? launch(distill_forward_kernel<T, 256, true>, 256) : launch(distill_forward_kernel<T, 256, false>, 256);
-    else tail ? launch(distill_forward_kernel<T, 512, true>, 512) : launch(distill_forward_kernel<T, 512, false>, 512);
+    for_bool(tail, [&](auto tail_tag) {
+      constexpr bool TAIL = decltype(tail_tag)::value;
+      if (together) {
+        auto launch = [&](auto kern, int threads) {
+          KB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)staged));
+          int per_sm = 0;
+          KB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads + 32, (size_t)staged));
+          const int64_t blocks = std::min<int64_t>(rows, (int64_t)std::max(1, per_sm) * num_sms(device));
+          launch_rows(kern, blocks, threads + 32, 1, (size_t)staged, s, (const T*)logits.data_ptr(), logits.stride(0),
+                      (T*)out->data_ptr(), out->stride(0), (int)vocab, rows, ids.data_ptr<int64_t>(),
+                      teacher.data_ptr<float>(), k, c, inv_t, w, loss.data_ptr<float>(), stats.data_ptr<float>(),
+                      (int)((units * 16 + 127) / 128 * 8), device_status_ptr(device));
+        };
+        if (vocab * (int64_t)sizeof(T) <= 16384) launch(distill_grad_kernel<T, 128, TAIL>, 128);
+        else launch(distill_grad_kernel<T, 512, TAIL>, 512);
+        return;
+      }
+      const RowLaunch how = row_launch(rows, vocab * (int64_t)sizeof(T), device);
+      for_row_launch(how, [&](auto nt_tag, auto split_tag) {
+        constexpr int NT = decltype(nt_tag)::value;
+        auto kern = distill_forward_kernel<T, NT, TAIL, decltype(split_tag)::value>;
+        if (bits > 32 * 1024)
+          KB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bits));
+        launch_rows(kern, rows, NT, how.parts, (size_t)bits, s, (const T*)logits.data_ptr(), logits.stride(0),
+                    (int)vocab, ids.data_ptr<int64_t>(), teacher.data_ptr<float>(), k, c, inv_t, w,
+                    loss.data_ptr<float>(), stats.data_ptr<float>());
+      });
+    });
   });
   KB_LAUNCHED();
 }
 
+// Gradient of sum(row_scale * loss) * scale; with `unless_one`, `out` stays as it is where the scale is one.
 void topk_distillation_backward(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher,
                                 const at::Tensor& stats, const c10::optional<at::Tensor>& row_scale,
-                                const c10::optional<at::Tensor>& scale, at::Tensor& out, int64_t vocab,
-                                double temperature, bool tail) {
+                                const c10::optional<at::Tensor>& scale, const at::Tensor& out, int64_t vocab,
+                                double temperature, bool tail, bool unless_one) {
   const int64_t rows = check_logits(logits, vocab, temperature, "logits");
   check_out(out, logits, vocab);
   const int k = check_teacher(ids, teacher, rows, logits);
@@ -280,14 +624,15 @@ void topk_distillation_backward(const at::Tensor& logits, const at::Tensor& ids,
   for_logits_type(logits.scalar_type(), [&](auto tag) {
     using T = typename decltype(tag)::type;
     const int nseg = row_segments(rows, vocab, sizeof(T), 256, logits.get_device());
-    auto launch = [&](auto kern) {
-      kern<<<dim3((unsigned)rows, nseg), 256, 0, s>>>(
-          (const T*)logits.data_ptr(), logits.stride(0), (T*)out.data_ptr(), out.stride(0), (int)vocab,
+    // Blocks that most often return at once are few, and take several rows where they do not.
+    const int64_t blocks = unless_one ? std::min<int64_t>(rows, 8 * (int64_t)num_sms(logits.get_device())) : rows;
+    for_bool(tail, [&](auto tail_tag) {
+      distill_backward_kernel<T, 256, decltype(tail_tag)::value><<<dim3((unsigned)blocks, nseg), 256, 0, s>>>(
+          (const T*)logits.data_ptr(), logits.stride(0), (T*)out.data_ptr(), out.stride(0), (int)vocab, rows,
           ids.data_ptr<int64_t>(), teacher.data_ptr<float>(), k, c, (float)(1.0 / temperature),
           stats.data_ptr<float>(), row_scale ? row_scale->data_ptr<float>() : nullptr,
-          scale ? scale->data_ptr<float>() : nullptr);
-    };
-    tail ? launch(distill_backward_kernel<T, 256, true>) : launch(distill_backward_kernel<T, 256, false>);
+          scale ? scale->data_ptr<float>() : nullptr, unless_one);
+    });
   });
   KB_LAUNCHED();
 }

@@ -357,15 +357,36 @@ def token_logprobs_ref(logits, tokens, *, top_k: int = 0, temperature: float = 1
     return logprobs, torch.where(counted, entropy, 0.0), top_logprobs, top_ids
 
 
-def topk_distillation_forward(logits, teacher_ids, teacher_logits, *, temperature: float = 1.0, tail: bool = False):
-    """Returns (loss rows, stats for the backward pass) of 2-D ``logits`` and ``[rows, k]`` teachers."""
+def topk_distillation_forward(logits, teacher_ids, teacher_logits, *, weight=None, temperature: float = 1.0,
+                              tail: bool = False):
+    """Returns (loss rows, stats for the backward pass) of 2-D ``logits`` and ``[rows, k]`` teachers.
+
+    ``weight`` (fp32 rows) multiplies the losses; rows of weight zero are not read.
+    """
 
     rows, vocab = logits.shape
     loss = torch.empty(rows, device=logits.device, dtype=torch.float32)
     stats = torch.empty((rows, native().TOPK_DISTILLATION_STATS), device=logits.device, dtype=torch.float32)
-    native().topk_distillation_forward(logits, teacher_ids, teacher_logits, loss, stats, int(vocab),
+    native().topk_distillation_forward(logits, teacher_ids, teacher_logits, weight, loss, stats, None, int(vocab),
                                        float(temperature), bool(tail))
     return loss, stats
+
+
+def topk_distillation_grad(logits, teacher_ids, teacher_logits, *, weight=None, temperature: float = 1.0,
+                           tail: bool = False, out: Optional[torch.Tensor] = None):
+    """Forward and backward in one kernel: (weighted loss rows, stats, gradient of their sum).
+
+    The logits are read from memory once; ``out=logits`` overwrites them with
+    their gradient.
+    """
+
+    rows, vocab = logits.shape
+    loss = torch.empty(rows, device=logits.device, dtype=torch.float32)
+    stats = torch.empty((rows, native().TOPK_DISTILLATION_STATS), device=logits.device, dtype=torch.float32)
+    out = _like_rows(logits) if out is None else out
+    native().topk_distillation_forward(logits, teacher_ids, teacher_logits, weight, loss, stats, out, int(vocab),
+                                       float(temperature), bool(tail))
+    return loss, stats, out
 
 
 def topk_distillation_backward(logits, teacher_ids, teacher_logits, stats, *, row_scale=None, scale=None,
@@ -378,32 +399,49 @@ def topk_distillation_backward(logits, teacher_ids, teacher_logits, stats, *, ro
 
     out = _like_rows(logits) if out is None else out
     native().topk_distillation_backward(logits, teacher_ids, teacher_logits, stats, row_scale, scale, out,
-                                        int(logits.shape[1]), float(temperature), bool(tail))
+                                        int(logits.shape[1]), float(temperature), bool(tail), False)
     return out
 
 
 class _TopkDistillationFn(torch.autograd.Function):
-    """Loss rows, or with ``weight`` their weighted sum."""
+    """Loss rows, or with ``weight`` their weighted sum.
+
+    The sum's gradient is written by the forward kernel, for an upstream
+    gradient of one, while the row is still in L2; the backward pass leaves it
+    where the upstream gradient is one (told on the device) and computes it
+    anew otherwise, so it is rounded once in either case. fp16 logits, whose
+    loss goes through a gradient scaler, take the two passes at once.
+    """
 
     @staticmethod
     def forward(ctx, logits, ids, teacher, weight, temperature, tail):
         z = _vocab_rows(logits, "topk_distillation")
-        loss, stats = topk_distillation_forward(z, ids, teacher, temperature=temperature, tail=tail)
-        ctx.save_for_backward(logits, ids, teacher, weight, stats)
         ctx.meta = (temperature, tail)
-        if weight is None:
-            return loss
-        return torch.where(weight == 0, 0.0, loss * weight).sum()
+        ctx.dz = None
+        if weight is not None and ctx.needs_input_grad[0] and logits.dtype != torch.float16:
+            loss, stats, ctx.dz = topk_distillation_grad(z, ids, teacher, weight=weight, temperature=temperature,
+                                                         tail=tail)
+        else:
+            loss, stats = topk_distillation_forward(z, ids, teacher, weight=weight, temperature=temperature, tail=tail)
+        ctx.save_for_backward(logits, ids, teacher, weight, stats)
+        return loss if weight is None else loss.sum()
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
         logits, ids, teacher, weight, stats = ctx.saved_tensors
         temperature, tail = ctx.meta
+        z = _vocab_rows(logits, "topk_distillation")
         g = _row_gradient(dloss)
-        dz = topk_distillation_backward(_vocab_rows(logits, "topk_distillation"), ids, teacher, stats,
-                                        row_scale=g if weight is None else weight,
-                                        scale=None if weight is None else g, temperature=temperature, tail=tail)
+        if weight is None:
+            dz = topk_distillation_backward(z, ids, teacher, stats, row_scale=g, temperature=temperature, tail=tail)
+        else:
+            # The gradient is handed out once; a second backward pass computes its own.
+            dz, ctx.dz = ctx.dz, None
+            ready = dz is not None
+            dz = dz if ready else _like_rows(z)
+            native().topk_distillation_backward(z, ids, teacher, stats, weight, g, dz, int(z.shape[1]), temperature,
+                                                tail, ready)
         return dz.view(logits.shape), None, None, None, None, None
 
 

@@ -455,11 +455,13 @@ def test_distillation_shapes(dtype, tail, rows, vocab, k, layout):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("rows,vocab,layout", [(1, 777, "contiguous"), (37, 1001, "offset"), (9, 50257, "padded"),
-                                               (333, 5000, "padded"), (3, 131072, "contiguous")])
+                                               (333, 5000, "padded"), (3, 131072, "contiguous"),
+                                               (333, 1001, "contiguous"), (700, 8223, "offset"), (160, 50257, "padded"),
+                                               (200, 3, "contiguous"), (1200, 9000, "contiguous")])
 @pytest.mark.parametrize("scale", [1.0, 0.375])
 def test_distillation_weighted_sum(dtype, tail, rows, vocab, layout, scale):
     z = _logits(rows, vocab, dtype, layout)
-    ids, t = _teacher(rows, vocab, 12, tail)
+    ids, t = _teacher(rows, vocab, min(12, vocab - 1), tail)
     weight = torch.rand(rows, device=DEV) + 0.1
     weight[rows // 2::4] = 0
     z[rows // 2::4] = math.nan  # rows of weight zero are left out
@@ -516,6 +518,34 @@ def test_distillation_rows_without_slots_are_not_read():
         (dz,) = torch.autograd.grad(loss.sum(), z)
         assert loss[0] == 0 and loss[2] == 0 and loss[1] > 0
         assert not dz[0].any() and not dz[2].any() and dz[1].isfinite().all()
+
+
+@gpu
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("left_out", [lambda i: i % 2 == 0, lambda i: i % 2 == 1, lambda i: i < 300, lambda i: i > 40,
+                                      lambda i: i % 3 != 0, lambda i: (i // 200) % 2 == 0, lambda i: i >= 0])
+@pytest.mark.parametrize("how", ["weight", "slots"])
+def test_rows_left_out_in_any_order(tail, left_out, how):
+    """Loss and gradient together, blocks taking several rows each, with rows left out between them."""
+
+    rows, vocab = 2500, 2100
+    z = _logits(1, vocab, torch.bfloat16, "contiguous").repeat(rows, 1)
+    z += torch.randn_like(z[:, :1])
+    ids, t = _teacher(1, vocab, 7, tail, ragged=False)
+    ids, t = ids.repeat(rows, 1), t.repeat(rows, 1)
+    out = torch.tensor([left_out(i) for i in range(rows)], device=DEV)
+    weight = torch.rand(rows, device=DEV) + 0.5
+    if how == "weight":
+        weight[out] = 0
+    else:
+        ids[out] = -1
+    loss, stats, dz = kf.topk_distillation_grad(z, ids, t, weight=weight, tail=tail)
+    apart, _ = kf.topk_distillation_forward(z, ids, t, weight=weight, tail=tail)
+    assert not loss[out].any() and not dz[out].any() and (stats[~out, -1] == 1).all()
+    # Both kernels are within the loss's tolerance of the exact value (16 + log V covers |log p| here).
+    _close(loss, apart, 2 * weight.double().cpu() * (16 + math.log(vocab)) * 2.0**-20, "loss")
+    back = kf.topk_distillation_backward(z, ids, t, stats, row_scale=weight, tail=tail)
+    assert torch.equal(back, dz)
 
 
 @gpu
