@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(NT)
   }
   __shared__ Acc join_sm[NT / 32], result;
   __shared__ std::conditional_t<TOPK, SelectShared<NT>, int> sh;
-  stream_units<T, NT, true, false>(FromMemory{row.unit_ptr()}, u0, u1, c, run, nullptr, [&](int batch, float mx) {
+  stream_units<T, NT, true>(FromMemory{row.unit_ptr()}, u0, u1, c, run, NoMarks{}, [&](int batch, float mx) {
     if constexpr (TOPK) {
       mine = max_nan(mine, mx);
       float& kept = sh.group_max[batch % sh.kGroups][tid];

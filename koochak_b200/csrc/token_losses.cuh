@@ -222,7 +222,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 template <bool ENT>
 struct Run {
   float m = -INFINITY, ms = 0.f;  // maximum, and the finite value to subtract
-  F2 s = 0, a = 0;
+  F2 s{}, a{};
   // Takes the maximum up to the lanes' `wide`; called by whole warps.
   __device__ __forceinline__ void raise(float wide, float c) {
     if (!__any_sync(0xffffffffu, !(wide <= m))) return;
@@ -281,26 +281,61 @@ __device__ __forceinline__ void store_unit(uint4* p, const uint4& q) {
                : "memory");
 }
 
-// Masks the elements of unit `u` whose bit is set (bit = u * E + j).
+// Masks the elements of a unit whose bit is set in `b`.
 template <typename T>
-__device__ __forceinline__ void mask_unit(uint4& q, const uint8_t* bits, int u) {
-  constexpr int E = Elem<T>::kUnit;
-  uint32_t b = E == 8 ? bits[u] : (bits[u >> 1] >> ((u & 1) * 4)) & 15u;
-  if (b == 0) return;
+__device__ __forceinline__ void mask_unit(uint4& q, uint32_t b) {
   uint32_t* w = reinterpret_cast<uint32_t*>(&q);
-  if (E == 8) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = (b >> (2 * i)) & 1u, hi = (b >> (2 * i + 1)) & 1u;
-      const uint32_t keep = (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
+  for (int i = 0; i < 4; ++i) {
+    if (Elem<T>::kUnit == 8) {
+      const uint32_t keep = ((b >> (2 * i)) & 1u ? 0u : 0xFFFFu) | ((b >> (2 * i + 1)) & 1u ? 0u : 0xFFFF0000u);
       w[i] = (w[i] & keep) | (Elem<T>::kNegInf & ~keep);
+    } else if ((b >> i) & 1u) {
+      w[i] = Elem<T>::kNegInf;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if ((b >> i) & 1u) w[i] = Elem<T>::kNegInf;
   }
 }
+
+// Marks of elements of a part of a row: the bits of a thread's batch lie together (a byte per unit of eight elements,
+// half a byte per unit of four), so that a thread finds with one load that none of its batch is marked. One more word is
+// for the ragged elements.
+template <typename T, int NT>
+struct Marks {
+  static constexpr int E = Elem<T>::kUnit;
+  uint32_t* words;
+  int u0, u1;
+  __device__ __forceinline__ Marks(uint32_t* w, int first, int last) : words(w), u0(first), u1(last) {}
+  static __host__ __device__ __forceinline__ int size(int units) {
+    return (units + kBatch * NT - 1) / (kBatch * NT) * (NT * E / 8) + 1;
+  }
+  // The place of a token's bit, if it lies in this part.
+  __device__ __forceinline__ bool place(const Row<T>& row, int id, bool ragged_too, int& bit) const {
+    const int at = id - row.head;
+    if (at < 0 || at >= row.units * E) {
+      bit = (size(u1 - u0) - 1) * 32 + (at < 0 ? id : id - row.units * E);
+      return ragged_too;
+    }
+    const int u = at / E - u0;
+    bit = ((u / (kBatch * NT) * NT + u % NT) * kBatch + u / NT % kBatch) * E + at % E;
+    return u >= 0 && u < u1 - u0;
+  }
+  // Whether it was marked before.
+  __device__ __forceinline__ bool mark(const Row<T>& row, int id, bool ragged_too) const {
+    int bit;
+    return place(row, id, ragged_too, bit) && ((atomicOr(words + bit / 32, 1u << (bit % 32)) >> (bit % 32)) & 1u);
+  }
+  // Forgets all marks next to a token's.
+  __device__ __forceinline__ void unmark(const Row<T>& row, int id) const {
+    int bit;
+    if (place(row, id, true, bit)) words[bit / 32] = 0;
+  }
+  __device__ __forceinline__ bool ragged(int i) const { return (words[size(u1 - u0) - 1] >> i) & 1u; }
+  __device__ __forceinline__ uint32_t of_batch(int batch) const {
+    const int at = batch * NT + threadIdx.x;
+    return E == 8 ? words[at] : reinterpret_cast<const uint16_t*>(words)[at];
+  }
+};
+struct NoMarks {};
 
 // Where a row's units come from: memory, or units [u0, ..) staged in shared memory.
 struct FromMemory {
@@ -315,9 +350,10 @@ struct FromMemory {
 // maximum, and in pairs a subtraction, a product, two 2^x and one or two sums.
 // Clamping the masked entries' exponents would cost one more instruction per
 // element; instead a batch whose A came out NaN (0 times -inf) takes its A again.
-template <typename T, int NT, bool ENT, bool MASK, typename Src, typename G>
-__device__ __forceinline__ void stream_units(const Src& src, int u0, int u1, float c, Run<ENT>& run,
-                                             const uint8_t* bits, const G& batch_max) {
+template <typename T, int NT, bool ENT, typename Src, typename M, typename G>
+__device__ __forceinline__ void stream_units(const Src& src, int u0, int u1, float c, Run<ENT>& run, const M& marks,
+                                             const G& batch_max) {
+  constexpr bool MASK = !std::is_same_v<M, NoMarks>;
   static_assert(!(ENT && MASK), "the masked form takes no entropy");
   constexpr int UN = kBatch, E = Elem<T>::kUnit;
   const F2 cc = pair(c, c);
@@ -337,10 +373,13 @@ __device__ __forceinline__ void stream_units(const Src& src, int u0, int u1, flo
         if (u + i * NT < u1) q[i] = src.load(u + i * NT);
       }
     }
-    if (MASK) {
+    if constexpr (MASK) {
+      const uint32_t set = marks.of_batch(batch);
+      if (set) {
 #pragma unroll
-      for (int i = 0; i < UN; ++i)
-        if (u + i * NT < u1) mask_unit<T>(q[i], bits, u + i * NT);
+        for (int i = 0; i < UN; ++i)
+          if ((set >> (E * i)) & ((1u << E) - 1u)) mask_unit<T>(q[i], set >> (E * i));
+      }
     }
     uint32_t mx = Elem<T>::max2(Elem<T>::max2(q[0].x, q[0].y), Elem<T>::max2(q[0].z, q[0].w));
 #pragma unroll

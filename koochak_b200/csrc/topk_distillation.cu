@@ -138,19 +138,6 @@ __device__ __forceinline__ float row_loss(const Acc& str, const ListStats& list,
   return loss;
 }
 
-// A bit per element: u * E + j for element j of unit u, the ragged elements behind the units.
-template <typename T>
-__device__ __forceinline__ int bit_of(const Row<T>& row, int id) {
-  const int body = row.units * Elem<T>::kUnit;
-  return id < row.head ? body + id : id < row.head + body ? id - row.head : id;
-}
-// Sets a bit; whether it was set before.
-__device__ __forceinline__ bool mark(uint8_t* bits, int bit) {
-  return (atomicOr(reinterpret_cast<uint32_t*>(bits) + (bit >> 5), 1u << (bit & 31)) >> (bit & 31)) & 1u;
-}
-__device__ __forceinline__ void unmark(uint8_t* bits, int bit) { reinterpret_cast<uint32_t*>(bits)[bit >> 5] = 0; }
-__device__ __forceinline__ bool marked(const uint8_t* bits, int bit) { return (bits[bit >> 3] >> (bit & 7)) & 1u; }
-
 // Gradient of the listed elements among units [u0, u1) and, if asked, the ragged ones: sums the q of slots that name
 // the same token.
 template <typename T>
@@ -189,17 +176,16 @@ __device__ __forceinline__ void write_gradient(const Row<T>& row, T* out, int u0
 }
 
 // Loss of each row, times its weight: a block per row, or with SPLIT a cluster of blocks that share it. Off-list
-// elements are told by a bit per element in shared memory (TAIL).
+// elements are told by marks in shared memory (TAIL).
 template <typename T, int NT, bool TAIL, bool SPLIT>
 __global__ void __launch_bounds__(NT)
     distill_forward_kernel(const T* __restrict__ logits, long long ld, int V, const int64_t* __restrict__ ids,
                            const float* __restrict__ teacher, int K, float c, float inv_t,
                            const float* __restrict__ weight, float* __restrict__ loss, float* __restrict__ stats) {
   namespace cg = cooperative_groups;
-  extern __shared__ __align__(16) uint8_t bits[];
+  extern __shared__ uint32_t words[];
   __shared__ ListShared sh;
   __shared__ Acc join_sm[NT / 32], result;
-  constexpr int E = Elem<T>::kUnit;
   const int tid = threadIdx.x;
   int part = 0, parts = 1;
   if constexpr (SPLIT) {
@@ -212,11 +198,10 @@ __global__ void __launch_bounds__(NT)
   segment(row.units, part, parts, u0, u1);
   const int ragged = part == 0 ? row.ragged : 0;
   const float w = weight ? weight[row_i] : 1.f;
+  const Marks<T, NT> marks(words, u0, u1);
   if (tid == 0) sh.repeated = 0;
-  if (TAIL) {
-    uint32_t* words = reinterpret_cast<uint32_t*>(bits);
-    for (int i = tid; i < (V + 31) / 32; i += NT) words[i] = 0;
-  }
+  if (TAIL)
+    for (int i = tid; i < Marks<T, NT>::size(u1 - u0); i += NT) words[i] = 0;
   const bool some = w != 0.f && read_slots<T, NT>(row.z, V, ids + row_i * K, teacher + row_i * K, K, sh);
   if (!some) {
     if (part == 0 && tid == 0) loss[row_i] = 0.f;
@@ -226,14 +211,20 @@ __global__ void __launch_bounds__(NT)
   Run<false> run;
   if (TAIL) {
     for (int i = tid; i < K; i += NT)
-      if (sh.id[i] >= 0 && mark(bits, bit_of(row, sh.id[i]))) sh.repeated = 1;
+      if (sh.id[i] >= 0 && marks.mark(row, sh.id[i], part == 0)) sh.repeated = 1;
+    // A block of a cluster sees the marks of its part only.
+    for (int i = tid % kMaxList; SPLIT && i < K; i += kMaxList)
+      for (int j = tid / kMaxList; j < i; j += NT / kMaxList)
+        if (sh.id[i] >= 0 && sh.id[i] == sh.id[j]) sh.repeated = 1;
     __syncthreads();
   }
   if (tid < 32) {  // fewer than two units of ragged elements
-    const bool in = tid < ragged && (!TAIL || !marked(bits, row.units * E + tid));
+    const bool in = tid < ragged && (!TAIL || !marks.ragged(tid));
     run.add_one(in ? Elem<T>::load(row.z + row.ragged_index(tid)) : -INFINITY, c);
   }
-  stream_units<T, NT, false, TAIL>(FromMemory{row.unit_ptr()}, u0, u1, c, run, bits, [](int, float) {});
+  const FromMemory src{row.unit_ptr()};
+  if constexpr (TAIL) stream_units<T, NT>(src, u0, u1, c, run, marks, [](int, float) {});
+  else stream_units<T, NT>(src, u0, u1, c, run, NoMarks{}, [](int, float) {});
   Acc all = block_join<NT, false>(run, c, join_sm);
   if constexpr (SPLIT) {
     if (tid == 0) result = all;
@@ -262,7 +253,7 @@ struct FromStage {
   uint32_t parity;
   volatile int* abort_flag;
   int* status;
-  // Waits for the batch's chunk; a copy that does not arrive is recorded, and the host raises on it.
+  // Waits for the batch's chunk to be there; a copy that does not arrive is recorded, and the host raises on it.
   __device__ __forceinline__ void begin(int batch) const {
     mbar_wait(&full[batch], parity, abort_flag, status, kStatusTimeoutRowStage);
   }
@@ -285,21 +276,21 @@ struct GradShared {
   ListShared list[2];
   KdStats stats;
   float weight[2];
-  int some[2];
-  uint64_t full[kChunks], empty[kChunks], ready, joined, solved, done;
+  int some[2], fetch[2];
+  uint64_t full[kChunks], empty[kChunks], told, ready, joined, solved, done;
   int abort_flag;
 };
 
 template <typename T, int NT, bool TAIL>
-__global__ void __launch_bounds__(NT + 32, 1024 / NT)
+__global__ void __launch_bounds__(NT + 64, 1024 / NT)
     distill_grad_kernel(const T* logits, long long ld, T* out, long long ld_out, int V, long long rows,
                         const int64_t* __restrict__ ids, const float* __restrict__ teacher, int K, float c, float inv_t,
                         const float* __restrict__ weight, float* __restrict__ loss, float* __restrict__ stats,
                         int stage_units, int* status) {
   extern __shared__ __align__(128) uint8_t dynamic[];
-  constexpr int E = Elem<T>::kUnit, NW = NT / 32, kChunk = kBatch * NT;  // units of a batch of the streaming warps
+  constexpr int NW = NT / 32, kChunk = kBatch * NT;  // units of a batch of the streaming warps
   uint4* stage = reinterpret_cast<uint4*>(dynamic);
-  uint8_t* bits = dynamic + 16 * (size_t)stage_units;
+  uint32_t* words = reinterpret_cast<uint32_t*>(dynamic + 16 * (size_t)stage_units);
   __shared__ GradShared sh;
   __shared__ Acc sums[NW];
   const int tid = threadIdx.x, lane = tid & 31;
@@ -309,21 +300,22 @@ __global__ void __launch_bounds__(NT + 32, 1024 / NT)
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.empty[i], NW);
     }
+    mbar_init(&sh.told, 1);
     mbar_init(&sh.ready, 1);
     mbar_init(&sh.joined, NW);
     mbar_init(&sh.solved, 1);
-    mbar_init(&sh.done, NW);
+    mbar_init(&sh.done, NW + 1);
     sh.abort_flag = 0;
     fence_barrier_init();
   }
-  for (int i = tid; i < (V + 31) / 32; i += NT + 32) reinterpret_cast<uint32_t*>(bits)[i] = 0;
+  for (int i = tid; i < Marks<T, NT>::size(stage_units); i += NT + 64) words[i] = 0;
   __syncthreads();
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     mbar_wait(bar, parity & 1u, &sh.abort_flag, status, kStatusTimeoutRowStage);
   };
-  // Rows so far, and rows with slots: `full` and `empty` complete once per row with slots, the other barriers once per
-  // row, each only after everyone who waits on it has seen the row before: ready(n + 1) follows joined(n), joined and
-  // done(n + 1) follow solved(n + 1), and that follows done(n).
+  // Rows so far, and rows with slots: `full` and `empty` complete once per row with slots, the other barriers
+  // once per row, each only after everyone who waits on it has seen the row before: told, joined and solved(n + 1) follow
+  // done(n), ready(n + 1) follows joined(n), and done(n) needs every warp to have seen solved or told(n).
   uint32_t count = 0, staged = 0;
 
   if (tid < NT) {
@@ -344,8 +336,10 @@ __global__ void __launch_bounds__(NT + 32, 1024 / NT)
       }
       Run<false> run;
       const FromStage src{stage, sh.full, staged & 1u, &sh.abort_flag, status};
-      if (tid < 32) run.add_one(TAIL && tid < row.ragged && marked(bits, row.units * E + tid) ? -INFINITY : rag, c);
-      stream_units<T, NT, false, TAIL>(src, 0, row.units, c, run, bits, [](int, float) {});
+      const Marks<T, NT> marks(words, 0, row.units);
+      if (tid < 32) run.add_one(TAIL && tid < row.ragged && marks.ragged(tid) ? -INFINITY : rag, c);
+      if constexpr (TAIL) stream_units<T, NT>(src, 0, row.units, c, run, marks, [](int, float) {});
+      else stream_units<T, NT>(src, 0, row.units, c, run, NoMarks{}, [](int, float) {});
       const Acc mine = run.total();
       if (lane == 0) {
         sums[tid >> 5] = mine;
@@ -371,6 +365,34 @@ __global__ void __launch_bounds__(NT + 32, 1024 / NT)
       ++staged;
     }
     return;
+  }
+
+  if (tid < NT + 32) {
+    // The fetching warp: told(n) says whether row n of this block has slots, or is behind
+    // the last.
+    for (long long r = blockIdx.x;; r += gridDim.x, ++count) {
+      wait(&sh.told, count);
+      const bool some = sh.fetch[count & 1];
+      __syncwarp();
+      if (lane == 0 && count > 0) mbar_arrive(&sh.done);  // of the row before
+      if (r >= rows) return;
+      if (!some) continue;
+      const Row<T> row(logits + r * ld, V);
+      for (int i = 0; i < chunks; ++i) {
+        if (staged > 0) wait(&sh.empty[i], staged - 1);
+        if (lane == 0) {
+          const int n = min(kChunk, row.units - i * kChunk);
+          if (n > 0) {
+            mbar_arrive_expect_tx(&sh.full[i], (uint32_t)n * 16);
+            bulk_load_1d(stage + i * kChunk, row.unit_ptr() + i * kChunk, (uint32_t)n * 16, &sh.full[i]);
+          } else {
+            mbar_arrive(&sh.full[i]);
+          }
+        }
+        __syncwarp();
+      }
+      ++staged;
+    }
   }
 
   // The serving warp. Slots lane, lane + 32, ... of the row that comes next:
@@ -410,7 +432,7 @@ __global__ void __launch_bounds__(NT + 32, 1024 / NT)
           list.id[i * 32 + lane] = id;
           list.t[i * 32 + lane] = valid(i) ? t[i] : -INFINITY;
           list.z[i * 32 + lane] = z[i];
-          if (id >= 0 && mark(bits, bit_of(row, id))) list.repeated = 1;
+          if (id >= 0 && Marks<T, NT>(words, 0, row.units).mark(row, id, true)) list.repeated = 1;
         }
       }
       __syncwarp();
@@ -424,26 +446,16 @@ __global__ void __launch_bounds__(NT + 32, 1024 / NT)
     if (lane == 0) mbar_arrive(&sh.ready);
     return ls;
   };
-  uint32_t fetched = 0;  // rows whose copies were issued
-  auto fetch = [&](const Row<T>& row, int i) {  // chunk i of a row; every barrier completes once per row
-    if (fetched > 0) wait(&sh.empty[i], fetched - 1);
+  auto tell = [&](uint32_t n, bool some) {
     if (lane == 0) {
-      const int n = min(kChunk, row.units - i * kChunk);
-      if (n > 0) {
-        mbar_arrive_expect_tx(&sh.full[i], (uint32_t)n * 16);
-        bulk_load_1d(stage + i * kChunk, row.unit_ptr() + i * kChunk, (uint32_t)n * 16, &sh.full[i]);
-      } else {
-        mbar_arrive(&sh.full[i]);
-      }
+      sh.fetch[n & 1] = some;
+      mbar_arrive(&sh.told);
     }
     __syncwarp();
   };
   ask(blockIdx.x);
   bool some = any_slot();
-  if (some) {
-    for (int i = 0; i < chunks; ++i) fetch(Row<T>(logits + blockIdx.x * ld, V), i);
-    ++fetched;
-  }
+  tell(0, some);
   ask_logits(blockIdx.x);
   ListStats list = prepare(Row<T>(logits + blockIdx.x * ld, V), 0, some);
   float w_now = w;
@@ -453,6 +465,7 @@ __global__ void __launch_bounds__(NT + 32, 1024 / NT)
     const Row<T> row(logits + r * ld, V), next_row(logits + (next < rows ? next : r) * ld, V);
     ListShared& now = sh.list[count & 1];
     const bool some_next = any_slot();
+    tell(count + 1, some_next);
     ask_logits(next);
     KdStats k;
     Acc all;
@@ -465,19 +478,14 @@ __global__ void __launch_bounds__(NT + 32, 1024 / NT)
     if (lane == 0) mbar_arrive(&sh.solved);
     // The streaming warps are in the second pass, or write zeros.
     const ListStats list_now = list;
-    if (some_next && chunks > 0) fetch(next_row, 0);
     if (some) {
       for (int i = lane; i < K; i += 32)
-        if (now.id[i] >= 0) unmark(bits, bit_of(row, now.id[i]));
+        if (now.id[i] >= 0) Marks<T, NT>(words, 0, row.units).unmark(row, now.id[i]);
       __syncwarp();
     }
     const float w_next = w;
     if (next < rows) list = prepare(next_row, count + 1, some_next);
     ask(next + gridDim.x);
-    if (some_next) {
-      for (int i = 1; i < chunks; ++i) fetch(next_row, i);
-      ++fetched;
-    }
     if (some) {
       const float l = row_loss<TAIL>(all, list_now, k, c, inv_t, K, now);
       if (lane == 0) {
@@ -558,10 +566,12 @@ void topk_distillation_forward(const at::Tensor& logits, const at::Tensor& ids, 
   check_rows(stats, "stats", rows, kStats, at::kFloat, logits);
   if (out) check_out(*out, logits, vocab);
   if (rows == 0) return;
-  const int64_t bits = tail ? (vocab + 31) / 32 * 4 : 0;
   const int device = logits.get_device();
   // Loss and gradient in one kernel where a row fits into half an SM's shared memory and the rows fill the device.
-  const int64_t units = vocab * logits.element_size() / 16, staged = (units * 16 + 127) / 128 * 128 + (vocab + 31) / 32 * 4;
+  const int64_t row_bytes = vocab * logits.element_size(), units = row_bytes / 16;
+  const int grad_threads = row_bytes <= 16384 ? 128 : 512, stage_units = (int)((units + 7) / 8 * 8);
+  const int64_t marks = 4 * (grad_threads == 128 ? Marks<__half, 128>::size(stage_units) : Marks<__half, 512>::size(stage_units));
+  const int64_t staged = 16 * (int64_t)stage_units + marks;
   const bool together = out && staged <= 108 * 1024 && rows >= num_sms(device);
   if (out && !together) {
     topk_distillation_forward(logits, ids, teacher, weight, loss, stats, c10::nullopt, vocab, temperature, tail);
@@ -580,14 +590,14 @@ void topk_distillation_forward(const at::Tensor& logits, const at::Tensor& ids, 
         auto launch = [&](auto kern, int threads) {
           KB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)staged));
           int per_sm = 0;
-          KB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads + 32, (size_t)staged));
+          KB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads + 64, (size_t)staged));
           const int64_t blocks = std::min<int64_t>(rows, (int64_t)std::max(1, per_sm) * num_sms(device));
-          launch_rows(kern, blocks, threads + 32, 1, (size_t)staged, s, (const T*)logits.data_ptr(), logits.stride(0),
+          launch_rows(kern, blocks, threads + 64, 1, (size_t)staged, s, (const T*)logits.data_ptr(), logits.stride(0),
                       (T*)out->data_ptr(), out->stride(0), (int)vocab, rows, ids.data_ptr<int64_t>(),
                       teacher.data_ptr<float>(), k, c, inv_t, w, loss.data_ptr<float>(), stats.data_ptr<float>(),
-                      (int)((units * 16 + 127) / 128 * 8), device_status_ptr(device));
+                      stage_units, device_status_ptr(device));
         };
-        if (vocab * (int64_t)sizeof(T) <= 16384) launch(distill_grad_kernel<T, 128, TAIL>, 128);
+        if (grad_threads == 128) launch(distill_grad_kernel<T, 128, TAIL>, 128);
         else launch(distill_grad_kernel<T, 512, TAIL>, 512);
         return;
       }
@@ -595,9 +605,9 @@ void topk_distillation_forward(const at::Tensor& logits, const at::Tensor& ids, 
       for_row_launch(how, [&](auto nt_tag, auto split_tag) {
         constexpr int NT = decltype(nt_tag)::value;
         auto kern = distill_forward_kernel<T, NT, TAIL, decltype(split_tag)::value>;
-        if (bits > 32 * 1024)
-          KB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bits));
-        launch_rows(kern, rows, NT, how.parts, (size_t)bits, s, (const T*)logits.data_ptr(), logits.stride(0),
+        const int smem = TAIL ? 4 * Marks<T, NT>::size((int)((units + how.parts - 1) / how.parts)) : 0;
+        if (smem > 32 * 1024) KB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        launch_rows(kern, rows, NT, how.parts, (size_t)smem, s, (const T*)logits.data_ptr(), logits.stride(0),
                     (int)vocab, ids.data_ptr<int64_t>(), teacher.data_ptr<float>(), k, c, inv_t, w,
                     loss.data_ptr<float>(), stats.data_ptr<float>());
       });
