@@ -19,6 +19,7 @@ void register_comm_ops(pybind11::module& m);
 void register_muon_gather_ops(pybind11::module& m);
 void register_token_logprobs_ops(pybind11::module& m);
 void register_topk_distillation_ops(pybind11::module& m);
+void register_token_loss_api(pybind11::module& m);
 }  // namespace kb
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -68,4 +69,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   kb::register_muon_gather_ops(m);
   kb::register_token_logprobs_ops(m);
   kb::register_topk_distillation_ops(m);
+  kb::register_token_loss_api(m);
 }

@@ -8,7 +8,7 @@ namespace kb {
 namespace {
 
 constexpr int kCand = 1024;  // candidates held while the alternatives are selected
-constexpr int kStats = 2;    // floats kept per row for the backward pass: m, log2 S
+constexpr int kStats = kTokenLogprobsStats;  // m, log2 S
 
 // ----------------------------------------------------------- alternatives
 
@@ -289,8 +289,7 @@ __global__ void __launch_bounds__(NT)
       if (tid == 0) {
         logprobs[row_i] = 0.f;
         entropy[row_i] = 0.f;
-        stats[kStats * row_i] = 0.f;
-        stats[kStats * row_i + 1] = 0.f;
+        if (stats) stats[kStats * row_i] = stats[kStats * row_i + 1] = 0.f;
       }
       for (int i = tid; TOPK && i < k; i += NT) {
         top_logprobs[row_i * k + i] = 0.f;
@@ -349,8 +348,10 @@ __global__ void __launch_bounds__(NT)
       logprobs[row_i] = inside ? (Elem<T>::load(row.z + token) - all.m) * inv_t - kLn2 * log2s : NAN;
     }
     entropy[row_i] = kLn2 * (log2s - all.a / all.s);
-    stats[kStats * row_i] = all.m;
-    stats[kStats * row_i + 1] = log2s;
+    if (stats) {
+      stats[kStats * row_i] = all.m;
+      stats[kStats * row_i + 1] = log2s;
+    }
     if (TOPK) {
       result.m = all.m;
       result.s = kLn2 * log2s;
@@ -392,11 +393,11 @@ __global__ void __launch_bounds__(NT)
     logprob_backward_kernel(const T* logits, long long ld, T* out, long long ld_out, int V,
                             const int64_t* __restrict__ tokens, int64_t ignore_index, float c, float inv_t,
                             const float* __restrict__ stats, const float* __restrict__ entropy,
-                            const float* __restrict__ dlogprobs, const float* __restrict__ dentropy) {
+                            RowGrad dlogprobs, RowGrad dentropy) {
   const long long row_i = gridDim.x - 1 - blockIdx.x;  // last rows first: the forward pass left them in L2
   const int64_t token = tokens ? tokens[row_i] : -1;
-  float g = dlogprobs ? dlogprobs[row_i] : 0.f;
-  const float gh = dentropy ? dentropy[row_i] : 0.f;
+  float g = dlogprobs.at(row_i, 0.f);
+  const float gh = dentropy.at(row_i, 0.f);
   int u0, u1;
   if ((tokens && token == ignore_index) || (g == 0.f && gh == 0.f)) {
     const Row<T> row(out + row_i * ld_out, V);
@@ -436,23 +437,22 @@ __global__ void __launch_bounds__(NT)
 
 }  // namespace
 
-void token_logprobs_forward(const at::Tensor& logits, const c10::optional<at::Tensor>& tokens,
-                            const c10::optional<at::Tensor>& logprobs, at::Tensor& entropy, at::Tensor& stats,
-                            const c10::optional<at::Tensor>& top_logprobs, const c10::optional<at::Tensor>& top_ids,
-                            int64_t vocab, double temperature, int64_t ignore_index) {
+void token_logprobs_forward(const at::Tensor& logits, const OptTensor& tokens, const OptTensor& logprobs,
+                            const at::Tensor& entropy, const OptTensor& stats, const OptTensor& top_logprobs,
+                            const OptTensor& top_ids, int64_t vocab, double temperature, int64_t ignore_index) {
   const int64_t rows = check_logits(logits, vocab, temperature, "logits");
   KB_CHECK(tokens.has_value() == logprobs.has_value(), "tokens and logprobs go together");
   KB_CHECK(top_logprobs.has_value() == top_ids.has_value(), "top_logprobs and top_ids go together");
   if (tokens) check_rows(*tokens, "tokens", rows, 1, at::kLong, logits);
   if (logprobs) check_rows(*logprobs, "logprobs", rows, 1, at::kFloat, logits);
   check_rows(entropy, "entropy", rows, 1, at::kFloat, logits);
-  check_rows(stats, "stats", rows, kStats, at::kFloat, logits);
+  if (stats) check_rows(*stats, "stats", rows, kStats, at::kFloat, logits);
   int k = 0;
   if (top_ids) {
-    KB_CHECK(top_ids->dim() == 2, "top_ids must be [rows, k]");
-    KB_CHECK(top_ids->size(1) >= 1 && top_ids->size(1) <= std::min<int64_t>(kMaxList, vocab),
+    KB_CHECK(top_ids->dim() >= 1, "top_ids must be [rows, k]");
+    KB_CHECK(top_ids->size(-1) >= 1 && top_ids->size(-1) <= std::min<int64_t>(kMaxList, vocab),
              "1 to 128 alternatives, and no more than the vocabulary holds");
-    k = (int)top_ids->size(1);
+    k = (int)top_ids->size(-1);
     check_rows(*top_ids, "top_ids", rows, k, at::kLong, logits);
     check_rows(*top_logprobs, "top_logprobs", rows, k, at::kFloat, logits);
   }
@@ -472,25 +472,25 @@ void token_logprobs_forward(const at::Tensor& logits, const c10::optional<at::Te
         constexpr int NT = decltype(nt_tag)::value;
         launch_rows(logprob_forward_kernel<T, NT, decltype(top_tag)::value, decltype(split_tag)::value>, rows, NT,
                     how.parts, 0, s, (const T*)logits.data_ptr(), logits.stride(0), (int)vocab, tok, ignore_index, c,
-                    (float)(1.0 / temperature), k, lp, entropy.data_ptr<float>(), stats.data_ptr<float>(), tl, ti);
+                    (float)(1.0 / temperature), k, lp, entropy.data_ptr<float>(), stats ? stats->data_ptr<float>() : nullptr,
+                    tl, ti);
       });
     });
   });
   KB_LAUNCHED();
 }
 
-void token_logprobs_backward(const at::Tensor& logits, const c10::optional<at::Tensor>& tokens,
-                             const at::Tensor& stats, const at::Tensor& entropy,
-                             const c10::optional<at::Tensor>& dlogprobs, const c10::optional<at::Tensor>& dentropy,
-                             at::Tensor& out, int64_t vocab, double temperature, int64_t ignore_index) {
+void token_logprobs_backward(const at::Tensor& logits, const OptTensor& tokens, const at::Tensor& stats,
+                             const at::Tensor& entropy, const OptTensor& dlogprobs, const OptTensor& dentropy,
+                             const at::Tensor& out, int64_t vocab, double temperature, int64_t ignore_index) {
   const int64_t rows = check_logits(logits, vocab, temperature, "logits");
   check_out(out, logits, vocab);
   if (tokens) check_rows(*tokens, "tokens", rows, 1, at::kLong, logits);
   KB_CHECK(tokens.has_value() || !dlogprobs.has_value(), "dlogprobs without tokens");
   check_rows(stats, "stats", rows, kStats, at::kFloat, logits);
   check_rows(entropy, "entropy", rows, 1, at::kFloat, logits);
-  if (dlogprobs) check_rows(*dlogprobs, "dlogprobs", rows, 1, at::kFloat, logits);
-  if (dentropy) check_rows(*dentropy, "dentropy", rows, 1, at::kFloat, logits);
+  const RowGrad dlp = check_row_grad(dlogprobs, "dlogprobs", rows, logits);
+  const RowGrad dh = check_row_grad(dentropy, "dentropy", rows, logits);
   if (rows == 0) return;
   const c10::cuda::CUDAGuard guard(logits.device());
   cudaStream_t s = c10::cuda::getCurrentCUDAStream().stream();
@@ -501,8 +501,7 @@ void token_logprobs_backward(const at::Tensor& logits, const c10::optional<at::T
     logprob_backward_kernel<T, 256><<<dim3((unsigned)rows, nseg), 256, 0, s>>>(
         (const T*)logits.data_ptr(), logits.stride(0), (T*)out.data_ptr(), out.stride(0), (int)vocab,
         tokens ? tokens->data_ptr<int64_t>() : nullptr, ignore_index, c, (float)(1.0 / temperature),
-        stats.data_ptr<float>(), entropy.data_ptr<float>(), dlogprobs ? dlogprobs->data_ptr<float>() : nullptr,
-        dentropy ? dentropy->data_ptr<float>() : nullptr);
+        stats.data_ptr<float>(), entropy.data_ptr<float>(), dlp, dh);
   });
   KB_LAUNCHED();
 }

@@ -22,13 +22,14 @@
 #include <type_traits>
 
 #include "host_utils.h"
+#include "token_losses.h"
 
 namespace kb {
 namespace {  // per translation unit: each source compiles its own kernels from these
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kMaxList = 128;  // alternatives, or teacher slots, per row
+constexpr int kMaxList = kMaxTopK;
 
 template <typename T>
 struct Elem;
@@ -538,13 +539,28 @@ void check_rows(const at::Tensor& t, const char* name, int64_t rows, int64_t col
   KB_CHECK(t.is_contiguous() && t.numel() == rows * cols, n + " must be contiguous with one entry per row and column");
 }
 
+// A row gradient: fp32, one per row, contiguous (stride 1) or expanded from one value (stride 0).
+struct RowGrad {
+  const float* p;
+  int stride;
+  __device__ __forceinline__ float at(long long row, float none) const { return p ? p[row * stride] : none; }
+};
+RowGrad check_row_grad(const c10::optional<at::Tensor>& t, const char* name, int64_t rows, const at::Tensor& like) {
+  if (!t) return RowGrad{nullptr, 0};
+  const std::string n(name);
+  KB_CHECK(t->is_cuda() && t->device() == like.device() && t->scalar_type() == at::kFloat, n + " must be fp32 on the logits' device");
+  KB_CHECK(t->dim() == 1 && t->size(0) == rows && (rows <= 1 || t->stride(0) == 1 || t->stride(0) == 0),
+           n + " must hold one value per row, contiguous or expanded");
+  return RowGrad{t->data_ptr<float>(), rows <= 1 || t->stride(0) == 0 ? 0 : 1};
+}
+
 // logits [rows, >= vocab] with unit inner stride; returns the row count.
 int64_t check_logits(const at::Tensor& logits, int64_t vocab, double temperature, const char* name) {
   const std::string n(name);
   check_cuda_tensor(logits, name);
   KB_CHECK(logits.dim() == 2, n + " must be [rows, vocab]");
   KB_CHECK(vocab >= 1 && vocab <= logits.size(1), n + " has fewer columns than the vocabulary");
-  KB_CHECK(vocab <= (1 << 19), "vocabularies of more than 524288 entries are not supported");
+  KB_CHECK(vocab <= kMaxListVocab, "vocabularies of more than 524288 entries are not supported");
   KB_CHECK(logits.size(1) == 1 || logits.stride(1) == 1, n + " must have unit inner stride");
   KB_CHECK(logits.size(0) <= 0x7FFFFFFF / 16, n + " has too many rows");
   KB_CHECK(reinterpret_cast<uintptr_t>(logits.data_ptr()) % logits.element_size() == 0, n + " is misaligned");
@@ -590,6 +606,24 @@ void for_row_launch(const RowLaunch& how, F&& f) {
   else if (how.threads == 128) f(Int<128>{}, std::false_type{});
   else if (how.threads == 256) f(Int<256>{}, std::false_type{});
   else f(Int<512>{}, std::false_type{});
+}
+
+// Lets a kernel use `smem` bytes of dynamic shared memory, once per kernel and size; with `threads`, returns how many
+// of its blocks an SM holds.
+template <typename Kern>
+int allow_smem(Kern kern, size_t smem, int threads, int device) {
+  static std::mutex mu;
+  static std::unordered_map<uint64_t, int> known;
+  const uint64_t key = reinterpret_cast<uint64_t>(reinterpret_cast<const void*>(kern)) * 0x9E3779B97F4A7C15ull ^
+                       ((uint64_t)smem << 16 | (uint64_t)threads << 6 | (uint64_t)device);
+  std::lock_guard<std::mutex> lock(mu);
+  const auto it = known.find(key);
+  if (it != known.end()) return it->second;
+  if (smem > 32 * 1024) KB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  int blocks = 0;
+  if (threads) KB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kern, threads, smem));
+  known.emplace(key, blocks);
+  return blocks;
 }
 
 template <typename... P, typename... A>

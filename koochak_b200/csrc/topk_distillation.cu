@@ -9,7 +9,7 @@ namespace kb {
 namespace {
 
 constexpr int kChunks = 32;  // bulk copies a block stages its units with, at most
-constexpr int kStats = 8;  // floats kept per row for the backward pass: KdStats, the last 0 for a row without slots
+constexpr int kStats = kTopkDistillationStats;  // KdStats, and 0 for a row without slots
 
 // --------------------------------------------------------- distillation
 
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(NT)
   const bool some = w != 0.f && read_slots<T, NT>(row.z, V, ids + row_i * K, teacher + row_i * K, K, sh);
   if (!some) {
     if (part == 0 && tid == 0) loss[row_i] = 0.f;
-    if (part == 0 && tid < kStats) stats[row_i * kStats + tid] = 0.f;
+    if (part == 0 && tid < kStats && stats) stats[row_i * kStats + tid] = 0.f;
     return;
   }
   Run<false> run;
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(NT)
     const float l = row_loss<TAIL>(all, list, r, c, inv_t, K, sh);
     if (tid == 0) {
       loss[row_i] = w * l;
-      store_stats(stats + row_i * kStats, r);
+      if (stats) store_stats(stats + row_i * kStats, r);
     }
   }
 }
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
       const float l = row_loss<TAIL>(all, list_now, k, c, inv_t, K, now);
       if (lane == 0) {
         loss[r] = w_now * l;
-        store_stats(stats + r * kStats, k);
+        if (stats) store_stats(stats + r * kStats, k);
       }
       for (int i = lane; i < K; i += 32) now.q[i] = ex2((now.t[i] - k.t_max) * (TAIL ? kLog2e : c)) * k.inv_e;
     }
@@ -499,8 +499,8 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
       __syncwarp();
       write_listed<T>(row, out + r * ld_out, 0, row.units, true, K, c, w_now * inv_t, k, now, lane, 32);
       ++staged;
-    } else if (lane < kStats) {
-      stats[r * kStats + lane] = 0.f;
+    } else {
+      if (stats && lane < kStats) stats[r * kStats + lane] = 0.f;
       if (lane == 0) loss[r] = 0.f;
     }
     __syncwarp();
@@ -514,15 +514,15 @@ template <typename T, int NT, bool TAIL>
 __global__ void __launch_bounds__(NT)
     distill_backward_kernel(const T* logits, long long ld, T* out, long long ld_out, int V, long long rows,
                             const int64_t* __restrict__ ids, const float* __restrict__ teacher, int K, float c,
-                            float inv_t, const float* __restrict__ stats, const float* __restrict__ row_scale,
-                            const float* __restrict__ scale, bool unless_one) {
+                            float inv_t, const float* __restrict__ stats, RowGrad row_scale, const float* __restrict__ scale,
+                            bool unless_one) {
   __shared__ ListShared sh;
   const float factor = scale ? *scale : 1.f;
   if (unless_one && factor == 1.f) return;
   for (long long i = blockIdx.x; i < rows; i += gridDim.x) {
     const long long row_i = rows - 1 - i;  // last rows first: the forward pass left them in L2
     const float* s = stats + row_i * kStats;
-    const float w = row_scale ? row_scale[row_i] : 1.f;
+    const float w = row_scale.at(row_i, 1.f);
     T* o = out + row_i * ld_out;
     int u0, u1;
     if (s[7] == 0.f || w == 0.f) {
@@ -550,20 +550,14 @@ int check_teacher(const at::Tensor& ids, const at::Tensor& teacher, int64_t rows
 }
 }  // namespace
 
-void topk_distillation_backward(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher,
-                                const at::Tensor& stats, const c10::optional<at::Tensor>& row_scale,
-                                const c10::optional<at::Tensor>& scale, const at::Tensor& out, int64_t vocab,
-                                double temperature, bool tail, bool unless_one);
-
-// With `out`, the gradient of the weighted sum of losses is written too (it may be the logits themselves).
 void topk_distillation_forward(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher,
-                               const c10::optional<at::Tensor>& weight, at::Tensor& loss, at::Tensor& stats,
-                               const c10::optional<at::Tensor>& out, int64_t vocab, double temperature, bool tail) {
+                               const OptTensor& weight, const at::Tensor& loss, const OptTensor& stats,
+                               const OptTensor& out, int64_t vocab, double temperature, bool tail) {
   const int64_t rows = check_logits(logits, vocab, temperature, "logits");
   const int k = check_teacher(ids, teacher, rows, logits);
   if (weight) check_rows(*weight, "weight", rows, 1, at::kFloat, logits);
   check_rows(loss, "loss", rows, 1, at::kFloat, logits);
-  check_rows(stats, "stats", rows, kStats, at::kFloat, logits);
+  if (stats) check_rows(*stats, "stats", rows, kStats, at::kFloat, logits);
   if (out) check_out(*out, logits, vocab);
   if (rows == 0) return;
   const int device = logits.get_device();
@@ -574,28 +568,27 @@ void topk_distillation_forward(const at::Tensor& logits, const at::Tensor& ids, 
   const int64_t staged = 16 * (int64_t)stage_units + marks;
   const bool together = out && staged <= 108 * 1024 && rows >= num_sms(device);
   if (out && !together) {
+    KB_CHECK(stats.has_value(), "the gradient needs stats");
     topk_distillation_forward(logits, ids, teacher, weight, loss, stats, c10::nullopt, vocab, temperature, tail);
-    topk_distillation_backward(logits, ids, teacher, stats, weight, c10::nullopt, *out, vocab, temperature, tail, false);
+    topk_distillation_backward(logits, ids, teacher, *stats, weight, c10::nullopt, *out, vocab, temperature, tail, false);
     return;
   }
   const c10::cuda::CUDAGuard guard(logits.device());
   cudaStream_t s = c10::cuda::getCurrentCUDAStream().stream();
   const float c = (float)(1.4426950408889634 / temperature), inv_t = (float)(1.0 / temperature);
   const float* w = weight ? weight->data_ptr<float>() : nullptr;
+  float* kept = stats ? stats->data_ptr<float>() : nullptr;
   for_logits_type(logits.scalar_type(), [&](auto tag) {
     using T = typename decltype(tag)::type;
     for_bool(tail, [&](auto tail_tag) {
       constexpr bool TAIL = decltype(tail_tag)::value;
       if (together) {
         auto launch = [&](auto kern, int threads) {
-          KB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)staged));
-          int per_sm = 0;
-          KB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads + 64, (size_t)staged));
+          const int per_sm = allow_smem(kern, (size_t)staged, threads + 64, device);
           const int64_t blocks = std::min<int64_t>(rows, (int64_t)std::max(1, per_sm) * num_sms(device));
           launch_rows(kern, blocks, threads + 64, 1, (size_t)staged, s, (const T*)logits.data_ptr(), logits.stride(0),
                       (T*)out->data_ptr(), out->stride(0), (int)vocab, rows, ids.data_ptr<int64_t>(),
-                      teacher.data_ptr<float>(), k, c, inv_t, w, loss.data_ptr<float>(), stats.data_ptr<float>(),
-                      stage_units, device_status_ptr(device));
+                      teacher.data_ptr<float>(), k, c, inv_t, w, loss.data_ptr<float>(), kept, stage_units, device_status_ptr(device));
         };
         if (grad_threads == 128) launch(distill_grad_kernel<T, 128, TAIL>, 128);
         else launch(distill_grad_kernel<T, 512, TAIL>, 512);
@@ -606,26 +599,24 @@ void topk_distillation_forward(const at::Tensor& logits, const at::Tensor& ids, 
         constexpr int NT = decltype(nt_tag)::value;
         auto kern = distill_forward_kernel<T, NT, TAIL, decltype(split_tag)::value>;
         const int smem = TAIL ? 4 * Marks<T, NT>::size((int)((units + how.parts - 1) / how.parts)) : 0;
-        if (smem > 32 * 1024) KB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        if (smem > 32 * 1024) allow_smem(kern, (size_t)smem, 0, device);
         launch_rows(kern, rows, NT, how.parts, (size_t)smem, s, (const T*)logits.data_ptr(), logits.stride(0),
                     (int)vocab, ids.data_ptr<int64_t>(), teacher.data_ptr<float>(), k, c, inv_t, w,
-                    loss.data_ptr<float>(), stats.data_ptr<float>());
+                    loss.data_ptr<float>(), kept);
       });
     });
   });
   KB_LAUNCHED();
 }
 
-// Gradient of sum(row_scale * loss) * scale; with `unless_one`, `out` stays as it is where the scale is one.
 void topk_distillation_backward(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher,
-                                const at::Tensor& stats, const c10::optional<at::Tensor>& row_scale,
-                                const c10::optional<at::Tensor>& scale, const at::Tensor& out, int64_t vocab,
-                                double temperature, bool tail, bool unless_one) {
+                                const at::Tensor& stats, const OptTensor& row_scale, const OptTensor& scale,
+                                const at::Tensor& out, int64_t vocab, double temperature, bool tail, bool unless_one) {
   const int64_t rows = check_logits(logits, vocab, temperature, "logits");
   check_out(out, logits, vocab);
   const int k = check_teacher(ids, teacher, rows, logits);
   check_rows(stats, "stats", rows, kStats, at::kFloat, logits);
-  if (row_scale) check_rows(*row_scale, "row_scale", rows, 1, at::kFloat, logits);
+  const RowGrad row_grad = check_row_grad(row_scale, "row_scale", rows, logits);
   if (scale) check_rows(*scale, "scale", 1, 1, at::kFloat, logits);
   if (rows == 0) return;
   const c10::cuda::CUDAGuard guard(logits.device());
@@ -640,7 +631,7 @@ void topk_distillation_backward(const at::Tensor& logits, const at::Tensor& ids,
       distill_backward_kernel<T, 256, decltype(tail_tag)::value><<<dim3((unsigned)blocks, nseg), 256, 0, s>>>(
           (const T*)logits.data_ptr(), logits.stride(0), (T*)out.data_ptr(), out.stride(0), (int)vocab, rows,
           ids.data_ptr<int64_t>(), teacher.data_ptr<float>(), k, c, (float)(1.0 / temperature),
-          stats.data_ptr<float>(), row_scale ? row_scale->data_ptr<float>() : nullptr,
+          stats.data_ptr<float>(), row_grad,
           scale ? scale->data_ptr<float>() : nullptr, unless_one);
     });
   });

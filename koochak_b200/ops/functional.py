@@ -228,10 +228,6 @@ def _check_temperature(temperature: float, name: str) -> None:
         raise ValueError(f"{name}: temperature must lie in [1e-4, 1e4], got {temperature}")
 
 
-def _row_gradient(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if g is None else g.float().reshape(-1).contiguous()
-
-
 def _like_rows(z: torch.Tensor) -> torch.Tensor:
     """An uninitialised [rows, vocab] tensor whose rows start where ``z``'s do modulo 16 bytes, if z's rows do not
     overlap."""
@@ -274,32 +270,6 @@ def token_logprobs_backward(logits, tokens, stats, entropy, dlogprobs, dentropy,
     return out
 
 
-class _TokenLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, top_k, temperature, ignore_index):
-        z = _vocab_rows(logits, "token_logprobs")
-        logprobs, entropy, stats, top_logprobs, top_ids = token_logprobs_forward(
-            z, tokens, top_k=top_k, temperature=temperature, ignore_index=ignore_index)
-        ctx.save_for_backward(logits, tokens, stats, entropy)
-        ctx.meta = (temperature, ignore_index)
-        ctx.set_materialize_grads(False)
-        if top_k:
-            ctx.mark_non_differentiable(top_logprobs, top_ids)
-        return logprobs, entropy, top_logprobs, top_ids
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dlogprobs, dentropy, _dtop, _dids):
-        logits, tokens, stats, entropy = ctx.saved_tensors
-        if dlogprobs is None and dentropy is None:
-            return None, None, None, None, None
-        temperature, ignore_index = ctx.meta
-        dz = token_logprobs_backward(_vocab_rows(logits, "token_logprobs"), tokens, stats, entropy,
-                                     _row_gradient(dlogprobs), _row_gradient(dentropy), temperature=temperature,
-                                     ignore_index=ignore_index)
-        return dz.view(logits.shape), None, None, None, None
-
-
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, top_k: int = 0,
                    temperature: float = 1.0, ignore_index: int = -100) -> TokenLogprobs:
     """Log probabilities of given tokens, entropies and the most likely alternatives, in one pass over the logits.
@@ -317,21 +287,20 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     rank above all others.
     """
 
+    if use_native(logits):
+        return TokenLogprobs(*native().token_logprobs(logits, tokens, top_k, temperature, ignore_index))
     name = "token_logprobs"
-    lead, vocab = logits.shape[:-1], logits.shape[-1]
     z = _vocab_rows(logits, name)
+    lead, vocab = logits.shape[:-1], logits.shape[-1]
     _check_temperature(temperature, name)
     if not 0 <= top_k <= min(MAX_TOP_K, vocab):
         raise ValueError(f"{name}: top_k must lie in [0, {min(MAX_TOP_K, vocab)}], got {top_k}")
     if tokens is not None:
         if tokens.shape != lead or tokens.dtype != torch.int64 or tokens.device != logits.device:
             raise ValueError(f"{name}: tokens must be int64 of shape {tuple(lead)} on {logits.device}")
-        tokens = tokens.reshape(-1).contiguous()
-    if not use_native(logits):
-        res = token_logprobs_ref(z, tokens, top_k=top_k, temperature=temperature, ignore_index=ignore_index)
-    else:
-        res = _TokenLogprobsFn.apply(logits, tokens, int(top_k), float(temperature), int(ignore_index))
-    logprobs, entropy, top_logprobs, top_ids = res
+        tokens = tokens.reshape(-1)
+    logprobs, entropy, top_logprobs, top_ids = token_logprobs_ref(z, tokens, top_k=top_k, temperature=temperature,
+                                                                  ignore_index=ignore_index)
     return TokenLogprobs(None if logprobs is None else logprobs.view(lead), entropy.view(lead),
                          None if top_logprobs is None else top_logprobs.view(*lead, top_k),
                          None if top_ids is None else top_ids.view(*lead, top_k))
@@ -403,48 +372,6 @@ def topk_distillation_backward(logits, teacher_ids, teacher_logits, stats, *, ro
     return out
 
 
-class _TopkDistillationFn(torch.autograd.Function):
-    """Loss rows, or with ``weight`` their weighted sum.
-
-    The sum's gradient is written by the forward kernel, for an upstream
-    gradient of one, while the row is still in L2; the backward pass leaves it
-    where the upstream gradient is one (told on the device) and computes it
-    anew otherwise, so it is rounded once in either case. fp16 logits, whose
-    loss goes through a gradient scaler, take the two passes at once.
-    """
-
-    @staticmethod
-    def forward(ctx, logits, ids, teacher, weight, temperature, tail):
-        z = _vocab_rows(logits, "topk_distillation")
-        ctx.meta = (temperature, tail)
-        ctx.dz = None
-        if weight is not None and ctx.needs_input_grad[0] and logits.dtype != torch.float16:
-            loss, stats, ctx.dz = topk_distillation_grad(z, ids, teacher, weight=weight, temperature=temperature,
-                                                         tail=tail)
-        else:
-            loss, stats = topk_distillation_forward(z, ids, teacher, weight=weight, temperature=temperature, tail=tail)
-        ctx.save_for_backward(logits, ids, teacher, weight, stats)
-        return loss if weight is None else loss.sum()
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dloss):
-        logits, ids, teacher, weight, stats = ctx.saved_tensors
-        temperature, tail = ctx.meta
-        z = _vocab_rows(logits, "topk_distillation")
-        g = _row_gradient(dloss)
-        if weight is None:
-            dz = topk_distillation_backward(z, ids, teacher, stats, row_scale=g, temperature=temperature, tail=tail)
-        else:
-            # The gradient is handed out once; a second backward pass computes its own.
-            dz, ctx.dz = ctx.dz, None
-            ready = dz is not None
-            dz = dz if ready else _like_rows(z)
-            native().topk_distillation_backward(z, ids, teacher, stats, weight, g, dz, int(z.shape[1]), temperature,
-                                                tail, ready)
-        return dz.view(logits.shape), None, None, None, None, None
-
-
 def topk_distillation(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
                       temperature: float = 1.0, tail: bool = False, weight: Optional[torch.Tensor] = None,
                       reduction: str = "none") -> torch.Tensor:
@@ -473,11 +400,14 @@ def topk_distillation(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     """
 
     name = "topk_distillation"
+    if reduction not in ("none", "sum"):
+        raise ValueError(f"{name}: reduction must be 'none' or 'sum', got {reduction!r}")
+    if use_native(logits):
+        return native().topk_distillation(logits, teacher_ids, teacher_logits, temperature, tail, weight,
+                                          reduction == "sum")
     lead = logits.shape[:-1]
     z = _vocab_rows(logits, name)
     _check_temperature(temperature, name)
-    if reduction not in ("none", "sum"):
-        raise ValueError(f"{name}: reduction must be 'none' or 'sum', got {reduction!r}")
     if teacher_ids.dim() != logits.dim() or teacher_ids.shape[:-1] != lead or teacher_ids.dtype != torch.int64:
         raise ValueError(f"{name}: teacher_ids must be int64 of shape {(*lead, 'k')}")
     if teacher_logits.shape != teacher_ids.shape or not teacher_logits.is_floating_point():
@@ -490,18 +420,14 @@ def topk_distillation(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
         if other is not None and other.device != logits.device:
             raise ValueError(f"{name}: all tensors must be on {logits.device}")
     k = teacher_ids.shape[-1]
-    ids = teacher_ids.reshape(-1, k).contiguous()
-    teacher = teacher_logits.detach().reshape(-1, k).float().contiguous()
-    if reduction == "sum" and weight is None:
-        weight = torch.ones(lead, device=logits.device, dtype=torch.float32)
-    weight = None if weight is None else _row_gradient(weight.detach())
-    if not use_native(logits):
-        loss = topk_distillation_ref(z, ids, teacher, temperature=temperature, tail=tail)
-        if weight is not None:
-            return torch.where(weight == 0, 0.0, loss * weight).sum()
-    else:
-        loss = _TopkDistillationFn.apply(logits, ids, teacher, weight, float(temperature), bool(tail))
-    return loss if reduction == "sum" else loss.view(lead)
+    loss = topk_distillation_ref(z, teacher_ids.reshape(-1, k), teacher_logits.detach().reshape(-1, k).float(),
+                                 temperature=temperature, tail=tail)
+    if reduction == "none":
+        return loss.view(lead)
+    if weight is None:
+        return loss.sum()
+    weight = weight.detach().float().reshape(-1)
+    return torch.where(weight == 0, 0.0, loss * weight).sum()
 
 
 def topk_distillation_ref(logits, teacher_ids, teacher_logits, *, temperature: float = 1.0, tail: bool = False):

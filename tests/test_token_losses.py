@@ -239,6 +239,29 @@ def test_refusals(device):
         kf.topk_distillation(z, ids, t, temperature=0)
 
 
+def test_native_refusals_without_a_gpu():
+    """The native entry points raise Python's errors, numbers in their messages included, before they touch a device."""
+
+    from koochak_b200.ops import available, native
+
+    if not available():
+        pytest.skip("native library not built")
+    z, tok = torch.randn(3, 40), torch.zeros(3, dtype=torch.int64)
+    ids, t = torch.zeros(3, 4, dtype=torch.int64), torch.zeros(3, 4)
+    with pytest.raises(ValueError, match="temperature .* got 0.0"):
+        native().token_logprobs(z, tok, 0, 0.0, IGNORE)
+    with pytest.raises(ValueError, match="got 41"):
+        native().token_logprobs(z, tok, 41, 1.0, IGNORE)
+    with pytest.raises(ValueError, match=r"shape \[3\]"):
+        native().token_logprobs(z, tok[:2], 0, 1.0, IGNORE)
+    with pytest.raises(TypeError, match="Double"):
+        native().token_logprobs(z.double(), tok, 0, 1.0, IGNORE)
+    with pytest.raises(ValueError, match=r"\[3\]"):
+        native().topk_distillation(z, ids, t, 1.0, False, z[0], True)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        native().topk_distillation(z, ids, t, 1.0, False, None, False)
+
+
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
 def test_leading_shapes_and_empty_batches(device):
     z = _logits(6, 50, torch.float32, "contiguous", device=device).view(2, 3, 50)
@@ -682,3 +705,25 @@ def test_offsets_beyond_32_bits():
     loss, stats = kf.topk_distillation_forward(z, ids, t, tail=True)
     d = kf.topk_distillation_backward(z, ids, t, stats, tail=True, out=z)
     assert not d[:-3].any() and d[-3:].any(1).all()
+
+
+@gpu
+def test_second_derivatives_are_refused():
+    z = _logits(3, 64, torch.float32, "contiguous").requires_grad_()
+    ids, t = _teacher(3, 64, 4, False, ragged=False)
+    for loss in (kf.token_logprobs(z, _tokens(3, 64, ignored=False)).logprobs.exp().sum(),
+                 kf.topk_distillation(z, ids, t).square().sum()):
+        (g,) = torch.autograd.grad(loss, z, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate"):
+            g.sum().backward()
+
+
+@gpu
+def test_logits_changed_after_the_forward_pass_are_noticed():
+    z = _logits(3, 64, torch.float32, "contiguous").requires_grad_()
+    y = z * 1.0
+    ids, t = _teacher(3, 64, 4, False, ragged=False)
+    for loss in (kf.token_logprobs(y).entropy.sum(), kf.topk_distillation(y, ids, t).sum()):
+        y.detach().zero_()
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward(retain_graph=True)
