@@ -50,8 +50,8 @@ struct SelectShared {
 //
 // Selection without a second pass over the row: the statistics' pass keeps
 // the maximum of each thread, and of each group of a thread's batches.
-// 1. With r = k / warps, rounded up, let t be the least of the warps' r-th
-//    largest thread maxima: at least k elements are >= t.
+// 1. With r = k / warps, rounded up, let t be the least of the (full) warps'
+//    r-th largest thread maxima: at least k elements are >= t.
 // 2. One warp bisects t among those groups' maxima until not many more than k
 //    are left. All k largest elements are >= t still, and lie in these groups.
 // 3. Those groups are read again (from L2), first for the units with an
@@ -68,15 +68,16 @@ __device__ void select_top(const Row<T>& row, int u0, int u1, int ragged, float 
   const int want = min(k, n_units * E + ragged);
   const bool has = tid < n_units || tid < ragged;
   const uint32_t key = has ? order_of(mine) : 0u;
+  const int warps = min(NW, n_units / 32);  // all of whose lanes have elements
+  const int r = warps > 0 ? (want + warps - 1) / warps : 33;
   {
     // The warp's r-th largest: take the maximum out until r are gone.
-    const int r = (want + NW - 1) / NW;
     uint32_t rest = key, top = 0;
     int gone = 0;
-    while (gone < r) {
+    while (gone < min(r, 32)) {
       top = __reduce_max_sync(0xffffffffu, rest);
       if (lane == 0 && gone == 0) sh.warp_top[warp] = top;
-      gone = top == 0 ? r : gone + __popc(__ballot_sync(0xffffffffu, rest == top));
+      gone = top == 0 ? 32 : gone + __popc(__ballot_sync(0xffffffffu, rest == top));
       rest = rest == top ? 0u : rest;
     }
     if (lane == 0) sh.warp_key[warp] = top;
@@ -87,8 +88,9 @@ __device__ void select_top(const Row<T>& row, int u0, int u1, int ragged, float 
     sh.hits = 0;
   }
   __syncthreads();
-  // 0: some warp has fewer elements, all stay
-  uint32_t t = max(__reduce_min_sync(0xffffffffu, sh.warp_key[lane & (NW - 1)]), 1u);
+  // Where the warps have too few lanes all elements stay: no key is 0.
+  uint32_t t = __reduce_min_sync(0xffffffffu, lane < warps ? sh.warp_key[lane] : 0xFFFFFFFFu);
+  t = r > 32 ? 1u : t;
   const uint32_t top = __reduce_max_sync(0xffffffffu, sh.warp_top[lane & (NW - 1)]);
   const int batches = (n_units + kBatch * NT - 1) / (kBatch * NT);
   if (key >= t) {
@@ -99,7 +101,8 @@ __device__ void select_top(const Row<T>& row, int u0, int u1, int ragged, float 
   __syncthreads();
   const int listed = sh.listed;
   constexpr int kOwn = 16;  // maxima per lane in step 2
-  if (listed > want + want / 8 + 2 && listed <= 32 * kOwn) {
+  // Few more than enough are looked at all the same.
+  if (listed > max(64, want + want / 8 + 2) && listed <= 32 * kOwn) {
     if (warp == 0) {
       uint32_t own[kOwn];
 #pragma unroll
@@ -310,7 +313,7 @@ __global__ void __launch_bounds__(NT)
   }
   __shared__ Acc join_sm[NT / 32], result;
   __shared__ std::conditional_t<TOPK, SelectShared<NT>, int> sh;
-  stream_units<T, NT, true>(FromMemory{row.unit_ptr()}, u0, u1, c, run, NoMarks{}, [&](int batch, float mx) {
+  stream_units<T, NT, TOPK>(FromMemory{row.unit_ptr()}, u0, u1, c, run, NoMarks{}, [&](int batch, float mx) {
     if constexpr (TOPK) {
       mine = max_nan(mine, mx);
       float& kept = sh.group_max[batch % sh.kGroups][tid];
@@ -364,19 +367,24 @@ __global__ void __launch_bounds__(NT)
     };
     if constexpr (SPLIT) {
       __syncthreads();
-      // A key's place is its place in its own list and the number of larger keys in the others.
+      // A key's place is the number of larger keys: counted, or from its place in its own list and searches in the others.
       for (int i = tid; i < parts * k; i += NT) {
         const unsigned long long key = sh.cand[i];
-        int place = i % k;
-        for (int other = 0; other < parts; ++other) {
-          if (other == i / k) continue;
-          int lo = 0, hi = k;  // keys before lo are larger, from hi on smaller
-          while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (sh.cand[other * k + mid] > key) lo = mid + 1;
-            else hi = mid;
+        int place = 0;
+        if (parts * k <= 128) {
+          for (int j = 0; j < parts * k; ++j) place += sh.cand[j] > key;
+        } else {
+          place = i % k;
+          for (int other = 0; other < parts; ++other) {
+            if (other == i / k) continue;
+            int lo = 0, hi = k;  // keys before lo are larger, from hi on smaller
+            while (lo < hi) {
+              const int mid = (lo + hi) / 2;
+              if (sh.cand[other * k + mid] > key) lo = mid + 1;
+              else hi = mid;
+            }
+            place += lo;
           }
-          place += lo;
         }
         if (key != 0 && place < k) emit(place, key);
       }
@@ -498,7 +506,9 @@ void token_logprobs_backward(const at::Tensor& logits, const OptTensor& tokens, 
   for_logits_type(logits.scalar_type(), [&](auto tag) {
     using T = typename decltype(tag)::type;
     const int nseg = row_segments(rows, vocab, sizeof(T), 256, logits.get_device());
-    logprob_backward_kernel<T, 256><<<dim3((unsigned)rows, nseg), 256, 0, s>>>(
+    const bool small = vocab * (int64_t)sizeof(T) <= kSmallRow;
+    const auto kern = small ? logprob_backward_kernel<T, 64> : logprob_backward_kernel<T, 256>;
+    kern<<<dim3((unsigned)rows, nseg), small ? 64 : 256, 0, s>>>(
         (const T*)logits.data_ptr(), logits.stride(0), (T*)out.data_ptr(), out.stride(0), (int)vocab,
         tokens ? tokens->data_ptr<int64_t>() : nullptr, ignore_index, c, (float)(1.0 / temperature),
         stats.data_ptr<float>(), entropy.data_ptr<float>(), dlp, dh);

@@ -217,18 +217,23 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Running statistics of a warp's elements. The maximum is the warp's, so it
-// rarely grows and the lanes' sums need no rescaling when they are joined;
-// each lane holds its sums as two halves.
+// Running statistics of a warp's elements: sums of 2^x with x = z c - r, for a
+// reference r that all lanes share, so that they need no rescaling when they are
+// joined; each lane holds its sums as two halves. With m the largest element when
+// the reference was last taken, r is m c rounded, which makes x one exact
+// product and one rounding; total() makes up for the rounding of r. Where
+// m c would overflow (or m is infinite or NaN), x = (z - m) c instead.
 template <bool ENT>
 struct Run {
-  float m = -INFINITY, ms = 0.f;  // maximum, and the finite value to subtract
+  float m = -INFINITY, r = 0.f;
+  bool plain = false;  // x = z c - r
   F2 s{}, a{};
-  // Takes the maximum up to the lanes' `wide`; called by whole warps.
+  // Takes the reference up to the largest of the lanes' `wide`; called by whole warps.
   __device__ __forceinline__ void raise(float wide, float c) {
     if (!__any_sync(0xffffffffu, !(wide <= m))) return;
-    const float mn = max_nan(m, warp_max_nan(wide));
-    const float x = (m - mn) * c;
+    const float mn = max_nan(m, warp_max_nan(wide)), rn = mn * c;
+    const bool pn = fabsf(rn) < 1e37f;
+    const float x = plain && pn ? r - rn : (m - mn) * c;
     const float f = (m == mn) ? 1.f : ex2(x);
     const F2 ff = pair(f, f);
     if (ENT) {
@@ -237,35 +242,43 @@ struct Run {
     }
     s = mul2(s, ff);
     m = mn;
-    ms = mn == -INFINITY ? 0.f : mn;
+    r = rn;
+    plain = pn;
   }
-  __device__ __forceinline__ void add(F2 z, F2 minus_ms, F2 c) {
-    const F2 x = mul2(add2(z, minus_ms), c);
+  // Two elements where `plain`.
+  __device__ __forceinline__ void add(F2 z, F2 c, F2 minus_r) {
+    const F2 x = fma2(z, c, minus_r);
     const float2 xs = split(x);
     const F2 e = pair(ex2(xs.x), ex2(xs.y));
     s = add2(s, e);
     if (ENT) a = fma2(e, x, a);
   }
-  // The same for A alone, with 2^-inf (-inf) = 0.
-  __device__ __forceinline__ void add_masked(F2 z, F2 minus_ms, F2 c) {
-    const float2 xs = split(mul2(add2(z, minus_ms), c));
-    a = fma2(pair(ex2(xs.x), ex2(xs.y)), pair(fmaxf(xs.x, -256.f), fmaxf(xs.y, -256.f)), a);
+  // An element's x in any case; -inf for a masked one.
+  __device__ __forceinline__ float exponent(float z, float c) const {
+    return plain ? fmaf(z, c, -r) : (z - (m == -INFINITY ? 0.f : m)) * c;
+  }
+  // An element in any case; with ONLY_A its part of A alone. 2^-inf (-inf) is 0.
+  template <bool ONLY_A>
+  __device__ __forceinline__ void add_any(float z, float c) {
+    const float x = exponent(z, c), e = ex2(x);
+    if (!ONLY_A) s = add2(s, pair(e, 0.f));
+    if (ENT) a = fma2(pair(e, 0.f), pair(fmaxf(x, -256.f), 0.f), a);
   }
   // One element per lane (-inf for none); called by whole warps.
   __device__ __forceinline__ void add_one(float z, float c) {
     raise(z, c);
-    const float x = (z - ms) * c, e = ex2(x);
-    s = add2(s, pair(e, 0.f));
-    if (ENT) a = fma2(pair(e, 0.f), pair(fmaxf(x, -256.f), 0.f), a);
+    add_any<false>(z, c);
   }
-  // The warp's statistics, in every lane.
-  __device__ __forceinline__ Acc total() const {
-    Acc r;
-    r.m = m;
+  // The warp's statistics to its reference's m, in every lane.
+  __device__ __forceinline__ Acc total(float c) const {
+    Acc t;
     const float2 ss = split(s), aa = split(a);
-    r.s = warp_sum(ss.x + ss.y);
-    r.a = ENT ? warp_sum(aa.x + aa.y) : 0.f;
-    return r;
+    const float off = plain ? fmaf(m, c, -r) : 0.f;  // of every x
+    const float f = ex2(-off);
+    t.m = m;
+    t.s = warp_sum(ss.x + ss.y) * f;
+    t.a = ENT ? warp_sum(aa.x + aa.y) * f - off * t.s : 0.f;
+    return t;
   }
 };
 
@@ -347,11 +360,15 @@ struct FromMemory {
 
 // Statistics of the units [u0, u1) of a row over the threads of a block, in
 // batches of four 16-byte loads per thread (unit u0 + tid + (4 b + i) NT is the
-// i-th of batch b); batch_max(b, m) gets each batch's maximum. Per element: widening, half a packed
-// maximum, and in pairs a subtraction, a product, two 2^x and one or two sums.
-// Clamping the masked entries' exponents would cost one more instruction per
+// i-th of batch b). With MAX, batch_max(b, m) gets each batch's maximum, and the
+// reference follows it. Without, the first batch gives the reference, and a
+// later one is taken again with a new one only if its sum has grown past
+// 2^20 (the maximum is at most 20 off then, which costs the entropy 20 2^-23):
+// half an instruction per element less. Per element that leaves the widening,
+// and in pairs a multiply-add, two 2^x and one or two sums.
+// Clamping masked entries' exponents would cost one more instruction per
 // element; instead a batch whose A came out NaN (0 times -inf) takes its A again.
-template <typename T, int NT, bool ENT, typename Src, typename M, typename G>
+template <typename T, int NT, bool MAX, bool ENT, typename Src, typename M, typename G>
 __device__ __forceinline__ void stream_units(const Src& src, int u0, int u1, float c, Run<ENT>& run, const M& marks,
                                              const G& batch_max) {
   constexpr bool MASK = !std::is_same_v<M, NoMarks>;
@@ -374,44 +391,74 @@ __device__ __forceinline__ void stream_units(const Src& src, int u0, int u1, flo
         if (u + i * NT < u1) q[i] = src.load(u + i * NT);
       }
     }
+    uint32_t set = 0;
     if constexpr (MASK) {
-      const uint32_t set = marks.of_batch(batch);
+      set = marks.of_batch(batch);
       if (set) {
 #pragma unroll
         for (int i = 0; i < UN; ++i)
           if ((set >> (E * i)) & ((1u << E) - 1u)) mask_unit<T>(q[i], set >> (E * i));
       }
     }
-    uint32_t mx = Elem<T>::max2(Elem<T>::max2(q[0].x, q[0].y), Elem<T>::max2(q[0].z, q[0].w));
+    if (MAX || run.m == -INFINITY) {
+      uint32_t mx = Elem<T>::max2(Elem<T>::max2(q[0].x, q[0].y), Elem<T>::max2(q[0].z, q[0].w));
 #pragma unroll
-    for (int i = 1; i < UN; ++i)
-      mx = Elem<T>::max2(mx, Elem<T>::max2(Elem<T>::max2(q[i].x, q[i].y), Elem<T>::max2(q[i].z, q[i].w)));
-    const float wide = Elem<T>::widen_max(mx);
-    batch_max(batch, wide);
-    run.raise(wide, c);
-    const F2 mm = pair(-run.ms, -run.ms);
-    const F2 a_before = run.a;
+      for (int i = 1; i < UN; ++i)
+        mx = Elem<T>::max2(mx, Elem<T>::max2(Elem<T>::max2(q[i].x, q[i].y), Elem<T>::max2(q[i].z, q[i].w)));
+      const float wide = Elem<T>::widen_max(mx);
+      batch_max(batch, wide);
+      run.raise(wide, c);
+    }
+    const F2 s_before = run.s, a_before = run.a;
+    bool again = !run.plain;
+    if (run.plain) {
+      const F2 rr = pair(-run.r, -run.r);
 #pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      if (whole || base + i * NT < u1) {  // lanes behind the end hold -inf
-        float v[E];
-        Elem<T>::unpack(q[i], v);
+      for (int i = 0; i < UN; ++i) {
+        if (whole || base + i * NT < u1) {  // lanes behind the end hold -inf
+          float v[E];
+          Elem<T>::unpack(q[i], v);
 #pragma unroll
-        for (int j = 0; j < E; j += 2) run.add(pair(v[j], v[j + 1]), mm, cc);
+          for (int j = 0; j < E; j += 2) run.add(pair(v[j], v[j + 1]), cc, rr);
+        }
+      }
+      if (!MAX) {
+        const float2 ss = split(run.s);
+        again = __any_sync(0xffffffffu, !(ss.x + ss.y <= 1048576.f));
       }
     }
-    if (ENT) {
+    // The ways below are rare and read the batch again.
+    if (again) {
+      run.s = s_before;
+      run.a = a_before;
+      for (int pass = MAX ? 1 : 0; pass < 2; ++pass) {
+        float wide = -INFINITY;
+#pragma unroll 1
+        for (int i = 0; i < UN; ++i) {
+          if (u + i * NT >= u1) continue;
+          uint4 w = src.load(u + i * NT);
+          if (MASK) mask_unit<T>(w, set >> (E * i));
+          float v[E];
+          Elem<T>::unpack(w, v);
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            if (pass == 0) wide = max_nan(wide, v[j]);
+            else run.template add_any<false>(v[j], c);
+          }
+        }
+        if (pass == 0) run.raise(wide, c);
+      }
+    } else if (ENT) {
       const float2 aa = split(run.a);
       if (!(aa.x + aa.y == aa.x + aa.y)) {
         run.a = a_before;
 #pragma unroll 1
         for (int i = 0; i < UN; ++i) {
-          if (u + i * NT < u1) {
-            float v[E];
-            Elem<T>::unpack(src.load(u + i * NT), v);
+          if (u + i * NT >= u1) continue;
+          float v[E];
+          Elem<T>::unpack(src.load(u + i * NT), v);
 #pragma unroll
-            for (int j = 0; j < E; j += 2) run.add_masked(pair(v[j], v[j + 1]), mm, cc);
-          }
+          for (int j = 0; j < E; ++j) run.template add_any<true>(v[j], c);
         }
       }
     }
@@ -440,7 +487,7 @@ __device__ __forceinline__ Acc join_lanes(Acc v, float c) {
 // Joins the statistics of a block's warps; the first warp returns with them.
 template <int NT, bool ENT>
 __device__ __forceinline__ Acc block_join(const Run<ENT>& run, float c, Acc* sm) {
-  const Acc w = run.total();
+  const Acc w = run.total(c);
   if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = w;
   __syncthreads();
   Acc r;
@@ -576,20 +623,28 @@ void check_out(const at::Tensor& out, const at::Tensor& logits, int64_t vocab) {
   KB_CHECK(out.size(0) <= 1 || out.stride(0) >= vocab, "rows of out overlap");
 }
 
-// Threads per row of the statistics' passes. Small blocks leave less of the device idle at a row's end (V = 50257 bf16,
-// 16384 rows: 264 us with 128 threads, 282 with 256, 337 with 512) as long as there are rows enough to fill it; rows
-// above 128 KB take 256 (V = 131072 fp32, 4096 rows: 313 against 333 us). Few rows are shared by clusters of blocks
-// of at least 16 KB each.
+// Threads per row of the statistics' passes, and blocks where a cluster shares a row. Many rows: small blocks leave less
+// of the device idle at a row's end (V = 50257 bf16, 16384 rows: 264 us with 128 threads, 282 with 256, 337 with 512),
+// but rows above 128 KB take 256 (V = 131072 fp32, 4096 rows: 313 against 333 us). Few rows: larger blocks (257 rows of
+// 50257 bf16: 8.0 us with 512 threads, 8.4 with 256, 11.0 with 128; rows of 16 KB: 3.7 with 256, 3.9 with 512), and
+// clusters while each block keeps at least 16 KB and has an SM of its own, or at least 64 KB and a third of one (one row
+// of 50257 bf16: 5.1 us with four blocks, 5.8 with one; 40 rows of 131072 fp32: 6.8 with eight, 12.3 with one; but 257
+// rows of 50257 bf16: 9.7 with two, 8.0 with one).
 struct RowLaunch {
   int threads, parts;
 };
 RowLaunch row_launch(int64_t rows, int64_t row_bytes, int device) {
-  const int64_t fill = 1536 * (int64_t)num_sms(device);
-  RowLaunch how{row_bytes > 128 * 1024 ? 256 : 128, 1};
-  while (how.threads < 512 && rows * how.threads < fill && row_bytes >= 32 * how.threads) how.threads *= 2;
-  if (how.threads < 512 || rows * 512 >= fill || row_bytes < 32768) return how;
-  how.threads = 256;
-  while (how.parts < 8 && rows * how.parts * 256 < fill && row_bytes >= how.parts * 2 * 16384) how.parts *= 2;
+  const int64_t sms = num_sms(device);
+  RowLaunch how{128, 1};
+  while (how.parts < 8) {
+    const int64_t blocks = rows * how.parts * 2, part = row_bytes / (how.parts * 2);
+    if (!(part >= 16384 && blocks <= sms) && !(part >= 65536 && blocks <= 3 * sms)) break;
+    how.parts *= 2;
+  }
+  if (how.parts > 1) how.threads = 256;
+  else if (row_bytes <= 32768) how.threads = rows < 400 && row_bytes >= 8192 ? 256 : 128;
+  else if (rows <= 2 * sms) how.threads = 512;
+  else if (rows < 1000 || row_bytes > 131072) how.threads = 256;
   return how;
 }
 
@@ -642,6 +697,9 @@ void launch_rows(void (*kern)(P...), int64_t rows, int threads, int parts, size_
   cfg.numAttrs = parts > 1 ? 1 : 0;
   KB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...));
 }
+
+// Rows of a gradient up to here are written by 64 threads: more have nothing to do.
+constexpr int64_t kSmallRow = 8192;
 
 int row_segments(int64_t rows, int64_t vocab, int64_t elem, int threads, int device) {
   const int64_t units = vocab * elem / 16;

@@ -8,7 +8,8 @@
 namespace kb {
 namespace {
 
-constexpr int kChunks = 32;  // bulk copies a block stages its units with, at most
+constexpr int kGradThreads = 512;  // streaming threads of the kernel that writes loss and gradient
+constexpr int kChunks = 8;  // bulk copies a block stages its units with, at most
 constexpr int kStats = kTopkDistillationStats;  // KdStats, and 0 for a row without slots
 
 // --------------------------------------------------------- distillation
@@ -176,16 +177,20 @@ __device__ __forceinline__ void write_gradient(const Row<T>& row, T* out, int u0
 }
 
 // Loss of each row, times its weight: a block per row, or with SPLIT a cluster of blocks that share it. Off-list
-// elements are told by marks in shared memory (TAIL).
-template <typename T, int NT, bool TAIL, bool SPLIT>
+// elements are told by marks in shared memory (TAIL). With GRAD, for short rows, a second pass over the row (from L2)
+// writes the gradient.
+template <typename T, int NT, bool TAIL, bool SPLIT, bool GRAD>
 __global__ void __launch_bounds__(NT)
-    distill_forward_kernel(const T* __restrict__ logits, long long ld, int V, const int64_t* __restrict__ ids,
-                           const float* __restrict__ teacher, int K, float c, float inv_t,
-                           const float* __restrict__ weight, float* __restrict__ loss, float* __restrict__ stats) {
+    distill_forward_kernel(const T* logits, long long ld, T* out, long long ld_out, int V,
+                           const int64_t* __restrict__ ids, const float* __restrict__ teacher, int K, float c,
+                           float inv_t, const float* __restrict__ weight, float* __restrict__ loss,
+                           float* __restrict__ stats) {
+  static_assert(!(SPLIT && GRAD), "a cluster leaves the gradient to the backward kernel");
   namespace cg = cooperative_groups;
   extern __shared__ uint32_t words[];
   __shared__ ListShared sh;
   __shared__ Acc join_sm[NT / 32], result;
+  __shared__ KdStats row_result;
   const int tid = threadIdx.x;
   int part = 0, parts = 1;
   if constexpr (SPLIT) {
@@ -206,16 +211,16 @@ __global__ void __launch_bounds__(NT)
   if (!some) {
     if (part == 0 && tid == 0) loss[row_i] = 0.f;
     if (part == 0 && tid < kStats && stats) stats[row_i * kStats + tid] = 0.f;
+    if constexpr (GRAD) {
+      const Row<T> to(out + row_i * ld_out, V);
+      zero_row<T, NT>(to, 0, to.units, to.ragged);
+    }
     return;
   }
   Run<false> run;
   if (TAIL) {
     for (int i = tid; i < K; i += NT)
       if (sh.id[i] >= 0 && marks.mark(row, sh.id[i], part == 0)) sh.repeated = 1;
-    // A block of a cluster sees the marks of its part only.
-    for (int i = tid % kMaxList; SPLIT && i < K; i += kMaxList)
-      for (int j = tid / kMaxList; j < i; j += NT / kMaxList)
-        if (sh.id[i] >= 0 && sh.id[i] == sh.id[j]) sh.repeated = 1;
     __syncthreads();
   }
   if (tid < 32) {  // fewer than two units of ragged elements
@@ -223,14 +228,19 @@ __global__ void __launch_bounds__(NT)
     run.add_one(in ? Elem<T>::load(row.z + row.ragged_index(tid)) : -INFINITY, c);
   }
   const FromMemory src{row.unit_ptr()};
-  if constexpr (TAIL) stream_units<T, NT>(src, u0, u1, c, run, marks, [](int, float) {});
-  else stream_units<T, NT>(src, u0, u1, c, run, NoMarks{}, [](int, float) {});
+  if constexpr (TAIL) stream_units<T, NT, false>(src, u0, u1, c, run, marks, [](int, float) {});
+  else stream_units<T, NT, false>(src, u0, u1, c, run, NoMarks{}, [](int, float) {});
   Acc all = block_join<NT, false>(run, c, join_sm);
   if constexpr (SPLIT) {
-    if (tid == 0) result = all;
+    if (tid == 0) {
+      result = all;
+      result.a = (float)sh.repeated;  // a block sees the marks of its part only
+    }
     cg::this_cluster().sync();
     if (part == 0 && tid < 32) {
       all = *cg::this_cluster().map_shared_rank(&result, (tid & 7) < parts ? tid & 7 : 0);
+      if (__any_sync(0xffffffffu, all.a != 0.f)) sh.repeated = 1;
+      __syncwarp();
       all = join_lanes<8, false>((tid & 7) < parts ? all : Acc(), c);
     }
     cg::this_cluster().sync();  // the parts' statistics are read
@@ -238,11 +248,17 @@ __global__ void __launch_bounds__(NT)
   if (part == 0 && tid < 32) {
     const ListStats list = list_stats<TAIL>(c, K, sh);
     const KdStats r = row_stats<TAIL>(all, list, c);
+    if (GRAD && tid == 0) row_result = r;
     const float l = row_loss<TAIL>(all, list, r, c, inv_t, K, sh);
     if (tid == 0) {
       loss[row_i] = w * l;
       if (stats) store_stats(stats + row_i * kStats, r);
     }
+  }
+  if constexpr (GRAD) {
+    if (!TAIL && tid == 0) sh.repeated = 1;  // not known
+    __syncthreads();
+    write_gradient<T, NT, TAIL>(row, out + row_i * ld_out, 0, row.units, row.ragged, K, c, w * inv_t, row_result, sh);
   }
 }
 
@@ -338,9 +354,9 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
       const FromStage src{stage, sh.full, staged & 1u, &sh.abort_flag, status};
       const Marks<T, NT> marks(words, 0, row.units);
       if (tid < 32) run.add_one(TAIL && tid < row.ragged && marks.ragged(tid) ? -INFINITY : rag, c);
-      if constexpr (TAIL) stream_units<T, NT>(src, 0, row.units, c, run, marks, [](int, float) {});
-      else stream_units<T, NT>(src, 0, row.units, c, run, NoMarks{}, [](int, float) {});
-      const Acc mine = run.total();
+      if constexpr (TAIL) stream_units<T, NT, false>(src, 0, row.units, c, run, marks, [](int, float) {});
+      else stream_units<T, NT, false>(src, 0, row.units, c, run, NoMarks{}, [](int, float) {});
+      const Acc mine = run.total(c);
       if (lane == 0) {
         sums[tid >> 5] = mine;
         mbar_arrive(&sh.joined);
@@ -561,13 +577,14 @@ void topk_distillation_forward(const at::Tensor& logits, const at::Tensor& ids, 
   if (out) check_out(*out, logits, vocab);
   if (rows == 0) return;
   const int device = logits.get_device();
-  // Loss and gradient in one kernel where a row fits into half an SM's shared memory and the rows fill the device.
+  // Loss and gradient in one kernel: rows of up to 32 KB pass twice through L2, and others are staged where they fit into
+  // half an SM's shared memory and fill the device. The rest takes two kernels.
   const int64_t row_bytes = vocab * logits.element_size(), units = row_bytes / 16;
-  const int grad_threads = row_bytes <= 16384 ? 128 : 512, stage_units = (int)((units + 7) / 8 * 8);
-  const int64_t marks = 4 * (grad_threads == 128 ? Marks<__half, 128>::size(stage_units) : Marks<__half, 512>::size(stage_units));
-  const int64_t staged = 16 * (int64_t)stage_units + marks;
-  const bool together = out && staged <= 108 * 1024 && rows >= num_sms(device);
-  if (out && !together) {
+  const int stage_units = (int)((units + 7) / 8 * 8);
+  const int64_t staged = 16 * (int64_t)stage_units + 4 * Marks<__half, kGradThreads>::size(stage_units);
+  const bool twice = out && row_bytes <= 32 * 1024;
+  const bool together = out && !twice && staged <= 108 * 1024 && rows >= num_sms(device);
+  if (out && !twice && !together) {
     KB_CHECK(stats.has_value(), "the gradient needs stats");
     topk_distillation_forward(logits, ids, teacher, weight, loss, stats, c10::nullopt, vocab, temperature, tail);
     topk_distillation_backward(logits, ids, teacher, *stats, weight, c10::nullopt, *out, vocab, temperature, tail, false);
@@ -583,25 +600,31 @@ void topk_distillation_forward(const at::Tensor& logits, const at::Tensor& ids, 
     for_bool(tail, [&](auto tail_tag) {
       constexpr bool TAIL = decltype(tail_tag)::value;
       if (together) {
-        auto launch = [&](auto kern, int threads) {
-          const int per_sm = allow_smem(kern, (size_t)staged, threads + 64, device);
-          const int64_t blocks = std::min<int64_t>(rows, (int64_t)std::max(1, per_sm) * num_sms(device));
-          launch_rows(kern, blocks, threads + 64, 1, (size_t)staged, s, (const T*)logits.data_ptr(), logits.stride(0),
-                      (T*)out->data_ptr(), out->stride(0), (int)vocab, rows, ids.data_ptr<int64_t>(),
-                      teacher.data_ptr<float>(), k, c, inv_t, w, loss.data_ptr<float>(), kept, stage_units, device_status_ptr(device));
-        };
-        if (grad_threads == 128) launch(distill_grad_kernel<T, 128, TAIL>, 128);
-        else launch(distill_grad_kernel<T, 512, TAIL>, 512);
+        auto kern = distill_grad_kernel<T, kGradThreads, TAIL>;
+        const int per_sm = allow_smem(kern, (size_t)staged, kGradThreads + 64, device);
+        const int64_t blocks = std::min<int64_t>(rows, (int64_t)std::max(1, per_sm) * num_sms(device));
+        launch_rows(kern, blocks, kGradThreads + 64, 1, (size_t)staged, s, (const T*)logits.data_ptr(), logits.stride(0),
+                    (T*)out->data_ptr(), out->stride(0), (int)vocab, rows, ids.data_ptr<int64_t>(),
+                    teacher.data_ptr<float>(), k, c, inv_t, w, loss.data_ptr<float>(), kept, stage_units,
+                    device_status_ptr(device));
+        return;
+      }
+      if (twice) {
+        constexpr int NT = 128;
+        launch_rows(distill_forward_kernel<T, NT, TAIL, false, true>, rows, NT, 1,
+                    TAIL ? 4 * (size_t)Marks<T, NT>::size((int)units) : 0, s, (const T*)logits.data_ptr(),
+                    logits.stride(0), (T*)out->data_ptr(), out->stride(0), (int)vocab, ids.data_ptr<int64_t>(),
+                    teacher.data_ptr<float>(), k, c, inv_t, w, loss.data_ptr<float>(), kept);
         return;
       }
       const RowLaunch how = row_launch(rows, vocab * (int64_t)sizeof(T), device);
       for_row_launch(how, [&](auto nt_tag, auto split_tag) {
         constexpr int NT = decltype(nt_tag)::value;
-        auto kern = distill_forward_kernel<T, NT, TAIL, decltype(split_tag)::value>;
+        auto kern = distill_forward_kernel<T, NT, TAIL, decltype(split_tag)::value, false>;
         const int smem = TAIL ? 4 * Marks<T, NT>::size((int)((units + how.parts - 1) / how.parts)) : 0;
         if (smem > 32 * 1024) allow_smem(kern, (size_t)smem, 0, device);
-        launch_rows(kern, rows, NT, how.parts, (size_t)smem, s, (const T*)logits.data_ptr(), logits.stride(0),
-                    (int)vocab, ids.data_ptr<int64_t>(), teacher.data_ptr<float>(), k, c, inv_t, w,
+        launch_rows(kern, rows, NT, how.parts, (size_t)smem, s, (const T*)logits.data_ptr(), logits.stride(0), nullptr,
+                    0, (int)vocab, ids.data_ptr<int64_t>(), teacher.data_ptr<float>(), k, c, inv_t, w,
                     loss.data_ptr<float>(), kept);
       });
     });
@@ -628,7 +651,10 @@ void topk_distillation_backward(const at::Tensor& logits, const at::Tensor& ids,
     // Blocks that most often return at once are few, and take several rows where they do not.
     const int64_t blocks = unless_one ? std::min<int64_t>(rows, 8 * (int64_t)num_sms(logits.get_device())) : rows;
     for_bool(tail, [&](auto tail_tag) {
-      distill_backward_kernel<T, 256, decltype(tail_tag)::value><<<dim3((unsigned)blocks, nseg), 256, 0, s>>>(
+      const bool small = vocab * (int64_t)sizeof(T) <= kSmallRow;
+      const auto kern = small ? distill_backward_kernel<T, 64, decltype(tail_tag)::value>
+                              : distill_backward_kernel<T, 256, decltype(tail_tag)::value>;
+      kern<<<dim3((unsigned)blocks, nseg), small ? 64 : 256, 0, s>>>(
           (const T*)logits.data_ptr(), logits.stride(0), (T*)out.data_ptr(), out.stride(0), (int)vocab, rows,
           ids.data_ptr<int64_t>(), teacher.data_ptr<float>(), k, c, (float)(1.0 / temperature),
           stats.data_ptr<float>(), row_grad,
