@@ -21,6 +21,13 @@ from .gemm import time_ms
 M, C, H, S, B, V = 16384, 768, 12, 1024, 16, 50304
 
 
+def _teacher(rows: int, vocab: int, k: int):
+    """Slots of a teacher: distinct tokens and log probabilities that leave some mass to the rest."""
+
+    ids = (torch.randint(0, vocab, (rows, 1), device="cuda") + 7919 * torch.arange(k, device="cuda")) % vocab
+    return ids, torch.log_softmax(torch.randn(rows, k + 1, device="cuda"), -1)[:, :k].contiguous()
+
+
 def cases() -> Dict[str, Tuple[Callable[[], object], float, str]]:
     from koochak_b200.ops import functional as kf
 
@@ -54,6 +61,16 @@ def cases() -> Dict[str, Tuple[Callable[[], object], float, str]]:
     gscale = torch.ones(1, device=dev)
     lg2 = logits.clone()
     out["ce_bwd"] = (lambda: kf.cross_entropy_backward_(lg2, tgt, lse, gscale, 50257), M * V * 4, "bytes")
+    full = logits[:, :50257]
+    out["token_logprobs"] = (lambda: kf.token_logprobs_forward(full, tgt), M * V * 2, "bytes")
+    out["token_logprobs_top20"] = (lambda: kf.token_logprobs_forward(full, tgt, top_k=20), M * V * 2, "bytes")
+    _, ent, stats, ids, tlp = (*kf.token_logprobs_forward(full, tgt)[:3], *_teacher(M, 50257, 64))
+    grow = torch.rand(M, device=dev)
+    out["token_logprobs_bwd"] = (lambda: kf.token_logprobs_backward(full, tgt, stats, ent, grow, grow, out=lg2[:, :50257]),
+                                 M * V * 4, "bytes")
+    out["topk_distillation"] = (lambda: kf.topk_distillation_forward(full, ids, tlp, tail=True), M * V * 2, "bytes")
+    out["topk_distillation_grad"] = (lambda: kf.topk_distillation_grad(full, ids, tlp, weight=grow, tail=True,
+                                                                       out=lg2[:, :50257]), M * V * 4, "bytes")
     qkv = torch.randn(B, S, 3, H, 64, device=dev).bfloat16()
     q, k, v = qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2]
     o, lse_a = kf.flash_attention_forward(q, k, v, causal=True)

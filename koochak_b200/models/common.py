@@ -158,3 +158,67 @@ def accumulation_target(*params: torch.Tensor) -> Optional[torch.Tensor]:
             return None
         rows += g.shape[0]
     return first.as_strided((rows, cols), (cols, 1))
+
+
+class HeadLogits(torch.autograd.Function):
+    """Final norm and LM head: ``[B, S, vocab]`` logits in the compute dtype (rows padded to 64 columns)."""
+
+    @staticmethod
+    def forward(ctx, x, norm_w, norm_b, head_w, head_w16, eps, rms):
+        B, S, C = x.shape
+        M, V = B * S, head_w.shape[0]
+        cdt = head_w16.dtype
+        x2 = x.reshape(M, C)
+        h, mean, rstd = kf.norm_forward(x2, norm_w, norm_b, eps, rms=rms, out_dtype=cdt)
+        vpad = (V + 63) // 64 * 64
+        logits = torch.empty((M, vpad), device=x.device, dtype=cdt)
+        kf.gemm(h, head_w16, out=logits[:, :V])
+        ctx.save_for_backward(x2, h, mean, rstd, norm_w, head_w16)
+        ctx.meta = (B, S, C, V, rms)
+        return logits.view(B, S, vpad)[..., :V]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlogits):
+        x2, h, mean, rstd, norm_w, head_w16 = ctx.saved_tensors
+        B, S, C, V, rms = ctx.meta
+        dlog = dlogits.to(h.dtype).reshape(B * S, V)
+        if dlog.stride(1) != 1 or dlog.stride(0) % 8 or dlog.data_ptr() % 16:  # the GEMM's operands: 16-byte aligned rows
+            padded = torch.empty((B * S, (V + 63) // 64 * 64), device=h.device, dtype=h.dtype)[:, :V]
+            dlog = padded.copy_(dlog)
+        dh = kf.gemm(dlog, head_w16, b_mn_major=True)
+        dw = kf.gemm(dlog, h, a_mn_major=True, b_mn_major=True, out_dtype=torch.float32)
+        dx, dnorm_w, dnorm_b, dx_lp = kf.norm_backward(dh, x2, norm_w, mean, rstd, rms=rms, dx_dtype=torch.float32,
+                                                       want_lp=True)
+        dx = dx.view(B, S, C)
+        dx._kb_lp = dx_lp  # the 16-bit copy the last layer's backward starts from
+        return dx, dnorm_w, dnorm_b, dw, None, None, None
+
+
+class TokenLosses:
+    """Per-token losses of a language model over its vocabulary; mixed into models that have ``logits(idx)``."""
+
+    def token_logprobs(self, idx: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, top_k: int = 0,
+                       temperature: float = 1.0, ignore_index: int = -100) -> kf.TokenLogprobs:
+        """``ops.functional.token_logprobs`` of the model's logits: scoring of given tokens, entropies, alternatives.
+
+        ``token_logprobs(idx, top_k=k)`` of a teacher gives the ``top_ids`` and ``top_logprobs`` that a student's
+        ``distillation_loss(..., tail=True)`` takes.
+        """
+
+        return kf.token_logprobs(self.logits(idx), tokens, top_k=top_k, temperature=temperature,
+                                 ignore_index=ignore_index)
+
+    def distillation_loss(self, idx: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
+                          weight: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                          tail: bool = False) -> torch.Tensor:
+        """Mean of ``ops.functional.topk_distillation`` over the positions that have teacher slots, or the mean
+        weighted by ``weight`` (``[B, S]``)."""
+
+        logits = self.logits(idx)
+        if weight is None:
+            weight = ((teacher_ids >= 0) & (teacher_ids < logits.shape[-1])).any(-1)
+        weight = weight.float()
+        weight = weight / weight.sum().clamp_min(torch.finfo(torch.float32).tiny)
+        return kf.topk_distillation(logits, teacher_ids, teacher_logits, temperature=temperature, tail=tail,
+                                    weight=weight, reduction="sum")

@@ -31,7 +31,7 @@ import torch.nn.functional as F
 
 from ..ops import functional as kf
 from ..utils.nn_utils import tag_param
-from .common import LowPrecisionShadows, compute_dtype, to_lp
+from .common import HeadLogits, LowPrecisionShadows, TokenLosses, compute_dtype, to_lp
 
 
 @dataclass
@@ -220,7 +220,7 @@ class _HeadLossFn(torch.autograd.Function):
         return _with_lp_copy(dx.view(B, S, C), dx_lp), dlnf_w, dlnf_b, dwte, None, None, None, None
 
 
-class GPT2(nn.Module):
+class GPT2(TokenLosses, nn.Module):
     """GPT-2 language model. ``forward(idx, targets)`` returns the mean loss;
     ``forward(idx)`` returns logits (reference path only materialises them)."""
 
@@ -265,20 +265,39 @@ class GPT2(nn.Module):
         if cdt is None or targets is None:
             return self._forward_reference(idx, targets, ignore_index)
         tr = self.transformer
-        eps = self.config.layer_norm_eps
         with torch.autocast("cuda", enabled=False):
             lp = self._shadows.get(cdt)
-            x = _EmbeddingFn.apply(idx, tr.wte.weight, tr.wpe.weight)
-            for blk in tr.h:
-                w16 = tuple(lp[id(w)] for w in blk.matrices())
-                x = _BlockFn.apply(
-                    x, blk.ln_1.weight, blk.ln_1.bias, blk.attn.c_attn.weight, blk.attn.c_attn.bias,
-                    blk.attn.c_proj.weight, blk.attn.c_proj.bias, blk.ln_2.weight, blk.ln_2.bias,
-                    blk.mlp.c_fc.weight, blk.mlp.c_fc.bias, blk.mlp.c_proj.weight, blk.mlp.c_proj.bias,
-                    w16, blk.attn.n_head, eps,
-                )
+            x = self._blocks(idx, lp)
             return _HeadLossFn.apply(x, tr.ln_f.weight, tr.ln_f.bias, tr.wte.weight, lp[id(tr.wte.weight)], targets,
-                                     eps, ignore_index)
+                                     self.config.layer_norm_eps, ignore_index)
+
+    def _blocks(self, idx, lp):
+        """The residual stream behind the last block (native path)."""
+
+        tr = self.transformer
+        eps = self.config.layer_norm_eps
+        x = _EmbeddingFn.apply(idx, tr.wte.weight, tr.wpe.weight)
+        for blk in tr.h:
+            w16 = tuple(lp[id(w)] for w in blk.matrices())
+            x = _BlockFn.apply(
+                x, blk.ln_1.weight, blk.ln_1.bias, blk.attn.c_attn.weight, blk.attn.c_attn.bias,
+                blk.attn.c_proj.weight, blk.attn.c_proj.bias, blk.ln_2.weight, blk.ln_2.bias,
+                blk.mlp.c_fc.weight, blk.mlp.c_fc.bias, blk.mlp.c_proj.weight, blk.mlp.c_proj.bias,
+                w16, blk.attn.n_head, eps,
+            )
+        return x
+
+    def logits(self, idx: torch.Tensor) -> torch.Tensor:
+        """Differentiable ``[B, S, vocab]`` logits (16-bit under autocast on CUDA)."""
+
+        cdt = compute_dtype(idx.device)
+        if cdt is None:
+            return self._forward_reference(idx, None, 0)
+        tr = self.transformer
+        with torch.autocast("cuda", enabled=False):
+            lp = self._shadows.get(cdt)
+            return HeadLogits.apply(self._blocks(idx, lp), tr.ln_f.weight, tr.ln_f.bias, tr.wte.weight,
+                                    lp[id(tr.wte.weight)], self.config.layer_norm_eps, False)
 
     def _forward_reference(self, idx, targets, ignore_index):
         B, S = idx.shape

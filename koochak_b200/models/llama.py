@@ -37,7 +37,7 @@ import torch.nn.functional as F
 from ..ops import functional as kf
 from ..ops._ext import native
 from ..utils.nn_utils import tag_param
-from .common import LowPrecisionShadows, accumulation_target, compute_dtype, to_lp
+from .common import HeadLogits, LowPrecisionShadows, TokenLosses, accumulation_target, compute_dtype, to_lp
 from .gpt2 import _lp_copy_of, _with_lp_copy
 
 __all__ = ["LlamaConfig", "Llama", "rope_tables"]
@@ -265,7 +265,7 @@ class _Model(nn.Module):
         self.norm = RMSNorm(cfg.dim, cfg.norm_eps)
 
 
-class Llama(nn.Module):
+class Llama(TokenLosses, nn.Module):
     """``forward(idx, targets)`` returns the mean loss; ``forward(idx)`` returns logits (reference path)."""
 
     def __init__(self, cfg: Optional[LlamaConfig] = None, **overrides) -> None:
@@ -312,22 +312,40 @@ class Llama(nn.Module):
         cos, sin = self.rope(S, idx.device)
         if cdt is None or targets is None:
             return self._forward_reference(idx, targets, ignore_index, cos, sin)
-        cfg = self.config
         with torch.autocast("cuda", enabled=False):
             lp = self._shadows.get(cdt)
-            x = _EmbedFn.apply(idx, self.model.embed_tokens.weight)
-            gi = 0
-            for layer in self.model.layers:
-                a, m = layer.self_attn, layer.mlp
-                w16 = (self._shadows.fused(gi, cdt), lp[id(a.o_proj.weight)], self._shadows.fused(gi + 1, cdt),
-                       lp[id(m.down_proj.weight)])
-                gi += 2
-                x = _LayerFn.apply(x, layer.input_layernorm.weight, layer.post_attention_layernorm.weight,
-                                   a.q_proj.weight, a.k_proj.weight, a.v_proj.weight, a.o_proj.weight,
-                                   m.gate_proj.weight, m.up_proj.weight, m.down_proj.weight, w16, cos, sin,
-                                   cfg.n_head, cfg.norm_eps)
+            x = self._layers(idx, lp, cdt, cos, sin)
             return _HeadFn.apply(x, self.model.norm.weight, self.lm_head.weight, lp[id(self.lm_head.weight)],
-                                 targets, cfg.norm_eps, ignore_index)
+                                 targets, self.config.norm_eps, ignore_index)
+
+    def _layers(self, idx, lp, cdt, cos, sin):
+        """The residual stream behind the last layer (native path)."""
+
+        cfg = self.config
+        x = _EmbedFn.apply(idx, self.model.embed_tokens.weight)
+        gi = 0
+        for layer in self.model.layers:
+            a, m = layer.self_attn, layer.mlp
+            w16 = (self._shadows.fused(gi, cdt), lp[id(a.o_proj.weight)], self._shadows.fused(gi + 1, cdt),
+                   lp[id(m.down_proj.weight)])
+            gi += 2
+            x = _LayerFn.apply(x, layer.input_layernorm.weight, layer.post_attention_layernorm.weight,
+                               a.q_proj.weight, a.k_proj.weight, a.v_proj.weight, a.o_proj.weight,
+                               m.gate_proj.weight, m.up_proj.weight, m.down_proj.weight, w16, cos, sin,
+                               cfg.n_head, cfg.norm_eps)
+        return x
+
+    def logits(self, idx: torch.Tensor) -> torch.Tensor:
+        """Differentiable ``[B, S, vocab]`` logits (16-bit under autocast on CUDA)."""
+
+        cdt = compute_dtype(idx.device)
+        cos, sin = self.rope(idx.shape[1], idx.device)
+        if cdt is None:
+            return self._forward_reference(idx, None, 0, cos, sin)
+        with torch.autocast("cuda", enabled=False):
+            lp = self._shadows.get(cdt)
+            return HeadLogits.apply(self._layers(idx, lp, cdt, cos, sin), self.model.norm.weight, None,
+                                    self.lm_head.weight, lp[id(self.lm_head.weight)], self.config.norm_eps, True)
 
     def _forward_reference(self, idx, targets, ignore_index, cos, sin):
         x = self.model.embed_tokens(idx)

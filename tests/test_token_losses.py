@@ -727,3 +727,73 @@ def test_logits_changed_after_the_forward_pass_are_noticed():
         y.detach().zero_()
         with pytest.raises(RuntimeError, match="inplace"):
             loss.backward(retain_graph=True)
+
+
+# ------------------------------------------------------------------ models
+
+
+def _small_models(device):
+    from koochak_b200.models import GPT2, Llama
+
+    torch.manual_seed(11)
+    return [(GPT2(n_layer=2, n_head=4, n_embd=256, vocab_size=1003, block_size=128).to(device),
+             GPT2(n_layer=1, n_head=4, n_embd=256, vocab_size=1003, block_size=128).to(device)),
+            (Llama(n_layer=2, n_head=4, dim=256, ffn_dim=384, vocab_size=1000, max_seq_len=128).to(device),
+             Llama(n_layer=1, n_head=4, dim=256, ffn_dim=384, vocab_size=1000, max_seq_len=128).to(device))]
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_models_teacher_and_student_on_cpu(which):
+    teacher, student = _small_models("cpu")[which]
+    idx = torch.randint(0, 1000, (2, 16))
+    targets = torch.randint(0, 1000, (2, 16))
+    targets[0, :4] = IGNORE
+    with torch.no_grad():
+        got = teacher.token_logprobs(idx, targets, top_k=10)
+        p = torch.log_softmax(teacher(idx), -1)
+    keep = targets != IGNORE
+    # fp32 against fp32 of the same formula in another order
+    assert torch.allclose(got.logprobs[keep], p.gather(-1, targets.clamp_min(0)[..., None])[..., 0][keep], atol=1e-5)
+    assert torch.allclose(got.entropy[keep], -(p.exp() * p).sum(-1)[keep], atol=1e-5)
+    assert (got.top_ids[~keep] == -1).all() and not got.logprobs[~keep].any()
+    loss = student.distillation_loss(idx, got.top_ids, got.top_logprobs, tail=True)
+    loss.backward()
+    z = student(idx).detach()
+    rows = kf.topk_distillation_ref(z.reshape(-1, z.shape[-1]).double(), got.top_ids.reshape(-1, 10),
+                                    got.top_logprobs.reshape(-1, 10), tail=True)
+    assert torch.allclose(loss.detach().double(), rows.sum() / keep.sum(), atol=1e-5)
+    assert all(q.grad is not None and q.grad.isfinite().all() for q in student.parameters())
+
+
+@gpu
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_models_teacher_and_student_native(which, dtype):
+    """The run as a user makes it: the teacher's alternatives feed the student's loss, on the native kernels, against
+    the fp32 reference path; 16-bit activations are compared as the other model tests do."""
+
+    teacher, student = _small_models(DEV)[which]
+    idx = torch.randint(0, 1000, (2, 128), device=DEV)
+    targets = torch.randint(0, 1000, (2, 128), device=DEV)
+    targets[1, 100:] = IGNORE
+    with torch.no_grad(), torch.autocast("cuda", dtype=dtype):
+        got = teacher.token_logprobs(idx, targets, top_k=16)
+    with torch.no_grad():
+        ref = teacher.token_logprobs(idx, targets, top_k=16)
+    assert (got.logprobs - ref.logprobs).abs().max() < 2e-2 and (got.entropy - ref.entropy).abs().max() < 2e-2
+
+    def grads(native):
+        student.zero_grad(set_to_none=True)
+        with torch.autocast("cuda", dtype=dtype, enabled=native):
+            loss = student.distillation_loss(idx, ref.top_ids, ref.top_logprobs, tail=True)
+            lp = student.token_logprobs(idx, targets)
+            total = loss - 0.1 * lp.logprobs.mean() - 0.01 * lp.entropy.mean()
+        total.backward()
+        return loss.item(), {n: q.grad.detach().clone() for n, q in student.named_parameters()}
+
+    loss_n, g_n = grads(True)
+    loss_r, g_r = grads(False)
+    assert abs(loss_n - loss_r) < 2e-2
+    for n in g_r:
+        err = ((g_n[n] - g_r[n]).abs().max() / (g_r[n].abs().max() + 1e-6)).item()
+        assert err < 0.08, (n, err)
