@@ -7,7 +7,7 @@
 namespace kb {
 namespace {
 
-constexpr int kCand = 1024;  // candidates held while the alternatives are selected
+constexpr int kCand = 512;   // candidates held while the alternatives are selected
 constexpr int kStats = kTokenLogprobsStats;  // m, log2 S
 
 // ----------------------------------------------------------- alternatives
@@ -26,20 +26,24 @@ __device__ __forceinline__ unsigned long long key_of(uint32_t order, int index) 
   return ((unsigned long long)order << 32) | (uint32_t)~index;
 }
 
-constexpr int kHits = 512;  // units looked at element by element
+constexpr int kHits = 256;  // units looked at element by element
 
 template <int NT>
 struct SelectShared {
-  static constexpr int kGroups = NT <= 256 ? 16 : 8;  // maxima kept per thread: batch b counts to group b % kGroups
+  static constexpr int kGroups = NT == 256 ? 16 : 8;  // maxima kept per thread: batch b counts to group b % kGroups
   union alignas(16) {
     float group_max[kGroups][NT];
     unsigned long long cand[kCand];
+    unsigned long long merged[8 * kMaxTopK];  // the sorted lists of a cluster's blocks
   };
   union {
     uint16_t list[kGroups * NT];
-    int sums[kCand];  // ranks, or counts per warp
+    int sums[NT / 32];  // counts per warp
   };
-  uint4 hit[kHits];
+  union {
+    uint4 hit[kHits];
+    uint32_t list_key[4 * kHits];  // maxima of the first listed groups
+  };
   int hit_unit[kHits];
   uint32_t warp_key[NT / 32], warp_top[NT / 32];
   int count, listed, hits;
@@ -59,8 +63,8 @@ struct SelectShared {
 // Ties and rows sorted in memory can make the candidates overflow; then the
 // k-th value is bisected over the row itself and ties are taken in index order.
 template <typename T, int NT, typename Emit>
-__device__ void select_top(const Row<T>& row, int u0, int u1, int ragged, float mine, int k, SelectShared<NT>& sh,
-                           const Emit& emit) {
+__device__ void select_top(const Row<T>& row, int u0, int u1, int ragged, float mine, int k, int few,
+                           SelectShared<NT>& sh, const Emit& emit) {
   constexpr int E = Elem<T>::kUnit, NW = NT / 32, kGroups = SelectShared<NT>::kGroups;
   static_assert(NW <= 32 && NT * kGroups <= 65536, "list entries are 16 bits wide");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -93,31 +97,28 @@ __device__ void select_top(const Row<T>& row, int u0, int u1, int ragged, float 
   t = r > 32 ? 1u : t;
   const uint32_t top = __reduce_max_sync(0xffffffffu, sh.warp_top[lane & (NW - 1)]);
   const int batches = (n_units + kBatch * NT - 1) / (kBatch * NT);
+  // Candidates are told by their values first: !(v < bound) holds for all of order >= t, and for NaN.
+  float bound = value_of(t);
   if (key >= t) {
-    for (int g = 0; g < min(batches, kGroups); ++g)
-      if (tid + g * kBatch * NT < n_units && order_of(sh.group_max[g][tid]) >= t)
-        sh.list[atomicAdd(&sh.listed, 1)] = (uint16_t)(g * NT + tid);
+    for (int g = 0; g < min(batches, kGroups); ++g) {
+      const float m = sh.group_max[g][tid];
+      if (tid + g * kBatch * NT >= n_units || m < bound) continue;
+      const int at = atomicAdd(&sh.listed, 1);
+      sh.list[at] = (uint16_t)(g * NT + tid);
+      if (at < 4 * kHits) sh.list_key[at] = order_of(m);
+    }
   }
   __syncthreads();
   const int listed = sh.listed;
-  constexpr int kOwn = 16;  // maxima per lane in step 2
-  // Few more than enough are looked at all the same.
-  if (listed > max(64, want + want / 8 + 2) && listed <= 32 * kOwn) {
+  // Where blocks are few and latency counts, some more than enough are looked at all the same.
+  if (listed > max(few, want + want / 8 + 2) && listed <= 4 * kHits) {
     if (warp == 0) {
-      uint32_t own[kOwn];
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) {
-        const int at = i * 32 + lane;
-        own[i] = 0;
-        if (at < listed) own[i] = order_of(sh.group_max[sh.list[at] / NT][sh.list[at] % NT]);
-      }
       uint32_t lo = t, hi = top;  // count(>= lo) >= want, count(> hi) < want
       while (lo < hi) {
         const uint32_t mid = lo + (hi - lo) / 2 + 1;
         int n = 0;
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i)
-          if (i * 32 < listed) n += __popc(__ballot_sync(0xffffffffu, own[i] >= mid));
+        for (int i = lane; i < listed; i += 32) n += sh.list_key[i] >= mid;
+        n = __reduce_add_sync(0xffffffffu, n);
         if (n >= want) {
           lo = mid;
           if (n <= want + want / 8 + 2) break;
@@ -129,22 +130,24 @@ __device__ void select_top(const Row<T>& row, int u0, int u1, int ragged, float 
     }
     __syncthreads();
     t = sh.warp_key[0];
+    bound = value_of(t);
   }
-  auto push = [&](uint32_t o, int idx) {
-    if (o >= t) {
-      const int at = atomicAdd(&sh.count, 1);
-      if (at < kCand) sh.cand[at] = key_of(o, idx);
-    }
+  auto push = [&](float v, int idx) {
+    if (v < bound) return;
+    const uint32_t o = order_of(v);
+    if (o < t) return;
+    const int at = atomicAdd(&sh.count, 1);
+    if (at < kCand) sh.cand[at] = key_of(o, idx);
   };
   const uint4* p = row.unit_ptr();
   for (int first = 0; first < batches; first += kGroups) {
     for (int i = tid; i < listed * kBatch; i += NT) {
       const int entry = sh.list[i / kBatch];
       const int u = u0 + entry % NT + ((entry / NT + first) * kBatch + i % kBatch) * NT;
-      if (u < u1 && order_of(sh.group_max[entry / NT][entry % NT]) >= t) {
+      if (u < u1 && !(sh.group_max[entry / NT][entry % NT] < bound)) {
         const uint4 q = load_unit(p + u);
         const float mx = Elem<T>::widen_max(Elem<T>::max2(Elem<T>::max2(q.x, q.y), Elem<T>::max2(q.z, q.w)));
-        if (order_of(mx) >= t) {
+        if (!(mx < bound)) {
           const int at = atomicAdd(&sh.hits, 1);
           if (at < kHits) {
             sh.hit[at] = q;
@@ -156,9 +159,9 @@ __device__ void select_top(const Row<T>& row, int u0, int u1, int ragged, float 
   }
   __syncthreads();
   const int hits = min(sh.hits, kHits);
-  if (tid < ragged) push(order_of(Elem<T>::load(row.z + row.ragged_index(tid))), row.ragged_index(tid));
+  if (tid < ragged) push(Elem<T>::load(row.z + row.ragged_index(tid)), row.ragged_index(tid));
   for (int i = tid; i < hits * E; i += NT)
-    push(order_of(Elem<T>::load(reinterpret_cast<const T*>(sh.hit) + i)), row.head + sh.hit_unit[i / E] * E + i % E);
+    push(Elem<T>::load(reinterpret_cast<const T*>(sh.hit) + i), row.head + sh.hit_unit[i / E] * E + i % E);
   __syncthreads();
   int n = sh.hits > kHits ? kCand + 1 : sh.count;
   __syncthreads();
@@ -273,7 +276,7 @@ __device__ void select_top(const Row<T>& row, int u0, int u1, int ragged, float 
 // in one pass, then the alternatives. The blocks of a cluster select their own
 // alternatives, and the first block merges the sorted lists.
 template <typename T, int NT, bool TOPK, bool SPLIT>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(NT, 1280 / NT)
     logprob_forward_kernel(const T* __restrict__ logits, long long ld, int V, const int64_t* __restrict__ tokens,
                            int64_t ignore_index, float c, float inv_t, int k, float* __restrict__ logprobs,
                            float* __restrict__ entropy, float* __restrict__ stats, float* __restrict__ top_logprobs,
@@ -326,7 +329,7 @@ __global__ void __launch_bounds__(NT)
     if (tid == 0) result = all;
     if constexpr (TOPK) {
       for (int i = tid; i < k; i += NT) sorted[i] = 0;  // below every key
-      select_top<T, NT>(row, u0, u1, ragged, mine, k, sh,
+      select_top<T, NT>(row, u0, u1, ragged, mine, k, 64, sh,
                         [&](int place, unsigned long long key) { sorted[place] = key; });
     }
     cg::this_cluster().sync();
@@ -337,7 +340,7 @@ __global__ void __launch_bounds__(NT)
         all = join_lanes<8, true>(all, c);
       }
       if constexpr (TOPK) {
-        for (int i = tid; i < parts * k; i += NT) sh.cand[i] = *cg::this_cluster().map_shared_rank(&sorted[i % k], i / k);
+        for (int i = tid; i < parts * k; i += NT) sh.merged[i] = *cg::this_cluster().map_shared_rank(&sorted[i % k], i / k);
       }
     }
     cg::this_cluster().sync();  // the other blocks' shared memory is not needed any more
@@ -369,10 +372,10 @@ __global__ void __launch_bounds__(NT)
       __syncthreads();
       // A key's place is the number of larger keys: counted, or from its place in its own list and searches in the others.
       for (int i = tid; i < parts * k; i += NT) {
-        const unsigned long long key = sh.cand[i];
+        const unsigned long long key = sh.merged[i];
         int place = 0;
         if (parts * k <= 128) {
-          for (int j = 0; j < parts * k; ++j) place += sh.cand[j] > key;
+          for (int j = 0; j < parts * k; ++j) place += sh.merged[j] > key;
         } else {
           place = i % k;
           for (int other = 0; other < parts; ++other) {
@@ -380,7 +383,7 @@ __global__ void __launch_bounds__(NT)
             int lo = 0, hi = k;  // keys before lo are larger, from hi on smaller
             while (lo < hi) {
               const int mid = (lo + hi) / 2;
-              if (sh.cand[other * k + mid] > key) lo = mid + 1;
+              if (sh.merged[other * k + mid] > key) lo = mid + 1;
               else hi = mid;
             }
             place += lo;
@@ -389,7 +392,7 @@ __global__ void __launch_bounds__(NT)
         if (key != 0 && place < k) emit(place, key);
       }
     } else {
-      select_top<T, NT>(row, u0, u1, ragged, mine, k, sh, emit);
+      select_top<T, NT>(row, u0, u1, ragged, mine, k, NT == 512 ? 64 : 0, sh, emit);
     }
   }
 }

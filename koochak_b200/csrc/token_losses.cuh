@@ -621,6 +621,21 @@ void check_out(const at::Tensor& out, const at::Tensor& logits, int64_t vocab) {
   KB_CHECK(out.dim() == 2 && out.size(0) == logits.size(0) && out.size(1) >= vocab, "out must be [rows, vocab]");
   KB_CHECK(out.size(1) == 1 || out.stride(1) == 1, "out must have unit inner stride");
   KB_CHECK(out.size(0) <= 1 || out.stride(0) >= vocab, "rows of out overlap");
+  // The logits themselves, or memory apart from theirs: a shifted view would be overwritten before it is read.
+  if (out.numel() == 0 || out.data_ptr() == logits.data_ptr()) {
+    KB_CHECK(out.numel() == 0 || out.size(0) <= 1 || out.stride(0) == logits.stride(0), "out overlaps the logits");
+    return;
+  }
+  const auto bytes_end = [vocab](const at::Tensor& t) {
+    return (const char*)t.data_ptr() + ((t.size(0) - 1) * t.stride(0) + vocab) * t.element_size();
+  };
+  const bool apart = bytes_end(out) <= (const char*)logits.data_ptr() || bytes_end(logits) <= (const char*)out.data_ptr();
+  // Two column ranges of one buffer interleave without meeting.
+  const int64_t row = out.stride(0) * out.element_size();
+  const int64_t gap = ((const char*)out.data_ptr() - (const char*)logits.data_ptr()) % std::max<int64_t>(row, 1);
+  const int64_t shift = gap < 0 ? gap + row : gap, width = vocab * out.element_size();
+  KB_CHECK(apart || (out.stride(0) == logits.stride(0) && shift >= width && row - shift >= width),
+           "out overlaps the logits");
 }
 
 // Threads per row of the statistics' passes, and blocks where a cluster shares a row. Many rows: small blocks leave less

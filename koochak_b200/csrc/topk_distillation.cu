@@ -20,8 +20,8 @@ struct ListShared {
   int repeated;
 };
 
-// Reads a row's slots: ids (-1 where empty), teacher values and the student's logits there. Returns whether any is
-// valid.
+// Reads a row's slots: ids (-1 where empty), teacher values and the student's logits there. Returns whether the
+// thread's are any valid.
 template <typename T, int NT>
 __device__ __forceinline__ bool read_slots(const T* z, int V, const int64_t* ids, const float* teacher, int K,
                                            ListShared& sh) {
@@ -34,7 +34,7 @@ __device__ __forceinline__ bool read_slots(const T* z, int V, const int64_t* ids
     sh.z[i] = ok ? Elem<T>::load(z + id) : 0.f;
     any |= ok;
   }
-  return __syncthreads_or(any);
+  return any;
 }
 
 // What a row's gradient needs besides its logits:
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(NT)
   if (tid == 0) sh.repeated = 0;
   if (TAIL)
     for (int i = tid; i < Marks<T, NT>::size(u1 - u0); i += NT) words[i] = 0;
-  const bool some = w != 0.f && read_slots<T, NT>(row.z, V, ids + row_i * K, teacher + row_i * K, K, sh);
+  const bool some = w != 0.f && __syncthreads_or(read_slots<T, NT>(row.z, V, ids + row_i * K, teacher + row_i * K, K, sh));
   if (!some) {
     if (part == 0 && tid == 0) loss[row_i] = 0.f;
     if (part == 0 && tid < kStats && stats) stats[row_i * kStats + tid] = 0.f;
@@ -552,6 +552,7 @@ __global__ void __launch_bounds__(NT)
     const KdStats r{s[0], s[1], s[2], s[3], s[4], s[5], s[6]};
     if (threadIdx.x == 0) sh.repeated = 1;  // not known here
     read_slots<T, NT>(row.z, V, ids + row_i * K, teacher + row_i * K, K, sh);
+    if (o == row.z) __syncthreads();  // the listed logits are read before the gradient takes their place
     write_gradient<T, NT, TAIL>(row, o, u0, u1, blockIdx.y == 0 ? row.ragged : 0, K, c, w * factor * inv_t, r, sh);
     __syncthreads();  // the list is read before the next row's replaces it
   }

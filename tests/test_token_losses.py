@@ -402,6 +402,20 @@ def test_in_place_gradients(dtype):
         assert (b[rows] == 7).all() and (b[:, vocab:] == 7).all()
 
 
+@gpu
+def test_outputs_that_overlap_are_refused():
+    buf = _logits(6, 64, torch.float32, "contiguous")
+    z = buf[:, :20]
+    tok = _tokens(6, 20, ignored=False)
+    stats, entropy = _lp_saved(z, tok)
+    g = torch.ones(6, device=DEV)
+    beside = kf.token_logprobs_backward(z, tok, stats, entropy, g, None, out=buf[:, 20:40])  # other columns are fine
+    assert torch.equal(beside, kf.token_logprobs_backward(z, tok, stats, entropy, g, None))
+    for out in (buf[:, 4:24], buf.flatten()[8:8 + 6 * 32].view(6, 32)[:, :20], buf[0, :20].expand(6, 20)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            kf.token_logprobs_backward(z, tok, stats, entropy, g, None, out=out)
+
+
 def _lp_saved(z, tok):
     _, entropy, stats, _, _ = kf.token_logprobs_forward(z, tok, ignore_index=IGNORE)
     return stats, entropy
