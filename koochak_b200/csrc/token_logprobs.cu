@@ -433,12 +433,12 @@ __global__ void __launch_bounds__(NT)
     return d;
   };
   if (b == 0.f) {
-    map_row<T, NT>(row, o, u0, u1, ragged, [&](F2 z, int j) {
+    map_row<T, NT, false>(row, o, u0, u1, ragged, [&](F2 z, int j) {
       const float2 y = split(fma2(add2(z, minus_m), cc, ml));
       return given(mul2(pair(ex2(y.x), ex2(y.y)), aa), j);
     });
   } else {
-    map_row<T, NT>(row, o, u0, u1, ragged, [&](F2 z, int j) {
+    map_row<T, NT, false>(row, o, u0, u1, ragged, [&](F2 z, int j) {
       float2 y = split(fma2(add2(z, minus_m), cc, ml));
       const F2 p = pair(ex2(y.x), ex2(y.y));
       return given(mul2(p, fma2(bb, pair(fmaxf(y.x, -256.f), fmaxf(y.y, -256.f)), aa)), j);  // 0 (-inf) is 0 here

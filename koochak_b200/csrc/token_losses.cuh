@@ -290,9 +290,14 @@ __device__ __forceinline__ uint4 load_unit(const uint4* p) {
   return q;
 }
 
+// KEEP leaves the line in L2 for writes that follow; without, it may go first.
+template <bool KEEP>
 __device__ __forceinline__ void store_unit(uint4* p, const uint4& q) {
-  asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w)
-               : "memory");
+  if (KEEP)
+    asm volatile("st.global.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w) : "memory");
+  else
+    asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w)
+                 : "memory");
 }
 
 // Masks the elements of a unit whose bit is set in `b`.
@@ -504,7 +509,7 @@ __device__ __forceinline__ void segment(int units, int i, int n, int& u0, int& u
 
 // Writes a thread's batch of units u, u + NT, ...: out = f(two elements, the index of the first). `loaded` is called
 // once the batch is in registers.
-template <typename T, int NT, typename Src, typename F, typename L>
+template <typename T, int NT, bool KEEP, typename Src, typename F, typename L>
 __device__ __forceinline__ void map_batch(const Row<T>& row, const Src& src, T* out, bool same, int u, int u1,
                                           const F& f, const L& loaded) {
   constexpr int E = Elem<T>::kUnit;
@@ -526,7 +531,7 @@ __device__ __forceinline__ void map_batch(const Row<T>& row, const Src& src, T* 
         v[j + 1] = d.y;
       }
       if (same) {
-        store_unit(reinterpret_cast<uint4*>(out + idx), Elem<T>::pack(v));
+        store_unit<KEEP>(reinterpret_cast<uint4*>(out + idx), Elem<T>::pack(v));
       } else {
 #pragma unroll
         for (int j = 0; j < E; ++j) Elem<T>::store(out + idx + j, v[j]);
@@ -542,7 +547,7 @@ __device__ __forceinline__ bool same_boundaries(const T* z, const T* out) {
 }
 
 // The same for the units [u0, u1) of a row and, for the first segment, its ragged elements.
-template <typename T, int NT, typename F>
+template <typename T, int NT, bool KEEP, typename F>
 __device__ __forceinline__ void map_row(const Row<T>& row, T* out, int u0, int u1, int ragged, const F& f) {
   const bool same = same_boundaries(row.z, out);
   if ((int)threadIdx.x < ragged) {
@@ -550,7 +555,8 @@ __device__ __forceinline__ void map_row(const Row<T>& row, T* out, int u0, int u
     Elem<T>::store(out + idx, split(f(pair(Elem<T>::load(row.z + idx), 0.f), idx)).x);
   }
   const FromMemory src{row.unit_ptr()};
-  for (int u = u0 + (int)threadIdx.x; u < u1; u += kBatch * NT) map_batch<T, NT>(row, src, out, same, u, u1, f, [] {});
+  for (int u = u0 + (int)threadIdx.x; u < u1; u += kBatch * NT)
+    map_batch<T, NT, KEEP>(row, src, out, same, u, u1, f, [] {});
 }
 
 template <typename T, int NT>
@@ -558,7 +564,7 @@ __device__ __forceinline__ void zero_row(const Row<T>& out, int u0, int u1, int 
   T* o = const_cast<T*>(out.z);
   if ((int)threadIdx.x < ragged) Elem<T>::store(o + out.ragged_index(threadIdx.x), 0.f);
   uint4* p = const_cast<uint4*>(out.unit_ptr());
-  for (int u = u0 + (int)threadIdx.x; u < u1; u += NT) store_unit(p + u, make_uint4(0, 0, 0, 0));
+  for (int u = u0 + (int)threadIdx.x; u < u1; u += NT) store_unit<false>(p + u, make_uint4(0, 0, 0, 0));
 }
 
 // ------------------------------------------------------------------ host
