@@ -358,6 +358,7 @@ struct NoMarks {};
 
 // Where a row's units come from: memory, or units [u0, ..) staged in shared memory.
 struct FromMemory {
+  static constexpr bool kPatch = false;
   const uint4* p;
   __device__ __forceinline__ void begin(int) const {}
   __device__ __forceinline__ uint4 load(int u) const { return load_unit(p + u); }
@@ -385,6 +386,17 @@ __device__ __forceinline__ void stream_units(const Src& src, int u0, int u1, flo
     const int u = base + (int)(threadIdx.x & 31);
     const bool whole = base + (UN - 1) * NT + 32 <= u1;
     src.begin(batch);
+    uint32_t set = 0;
+    if constexpr (MASK) {
+      set = marks.of_batch(batch);
+      if constexpr (Src::kPatch) {
+        // The lane's own units: no one else reads them.
+        for (; set; set &= set - 1) {
+          const int b = __ffs(set) - 1;
+          src.template patch<T>(u + b / E * NT, b % E);
+        }
+      }
+    }
     uint4 q[UN];
     if (whole) {
 #pragma unroll
@@ -396,9 +408,7 @@ __device__ __forceinline__ void stream_units(const Src& src, int u0, int u1, flo
         if (u + i * NT < u1) q[i] = src.load(u + i * NT);
       }
     }
-    uint32_t set = 0;
     if constexpr (MASK) {
-      set = marks.of_batch(batch);
       if (set) {
 #pragma unroll
         for (int i = 0; i < UN; ++i)

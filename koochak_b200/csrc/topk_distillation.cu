@@ -266,7 +266,8 @@ __global__ void __launch_bounds__(NT)
 
 // A row's units [0, ..) staged in shared memory.
 struct FromStage {
-  const uint4* stage;
+  static constexpr bool kPatch = true;  // marked elements are put to -inf where they are
+  uint4* stage;
   uint64_t* full;
   uint32_t parity;
   volatile int* abort_flag;
@@ -276,6 +277,10 @@ struct FromStage {
     mbar_wait(&full[batch], parity, abort_flag, status, kStatusTimeoutRowStage);
   }
   __device__ __forceinline__ uint4 load(int u) const { return stage[u]; }
+  template <typename T>
+  __device__ __forceinline__ void patch(int u, int j) const {
+    Elem<T>::store(reinterpret_cast<T*>(stage + u) + j, -INFINITY);
+  }
 };
 
 // Loss and gradient of each row in one go: the logits are read from memory once and the gradient written once.
@@ -359,6 +364,7 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
       if constexpr (TAIL) stream_units<T, NT, false>(src, 0, row.units, c, run, marks, [](int, float) {});
       else stream_units<T, NT, false>(src, 0, row.units, c, run, NoMarks{}, [](int, float) {});
       const Acc mine = run.total(c);
+      if (TAIL) fence_proxy_async_smem();  // what was put to -inf is overwritten by a bulk copy next
       if (lane == 0) {
         sums[tid >> 5] = mine;
         mbar_arrive(&sh.joined);
