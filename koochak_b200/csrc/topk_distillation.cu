@@ -364,7 +364,6 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
       if constexpr (TAIL) stream_units<T, NT, false>(src, 0, row.units, c, run, marks, [](int, float) {});
       else stream_units<T, NT, false>(src, 0, row.units, c, run, NoMarks{}, [](int, float) {});
       const Acc mine = run.total(c);
-      if (TAIL) fence_proxy_async_smem();  // what was put to -inf is overwritten by a bulk copy next
       if (lane == 0) {
         sums[tid >> 5] = mine;
         mbar_arrive(&sh.joined);
@@ -379,6 +378,9 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
       const bool same = same_boundaries(row.z, o);
       for (int i = 0; i < chunks; ++i) {
         map_batch<T, NT, true>(row, src, o, same, i * kChunk + tid, row.units, gradient, [&] {
+          // The chunk's place is written by a bulk copy next, through another proxy: without the fence that copy could
+          // overtake these loads (it did, for some hundred of 10^9 elements), and what was put to -inf.
+          fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.empty[i]);
         });

@@ -586,6 +586,32 @@ def test_rows_left_out_in_any_order(tail, left_out, how):
 
 
 @gpu
+@pytest.mark.parametrize("tail", [False, True])
+def test_every_element_of_a_large_gradient(tail):
+    """Loss and gradient together against the two kernels apart, element by element and several times: chunks of a row
+    are replaced by the next row's while the gradient is written.
+
+    A dense element is coef 2^x with coef free of cancellation here (no rest): both sides round the same number, known
+    to 2^-18, to bf16, so they differ by at most one step, 2^-7 of the value."""
+
+    rows, vocab, k = 16384, 50257, 64
+    gen = torch.Generator(DEV).manual_seed(5)
+    z = torch.empty(rows, 50304, device=DEV, dtype=torch.bfloat16).normal_(generator=gen).mul_(2)[:, :vocab]
+    ids = (torch.randint(0, vocab, (rows, 1), device=DEV, generator=gen) + 7919 * torch.arange(k, device=DEV)) % vocab
+    z.scatter_(1, ids, torch.randn(rows, k, device=DEV, generator=gen).add_(8).bfloat16())
+    t = torch.log_softmax(torch.randn(rows, k, device=DEV, generator=gen), -1) + 1e-6
+    loss, stats = kf.topk_distillation_forward(z, ids, t, tail=tail)
+    want = kf.topk_distillation_backward(z, ids, t, stats, tail=tail).scatter_(1, ids, 0.0)
+    for _ in range(6):
+        got_loss, _, got = kf.topk_distillation_grad(z, ids, t, tail=tail)
+        got.scatter_(1, ids, 0.0)
+        off = sum(int(((a.float() - b.float()).abs_() > b.float().abs_() * 2.0**-7).sum())
+                  for a, b in zip(got.split(2048), want.split(2048)))
+        assert off == 0, f"{off} elements"
+        assert (got_loss - loss).abs().max() < (16 + math.log(vocab)) * 2.0**-19
+
+
+@gpu
 def test_student_mass_far_below_fp32():
     """The rest's probability is a sum of its own: exact where one minus the listed mass would be zero."""
 
