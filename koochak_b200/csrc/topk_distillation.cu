@@ -613,7 +613,7 @@ void topk_distillation_forward(const at::Tensor& logits, const at::Tensor& ids, 
       if (together) {
         auto kern = distill_grad_kernel<T, kGradThreads, TAIL>;
         const int per_sm = allow_smem(kern, (size_t)staged, kGradThreads + 64, device);
-        const int64_t blocks = std::min<int64_t>(rows, (int64_t)std::max(1, per_sm) * num_sms(device));
+        const int64_t blocks = std::min<int64_t>(rows, (int64_t)std::max(1, per_sm) * compute_sms(device));
         launch_rows(kern, blocks, kGradThreads + 64, 1, (size_t)staged, s, (const T*)logits.data_ptr(), logits.stride(0),
                     (T*)out->data_ptr(), out->stride(0), (int)vocab, rows, ids.data_ptr<int64_t>(),
                     teacher.data_ptr<float>(), k, c, inv_t, w, loss.data_ptr<float>(), kept, stage_units,

@@ -302,7 +302,7 @@ def test_logprobs_shapes(dtype, rows, vocab, layout):
 @pytest.mark.parametrize("vocab", [128, 1000, 4100, 4500, 50257])
 @pytest.mark.parametrize("top_k", [1, 2, 31, 33, 128])
 def test_alternatives(dtype, vocab, top_k):
-    _check_logprobs(_logits(5, vocab, dtype, "contiguous", seed=top_k), None, top_k=top_k, grads=False)
+    _check_logprobs(_logits(5, vocab, dtype, "contiguous", seed=top_k), None, top_k=top_k, grads=top_k == 2)
 
 
 @gpu
@@ -644,6 +644,53 @@ def test_teacher_to_student_run():
 
 
 @gpu
+def test_expanded_logits_and_empty_batches():
+    """One row of logits for many tokens (stride zero), whose gradient is the sum; batches of no rows."""
+
+    row = _logits(1, 3001, torch.float32, "contiguous").requires_grad_()
+    tok = _tokens(7, 3001, ignored=False)
+    ids, t = _teacher(7, 3001, 5, True)
+    z = row.expand(7, -1)
+    res = kf.token_logprobs(z, tok)
+    a, = torch.autograd.grad(res.logprobs.sum() + res.entropy.sum() + kf.topk_distillation(z, ids, t, tail=True).sum()
+                             + kf.topk_distillation(z, ids, t, tail=True, reduction="sum"), row)
+    rr = row.detach().cpu().double().requires_grad_()
+    lp, ent, _, _ = kf.token_logprobs_ref(rr.expand(7, -1), tok.cpu())
+    kd = kf.topk_distillation_ref(rr.expand(7, -1), ids.cpu(), t.cpu(), tail=True)
+    (lp.sum() + ent.sum() + 2 * kd.sum()).backward()
+    # 28 gradients, each within 2^-16 (see _check_distill) of factors of at most 1 + H
+    _close(a, rr.grad, 28 * 2.0**-16 * (1 + math.log(3001)), "sum over the expanded rows")
+    for dtype in DTYPES:
+        e = torch.empty(0, 3001, device=DEV, dtype=dtype, requires_grad=True)
+        none = kf.token_logprobs(e, tok[:0], top_k=3)
+        total = none.logprobs.sum() + none.entropy.sum() + kf.topk_distillation(e, ids[:0], t[:0]).sum()
+        total = total + kf.topk_distillation(e, ids[:0], t[:0], weight=t[:0, 0], reduction="sum")
+        total.backward()
+        assert total == 0 and e.grad.shape == e.shape
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_widest_vocabulary_in_a_batch(dtype):
+    """Two rows of 524288 repeated: blocks of their own instead of the clusters that take the two alone."""
+
+    two = _logits(2, 1 << 19, dtype, "contiguous")
+    ids, t = _teacher(2, 1 << 19, 30, True, ragged=False)
+    tok = _tokens(2, 1 << 19, ignored=False)
+    n = 200
+    z = two.repeat(n, 1)
+    want = kf.token_logprobs(two, tok, top_k=128)
+    got = kf.token_logprobs(z, tok.repeat(n), top_k=128)
+    assert torch.equal(got.top_ids, want.top_ids.repeat(n, 1))
+    # both within their tolerance of the exact value
+    _close(got.logprobs, want.logprobs.repeat(n), 2 * _logprob_tol(want.logprobs.double()).repeat(n), "logprobs")
+    loss = kf.topk_distillation(z, ids.repeat(n, 1), t.repeat(n, 1), tail=True)
+    one = kf.topk_distillation(two, ids, t, tail=True)
+    _close(loss, one.repeat(n), 2 * (16 + math.log(1 << 19)) * 2.0**-20, "loss")
+    _check_distill(two, ids, t, True)
+
+
+@gpu
 def test_broadcast_gradients_and_reuse():
     """Expanded upstream gradients, two losses on one set of logits, and backward twice."""
 
@@ -708,6 +755,35 @@ def test_other_stream_and_graph():
 
 
 @gpu
+def test_capture_beside_an_eager_graph_of_the_same_leaf():
+    """Eager calls and the capture run on one stream, as in the loop's graph mode: the leaf's accumulation node of a graph
+    made on the default stream would make torch refuse the capture, whatever the ops are."""
+
+    z = _logits(20, 1003, torch.bfloat16, "contiguous").requires_grad_()
+    ids, t = _teacher(20, 1003, 6, True)
+
+    def loss():
+        return kf.topk_distillation(z, ids, t, tail=True, reduction="sum") + kf.token_logprobs(z).entropy.sum()
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        alive = loss()
+        want = torch.autograd.grad(loss(), z)[0]
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = torch.autograd.grad(loss(), z)[0]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    with torch.cuda.stream(stream):
+        (later,) = torch.autograd.grad(alive, z)
+    torch.cuda.synchronize()
+    assert torch.equal(later, want)
+
+
+@gpu
 def test_repeatable():
     z = _logits(500, 32000, torch.bfloat16)
     tok = _tokens(500, 32000)
@@ -745,6 +821,20 @@ def test_offsets_beyond_32_bits():
     loss, stats = kf.topk_distillation_forward(z, ids, t, tail=True)
     d = kf.topk_distillation_backward(z, ids, t, stats, tail=True, out=z)
     assert not d[:-3].any() and d[-3:].any(1).all()
+    del z, d
+    rows, vocab = 46000, 50257  # the same for rows that are staged
+    z = torch.zeros(rows, vocab, device=DEV, dtype=torch.bfloat16)
+    z[-2:] = _logits(2, vocab, torch.bfloat16, "contiguous")
+    ids = torch.full((rows, 8), -1, device=DEV)
+    ids[-2:], t = _teacher(2, vocab, 8, False, ragged=False)
+    t = t.repeat(rows // 2, 1)
+    small = z[-2:].clone()
+    loss, _, d = kf.topk_distillation_grad(z, ids, t, out=z)
+    lone, _, done = kf.topk_distillation_grad(small, ids[-2:], t[-2:], out=small)
+    assert not d[:-2].any() and not loss[:-2].any()
+    # as in test_every_element_of_a_large_gradient, and twice the gradient's own tolerance on the list
+    _close(d[-2:], done, done.double().abs() * 2.0**-7 + 2.0**-15, "dlogits")
+    _close(loss[-2:], lone, (16 + math.log(vocab)) * 2.0**-19, "loss")
 
 
 @gpu
