@@ -518,19 +518,19 @@ __device__ __forceinline__ void segment(int units, int i, int n, int& u0, int& u
 }
 
 // Writes a thread's batch of units u, u + NT, ...: out = f(two elements, the index of the first). `loaded` is called
-// once the batch is in registers.
-template <typename T, int NT, bool KEEP, typename Src, typename F, typename L>
+// once the batch is in registers. WHOLE: no unit of the batch is behind the end.
+template <typename T, int NT, bool KEEP, bool WHOLE, typename Src, typename F, typename L>
 __device__ __forceinline__ void map_batch(const Row<T>& row, const Src& src, T* out, bool same, int u, int u1,
                                           const F& f, const L& loaded) {
   constexpr int E = Elem<T>::kUnit;
   uint4 q[kBatch];
 #pragma unroll
   for (int i = 0; i < kBatch; ++i)
-    if (u + i * NT < u1) q[i] = src.load(u + i * NT);
+    if (WHOLE || u + i * NT < u1) q[i] = src.load(u + i * NT);
   loaded();
 #pragma unroll
   for (int i = 0; i < kBatch; ++i) {
-    if (u + i * NT < u1) {
+    if (WHOLE || u + i * NT < u1) {
       const int idx = row.head + (u + i * NT) * E;
       float v[E];
       Elem<T>::unpack(q[i], v);
@@ -565,8 +565,10 @@ __device__ __forceinline__ void map_row(const Row<T>& row, T* out, int u0, int u
     Elem<T>::store(out + idx, split(f(pair(Elem<T>::load(row.z + idx), 0.f), idx)).x);
   }
   const FromMemory src{row.unit_ptr()};
-  for (int u = u0 + (int)threadIdx.x; u < u1; u += kBatch * NT)
-    map_batch<T, NT, KEEP>(row, src, out, same, u, u1, f, [] {});
+  int u = u0 + (int)threadIdx.x;
+  for (; u + (kBatch - 1) * NT < u1; u += kBatch * NT)
+    map_batch<T, NT, KEEP, true>(row, src, out, same, u, u1, f, [] {});
+  if (u < u1) map_batch<T, NT, KEEP, false>(row, src, out, same, u, u1, f, [] {});
 }
 
 template <typename T, int NT>

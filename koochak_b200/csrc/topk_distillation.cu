@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
       };
       const bool same = same_boundaries(row.z, o);
       for (int i = 0; i < chunks; ++i) {
-        map_batch<T, NT, true>(row, src, o, same, i * kChunk + tid, row.units, gradient, [&] {
+        map_batch<T, NT, true, false>(row, src, o, same, i * kChunk + tid, row.units, gradient, [&] {
           // The chunk's place is written by a bulk copy next, through another proxy: without the fence that copy could
           // overtake these loads (it did, for some hundred of 10^9 elements), and what was put to -inf.
           fence_proxy_async_smem();
@@ -594,7 +594,7 @@ void topk_distillation_forward(const at::Tensor& logits, const at::Tensor& ids, 
   const int stage_units = (int)((units + 7) / 8 * 8);
   const int64_t staged = 16 * (int64_t)stage_units + 4 * Marks<__half, kGradThreads>::size(stage_units);
   const bool twice = out && row_bytes <= 32 * 1024;
-  const bool together = out && !twice && staged <= 108 * 1024 && rows >= num_sms(device);
+  const bool together = out && !twice && staged <= 107 * 1024 && rows >= num_sms(device);
   if (out && !twice && !together) {
     KB_CHECK(stats.has_value(), "the gradient needs stats");
     topk_distillation_forward(logits, ids, teacher, weight, loss, stats, c10::nullopt, vocab, temperature, tail);
