@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(NT, 1280 / NT)
     mine = tid < ragged ? Elem<T>::load(row.z + row.ragged_index(tid)) : -INFINITY;
     run.add_one(mine, c);
   }
-  __shared__ Acc join_sm[NT / 32], result;
+  __shared__ Acc join_sm[NT / 32], result, own;
   __shared__ std::conditional_t<TOPK, SelectShared<NT>, int> sh;
   stream_units<T, NT, TOPK>(FromMemory{row.unit_ptr()}, u0, u1, c, run, NoMarks{}, [&](int batch, float mx) {
     if constexpr (TOPK) {
@@ -323,7 +323,21 @@ __global__ void __launch_bounds__(NT, 1280 / NT)
       kept = batch < sh.kGroups ? mx : max_nan(kept, mx);
     }
   });
-  Acc all = block_join<NT, true>(run, c, join_sm);
+  // The thread that saw the given token stays out of the sum: see below.
+  const bool inside = tokens && token >= 0 && token < V;
+  const int per = (row.units + parts - 1) / parts;
+  int owner = -1, owner_part = 0;
+  if (inside) {
+    const int at = (int)token - row.head;
+    owner = at < 0 ? (int)token : (int)token - row.units * Elem<T>::kUnit;  // a ragged element's
+    if (at >= 0 && at < row.units * Elem<T>::kUnit) {
+      owner_part = at / Elem<T>::kUnit / per;
+      owner = (at / Elem<T>::kUnit - owner_part * per) % NT;
+    }
+    if (tid == owner && part == owner_part) own = run.take(c);
+  }
+  Acc all = block_join<NT, true>(run, c, join_sm), theirs;
+  if (!SPLIT && inside) theirs = own;
   if constexpr (SPLIT) {
     __shared__ unsigned long long sorted[TOPK ? kMaxList : 1];
     if (tid == 0) result = all;
@@ -338,6 +352,7 @@ __global__ void __launch_bounds__(NT, 1280 / NT)
         all = *cg::this_cluster().map_shared_rank(&result, (tid & 7) < parts ? tid & 7 : 0);
         if ((tid & 7) >= parts) all = Acc();
         all = join_lanes<8, true>(all, c);
+        if (inside) theirs = *cg::this_cluster().map_shared_rank(&own, owner_part);
       }
       if constexpr (TOPK) {
         for (int i = tid; i < parts * k; i += NT) sh.merged[i] = *cg::this_cluster().map_shared_rank(&sorted[i % k], i / k);
@@ -347,20 +362,54 @@ __global__ void __launch_bounds__(NT, 1280 / NT)
     if (part != 0) return;
   }
   // Log probabilities are taken in units of z / T, not of c z: (lowest - m) c would overflow.
-  if (tid == 0) {
+  if (tid < 32) {
+    const Acc others = all;
+    if (inside) all.join<true>(theirs.m, theirs.s, theirs.a, c);
     const float log2s = log2f(all.s);
-    if (tokens) {
-      const bool inside = token >= 0 && token < V;
-      logprobs[row_i] = inside ? (Elem<T>::load(row.z + token) - all.m) * inv_t - kLn2 * log2s : NAN;
+    float logp = NAN, h = kLn2 * (log2s - all.a / all.s);
+    if (inside) {
+      const float z = Elem<T>::load(row.z + token), x = (z - all.m) * c, e = ex2(x);
+      logp = (z - all.m) * inv_t - kLn2 * log2s;
+      if (2.f * e > all.s) {
+        // A token more likely than all others together: ln p and the entropy are small differences of large numbers,
+        // unless they are taken from the rest of the sum, -ln p = ln(1 + rest / e) and
+        // H = -ln p - sum over the rest of p_j ln 2 (x_j - x). What the token's thread has added to it is summed anew.
+        Acc rest;
+        rest.m = all.m;
+        const int first = owner_part * per + owner, last = min(row.units, (owner_part + 1) * per);
+        const auto add = [&](float v) {
+          const float y = (v - all.m) * c, f = ex2(y);
+          rest.s += f;
+          rest.a = fmaf(f, fmaxf(y, -256.f), rest.a);
+        };
+        for (int u = first + tid * NT; u < last; u += 32 * NT) {
+          float v[Elem<T>::kUnit];
+          Elem<T>::unpack(load_unit(row.unit_ptr() + u), v);
+#pragma unroll
+          for (int j = 0; j < Elem<T>::kUnit; ++j)
+            if (row.head + u * Elem<T>::kUnit + j != (int)token) add(v[j]);
+        }
+        if (tid == 0 && owner_part == 0 && owner < row.ragged && row.ragged_index(owner) != (int)token)
+          add(Elem<T>::load(row.z + row.ragged_index(owner)));
+        rest.s = warp_sum(rest.s);
+        rest.a = warp_sum(rest.a);
+        rest.join<true>(others.m, others.s, others.a, c);
+        const float l = log1pf(rest.s / e);
+        logp = -l;
+        h = l - kLn2 * (rest.a - x * rest.s) / (rest.s + e);
+      }
     }
-    entropy[row_i] = kLn2 * (log2s - all.a / all.s);
-    if (stats) {
-      stats[kStats * row_i] = all.m;
-      stats[kStats * row_i + 1] = log2s;
-    }
-    if (TOPK) {
-      result.m = all.m;
-      result.s = kLn2 * log2s;
+    if (tid == 0) {
+      if (tokens) logprobs[row_i] = logp;
+      entropy[row_i] = h;
+      if (stats) {
+        stats[kStats * row_i] = all.m;
+        stats[kStats * row_i + 1] = log2s;
+      }
+      if (TOPK) {
+        result.m = all.m;
+        result.s = kLn2 * log2s;
+      }
     }
   }
   if constexpr (TOPK) {

@@ -314,6 +314,33 @@ def test_logprobs_temperature(dtype, temperature):
     _check_logprobs(z, _tokens(6, 5000), top_k=7, temperature=temperature)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,layout", [(12, 1003, "offset"), (12, 50257, "padded"), (3, 50257, "contiguous"),
+                                               (500, 4099, "contiguous")])
+def test_likely_tokens_keep_their_digits(dtype, rows, vocab, layout):
+    """-log p and the entropy of a token that has nearly all of the probability, relative to their own size.
+
+    -log p = log(1 + rest / e): the rest is a sum of terms 2^x, off by 2^-22 and by ln 2 |x| 2^-24 with |x| below 64,
+    relative, 2^-18 together; as much again for its sum, the ratio and the logarithm. The entropy's terms carry the
+    same once more through x. The reference takes the rest apart too: 1 + 1e-10 loses digits in 64 bits already."""
+
+    z = _logits(rows, vocab, dtype, layout, sigma=1.0)
+    tok = _tokens(rows, vocab, ignored=False)
+    tok[0], tok[1], tok[2] = 0, vocab - 1, min(8, vocab - 1)
+    z.scatter_(1, tok[:, None], (torch.arange(rows, device=DEV) % 12 * 2.0 + 12.0)[:, None].to(dtype))
+    res = kf.token_logprobs(z, tok)
+    d = z.double() - z.double().gather(1, tok[:, None])
+    e = d.exp().scatter_(1, tok[:, None], 0.0)
+    logp = -torch.log1p(e.sum(1))
+    ent = (-logp - (e * d).sum(1) / (1 + e.sum(1))).cpu()
+    logp = logp.cpu()
+    assert (logp > -0.6).any() and (rows < 12 or (logp > -1e-8).any())
+    likely = logp > math.log(0.5) + 1e-3
+    _close(res.logprobs.cpu()[likely], logp[likely], logp[likely].abs() * 2.0**-17, "logprobs")
+    _close(res.entropy.cpu()[likely], ent[likely], ent[likely] * 2.0**-16, "entropy")
+
+
 def _hard_rows(vocab, dtype, device):
     """Rows where selection and sums can go wrong: ties, masks, order in memory, extremes."""
 
