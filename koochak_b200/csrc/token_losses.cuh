@@ -3,14 +3,14 @@
 //
 // Notation: z is a row of V logits, c = log2(e) / T, m = max z,
 // S = sum_j 2^((z_j - m) c), so p_j = 2^((z_j - m) c) / S is softmax(z / T)
-// and ln p_j = ln 2 ((z_j - m) c - log2 S). Differences to the maximum are
-// taken before the scaling: they are exact for near values, and a row whose
-// entries all are the type's lowest value is a uniform one instead of an
-// overflow. A row of -inf only has no distribution and gives NaN.
+// and ln p_j = ln 2 ((z_j - m) c - log2 S). A row whose entries all are the
+// type's lowest value is a uniform one, not an overflow. A row of -inf only has
+// no distribution and gives NaN.
 //
-// Statistics are held in fp32 per thread (maximum, sum, and for the entropy
-// A = sum 2^x x with x = (z_j - m) c), rescaled when the thread's maximum
-// grows, and joined in a fixed order, so results do not depend on timing.
+// Statistics are held in fp32 per warp (a reference near the maximum, the sum,
+// and for the entropy A = sum 2^x x with x = (z_j - m) c), rescaled when the
+// reference grows, and joined in a fixed order, so results do not depend on
+// timing.
 #pragma once
 
 #include <ATen/ATen.h>
