@@ -526,7 +526,7 @@ void token_logprobs_forward(const at::Tensor& logits, const OptTensor& tokens, c
   int64_t* ti = top_ids ? top_ids->data_ptr<int64_t>() : nullptr;
   for_logits_type(logits.scalar_type(), [&](auto tag) {
     using T = typename decltype(tag)::type;
-    const RowLaunch how = row_launch(rows, vocab * (int64_t)sizeof(T), logits.get_device());
+    const RowLaunch how = row_launch(rows, vocab * (int64_t)sizeof(T), false, logits.get_device());
     for_bool(k > 0, [&](auto top_tag) {
       for_row_launch(how, [&](auto nt_tag, auto split_tag) {
         constexpr int NT = decltype(nt_tag)::value;

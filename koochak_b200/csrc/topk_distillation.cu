@@ -628,7 +628,7 @@ void topk_distillation_forward(const at::Tensor& logits, const at::Tensor& ids, 
                     teacher.data_ptr<float>(), k, c, inv_t, w, loss.data_ptr<float>(), kept);
         return;
       }
-      const RowLaunch how = row_launch(rows, vocab * (int64_t)sizeof(T), device);
+      const RowLaunch how = row_launch(rows, vocab * (int64_t)sizeof(T), true, device);
       for_row_launch(how, [&](auto nt_tag, auto split_tag) {
         constexpr int NT = decltype(nt_tag)::value;
         auto kern = distill_forward_kernel<T, NT, TAIL, decltype(split_tag)::value, false>;
