@@ -301,7 +301,7 @@ struct GradShared {
   KdStats stats;
   float weight[2];
   int some[2], fetch[2];
-  uint64_t full[kChunks], empty[kChunks], told, ready, joined, solved, done;
+  uint64_t full[kChunks], empty[kChunks], told[2], ready, joined, solved, done;
   int abort_flag;
 };
 
@@ -324,7 +324,8 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.empty[i], NW);
     }
-    mbar_init(&sh.told, 1);
+    mbar_init(&sh.told[0], 1);
+    mbar_init(&sh.told[1], 1);
     mbar_init(&sh.ready, 1);
     mbar_init(&sh.joined, NW);
     mbar_init(&sh.solved, 1);
@@ -337,9 +338,12 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     mbar_wait(bar, parity & 1u, &sh.abort_flag, status, kStatusTimeoutRowStage);
   };
-  // Rows so far, and rows with slots: `full` and `empty` complete once per row with slots, the other barriers
-  // once per row, each only after everyone who waits on it has seen the row before: told, joined and solved(n + 1) follow
-  // done(n), ready(n + 1) follows joined(n), and done(n) needs every warp to have seen solved or told(n).
+  // Rows so far, and rows with slots: `full` and `empty` complete once per row with slots, `told` once per other row (one
+  // barrier for even rows and one for odd ones), the other barriers once per row. Each may complete only after everyone
+  // who waits on it has seen it complete before: joined and solved(n + 1) follow done(n), which needs every streaming warp
+  // to have seen solved(n); ready(n + 1) follows joined(n); told(n + 2) follows done(n), which the fetching warp
+  // arrives on once it has seen told(n + 1). told(n + 1) follows nothing that the fetching warp does in row n, so on one
+  // barrier it could complete twice before that warp looks.
   uint32_t count = 0, staged = 0;
 
   if (tid < NT) {
@@ -398,7 +402,7 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
     // The fetching warp: told(n) says whether row n of this block has slots, or is behind
     // the last.
     for (long long r = blockIdx.x;; r += gridDim.x, ++count) {
-      wait(&sh.told, count);
+      wait(&sh.told[count & 1], count >> 1);
       const bool some = sh.fetch[count & 1];
       __syncwarp();
       if (lane == 0 && count > 0) mbar_arrive(&sh.done);  // of the row before
@@ -476,7 +480,7 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
   auto tell = [&](uint32_t n, bool some) {
     if (lane == 0) {
       sh.fetch[n & 1] = some;
-      mbar_arrive(&sh.told);
+      mbar_arrive(&sh.told[n & 1]);
     }
     __syncwarp();
   };

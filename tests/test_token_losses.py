@@ -614,6 +614,28 @@ def test_rows_left_out_in_any_order(tail, left_out, how):
 
 @gpu
 @pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("rows", [148, 200, 296, 600])
+@pytest.mark.parametrize("how", ["weight", "slots"])
+def test_blocks_whose_only_rows_are_left_out(tail, rows, how):
+    """Staged rows (34 KB) that all are left out, most blocks with a single one: nothing between the fetching warp's first
+    two messages takes time there. Many launches, as the order of the warps differs from one to the next."""
+
+    vocab = 17001
+    z = torch.full((rows, vocab), math.nan, device=DEV, dtype=torch.bfloat16)
+    ids, t = _teacher(rows, vocab, 5, tail, ragged=False)
+    weight = torch.ones(rows, device=DEV)
+    if how == "weight":
+        weight[:] = 0
+    else:
+        ids[:] = -1
+    out = torch.empty_like(z)
+    for _ in range(50):
+        loss, stats, dz = kf.topk_distillation_grad(z, ids, t, weight=weight, tail=tail, out=out.fill_(1.0))
+        assert not loss.any() and not stats.any() and not dz.any()
+
+
+@gpu
+@pytest.mark.parametrize("tail", [False, True])
 def test_every_element_of_a_large_gradient(tail):
     """Loss and gradient together against the two kernels apart, element by element and several times: chunks of a row
     are replaced by the next row's while the gradient is written.
