@@ -19,7 +19,10 @@
 #include <cuda_fp16.h>
 
 #include <cmath>
+#include <map>
+#include <tuple>
 #include <type_traits>
+#include <utility>
 
 #include "host_utils.h"
 #include "token_losses.h"
@@ -710,22 +713,25 @@ void for_row_launch(const RowLaunch& how, F&& f) {
   else f(Int<512>{}, std::false_type{});
 }
 
-// Lets a kernel use `smem` bytes of dynamic shared memory, once per kernel and size; with `threads`, returns how many
-// of its blocks an SM holds.
+// Lets a kernel use `smem` bytes of dynamic shared memory; with `threads`, returns how many of its blocks an SM holds.
+// The limit is one value per kernel and device, which calls with other sizes share: it is only ever raised.
 template <typename Kern>
 int allow_smem(Kern kern, size_t smem, int threads, int device) {
   static std::mutex mu;
-  static std::unordered_map<uint64_t, int> known;
-  const uint64_t key = reinterpret_cast<uint64_t>(reinterpret_cast<const void*>(kern)) * 0x9E3779B97F4A7C15ull ^
-                       ((uint64_t)smem << 16 | (uint64_t)threads << 6 | (uint64_t)device);
+  static std::map<std::pair<const void*, int>, size_t> limits;
+  static std::map<std::tuple<const void*, int, size_t, int>, int> known;
+  const void* const id = reinterpret_cast<const void*>(kern);
   std::lock_guard<std::mutex> lock(mu);
-  const auto it = known.find(key);
-  if (it != known.end()) return it->second;
-  if (smem > 32 * 1024) KB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  int blocks = 0;
-  if (threads) KB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kern, threads, smem));
-  known.emplace(key, blocks);
-  return blocks;
+  size_t& limit = limits.try_emplace({id, device}, 32 * 1024).first->second;
+  if (smem > limit) {
+    KB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    limit = smem;
+  }
+  if (!threads) return 0;
+  const auto at = known.try_emplace({id, device, smem, threads}, 0);
+  if (at.second)
+    KB_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&at.first->second, kern, threads, smem));
+  return at.first->second;
 }
 
 template <typename... P, typename... A>

@@ -635,6 +635,43 @@ def test_blocks_whose_only_rows_are_left_out(tail, rows, how):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("vocabs", [(50257, 32000, 50257), (25001, 50257, 20000, 40000, 25001)])
+def test_vocabularies_one_after_another(dtype, tail, vocabs):
+    """One kernel with more shared memory, less, and more again. Twenty different rows, repeated until blocks of
+    different SMs take them; rows at the same 16-byte boundaries (160 odd rows further on) have the same results."""
+
+    if dtype == torch.float32:
+        vocabs = [v // 2 for v in vocabs]
+    known = {}
+    for vocab in vocabs:
+        z = _logits(20, vocab, dtype, "padded").repeat(10, 1)
+        ids, t = (x.repeat(10, 1) for x in _teacher(20, vocab, 11, tail))
+        weight = torch.rand(20, device=DEV, generator=torch.Generator(DEV).manual_seed(1)).add_(0.5).repeat(10)
+        _check_distill(z, ids, t, tail, weight=weight)
+        got = kf.topk_distillation_grad(z, ids, t, weight=weight, tail=tail)
+        assert all(torch.equal(a[:20], a[160:180]) for a in got)
+        if vocab in known:
+            assert all(torch.equal(a, b) for a, b in zip(got, known[vocab]))
+        known[vocab] = got
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_wide_vocabularies_one_after_another(dtype):
+    """The same for the loss alone, whose marks take 64 KB of shared memory at the widest vocabulary."""
+
+    for vocab in (1 << 19, 300000, 1 << 19, 270000, 400000):
+        z = _logits(1, vocab, dtype, "contiguous")
+        ids, t = _teacher(1, vocab, 20, True, ragged=False)
+        want = kf.topk_distillation_ref(z.double(), ids, t, tail=True)
+        got = kf.topk_distillation(z.expand(400, -1), ids.expand(400, -1), t.expand(400, -1), tail=True)
+        # as in _check_distill: 16 + log V covers |log p| here
+        _close(got, want.expand(400), (16 + math.log(vocab)) * 2.0**-20, "loss")
+
+
+@gpu
 @pytest.mark.parametrize("tail", [False, True])
 def test_every_element_of_a_large_gradient(tail):
     """Loss and gradient together against the two kernels apart, element by element and several times: chunks of a row
