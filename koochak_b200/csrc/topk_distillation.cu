@@ -382,6 +382,9 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
       };
       const bool same = same_boundaries(row.z, o);
       for (int i = 0; i < chunks; ++i) {
+        // Rows at other boundaries may end just before a chunk. No one has waited for it in the first pass then, and it
+        // may not be given up before the fetching warp has come to it.
+        if (i * kChunk >= row.units) wait(&sh.full[i], staged);
         map_batch<T, NT, true, false>(row, src, o, same, i * kChunk + tid, row.units, gradient, [&] {
           // The chunk's place is written by a bulk copy next, through another proxy: without the fence that copy could
           // overtake these loads (it did, for some hundred of 10^9 elements), and what was put to -inf.

@@ -673,6 +673,33 @@ def test_wide_vocabularies_one_after_another(dtype):
 
 @gpu
 @pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype,vocab", [(torch.bfloat16, 32776), (torch.bfloat16, 16392), (torch.float32, 16388)])
+def test_rows_that_end_at_a_chunk(tail, dtype, vocab):
+    """Staged rows with one 16-byte unit more than whole chunks (2048 units) hold, or none where the row starts off a
+    boundary: the last chunk is empty for some of a block's rows and not for others."""
+
+    rows = 1500
+    few = _logits(10, vocab, dtype, "contiguous")
+    buf = torch.empty(rows, vocab + 5, device=DEV, dtype=dtype)[:, 1:1 + vocab]
+    buf.copy_(few.repeat(rows // 10, 1))
+    units = 16 // few.element_size()
+    first = (buf.data_ptr() // few.element_size() + torch.arange(rows) * (vocab + 5)) % units
+    head = -first % units
+    assert len(set(((vocab - head) // units).tolist())) == 2
+    ids, t = _teacher(10, vocab, 9, tail)
+    ids, t = ids.repeat(rows // 10, 1), t.repeat(rows // 10, 1)
+    want_loss, stats = kf.topk_distillation_forward(buf, ids, t, tail=tail)
+    want = kf.topk_distillation_backward(buf, ids, t, stats, tail=tail)
+    for _ in range(5):
+        loss, _, dz = kf.topk_distillation_grad(buf, ids, t, tail=tail)
+        # Loss: both kernels within (16 + log V) 2^-20 of the exact value. Gradient: 2^-16 each (see _check_distill), and
+        # half a step of the logits' type each, relative.
+        _close(loss, want_loss, (16 + math.log(vocab)) * 2.0**-19, "loss")
+        _close(dz, want, 2.0**-15 + 2 * _half_step(dtype) * want.double().abs().cpu(), "dlogits")
+
+
+@gpu
+@pytest.mark.parametrize("tail", [False, True])
 def test_every_element_of_a_large_gradient(tail):
     """Loss and gradient together against the two kernels apart, element by element and several times: chunks of a row
     are replaced by the next row's while the gradient is written.
