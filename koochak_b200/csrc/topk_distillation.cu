@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
   for (int i = tid; i < Marks<T, NT>::size(stage_units); i += NT + 64) words[i] = 0;
   __syncthreads();
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    mbar_wait(bar, parity & 1u, &sh.abort_flag, status, kStatusTimeoutRowStage);
+    return mbar_wait(bar, parity & 1u, &sh.abort_flag, status, kStatusTimeoutRowStage);
   };
   // Rows so far, and rows with slots: `full` and `empty` complete once per row with slots, `told` once per other row (one
   // barrier for even rows and one for odd ones), the other barriers once per row. Each may complete only after everyone
@@ -404,16 +404,18 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
   if (tid < NT + 32) {
     // The fetching warp: told(n) says whether row n of this block has slots, or is behind
     // the last.
-    for (long long r = blockIdx.x;; r += gridDim.x, ++count) {
-      wait(&sh.told[count & 1], count >> 1);
+    int filled = chunks;  // chunks of the row under way whose copies are issued
+    for (long long r = blockIdx.x; filled == chunks; r += gridDim.x, ++count) {
+      if (!__all_sync(0xffffffffu, wait(&sh.told[count & 1], count >> 1))) break;
       const bool some = sh.fetch[count & 1];
       __syncwarp();
       if (lane == 0 && count > 0) mbar_arrive(&sh.done);  // of the row before
       if (r >= rows) return;
       if (!some) continue;
       const Row<T> row(logits + r * ld, V);
-      for (int i = 0; i < chunks; ++i) {
-        if (staged > 0) wait(&sh.empty[i], staged - 1);
+      for (filled = 0; filled < chunks; ++filled) {
+        const int i = filled;
+        if (staged > 0 && !__all_sync(0xffffffffu, wait(&sh.empty[i], staged - 1))) break;
         if (lane == 0) {
           const int n = min(kChunk, row.units - i * kChunk);
           if (n > 0) {
@@ -425,8 +427,15 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
         }
         __syncwarp();
       }
-      ++staged;
+      if (filled == chunks) ++staged;
     }
+    // A wait ran out: no more is fetched, and what is on its way to this block's memory is waited for (with a limit).
+    volatile int never = 0;
+    for (int i = 0; i < chunks; ++i) {
+      const uint32_t copies = staged + (filled < chunks && i < filled ? 1 : 0);
+      if (copies > 0 && !mbar_wait(&sh.full[i], (copies - 1) & 1u, &never, status, kStatusTimeoutDrain)) break;
+    }
+    return;
   }
 
   // The serving warp. Slots lane, lane + 32, ... of the row that comes next:
