@@ -2,6 +2,8 @@
 // rows of a decoding step or a short batch the host's work (checks,
 // allocations, autograd nodes) outweighs the kernels'.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -178,13 +180,24 @@ Logprobs token_logprobs(const at::Tensor& logits, const OptTensor& given, int64_
           top_k > 0 ? OptTensor(out[top + 1]) : OptTensor()};
 }
 
+// Names the graph capture that the current stream of a device is in; 0 outside of any.
+int64_t capture_id(const at::Tensor& t) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(c10::cuda::getCurrentCUDAStream(t.get_device()).stream(), &status, &id));
+  return status == cudaStreamCaptureStatusActive ? (int64_t)id : 0;
+}
+
 // Loss rows, or with a weight their weighted sum.
 //
 // The sum's gradient is written by the forward kernel, for an upstream
 // gradient of one, while the row is on the chip; the backward pass leaves it
 // where the upstream gradient is one (told on the device) and computes it anew
 // otherwise, so it is rounded once in either case. fp16 logits, whose loss
-// goes through a gradient scaler, take the two passes at once.
+// goes through a gradient scaler, take the two passes at once. A backward pass
+// captured without its forward pass runs many times on one forward pass, with
+// other upstream gradients and on what was made of its last result, so it
+// computes its own.
 struct DistillationFn : torch::autograd::Function<DistillationFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& ids,
                             const at::Tensor& teacher, const OptTensor& weight, double temperature, bool tail) {
@@ -198,7 +211,10 @@ struct DistillationFn : torch::autograd::Function<DistillationFn> {
     ctx->save_for_backward({logits, ids, teacher, weight ? *weight : at::Tensor(), stats});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["tail"] = tail;
-    if (dz) ctx->saved_data["dz"] = *dz;
+    if (dz) {
+      ctx->saved_data["dz"] = *dz;
+      ctx->saved_data["capture"] = capture_id(z);
+    }
     return weight ? loss.sum() : loss;
   }
 
@@ -211,7 +227,7 @@ struct DistillationFn : torch::autograd::Function<DistillationFn> {
     const bool summed = saved[3].defined();
     // A gradient that is there is handed out once; a second backward pass computes its own.
     const auto found = ctx->saved_data.find("dz");
-    const bool ready = found != ctx->saved_data.end();
+    const bool ready = found != ctx->saved_data.end() && ctx->saved_data["capture"].toInt() == capture_id(z);
     at::Tensor dz;
     if (ready) {
       dz = found->second.toTensor();

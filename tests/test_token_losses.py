@@ -897,6 +897,45 @@ def test_capture_beside_an_eager_graph_of_the_same_leaf():
 
 
 @gpu
+@pytest.mark.parametrize("vocab", [1003, 20001])
+@pytest.mark.parametrize("captured_forward", [False, True])
+def test_backward_captured_apart_from_its_forward(vocab, captured_forward):
+    """A backward pass in a graph of its own: every replay is the gradient for the upstream factor of that replay, and
+    what was done to an earlier replay's result does not matter."""
+
+    rows = 200
+    z = _logits(rows, vocab, torch.bfloat16, "contiguous").requires_grad_()
+    ids, t = _teacher(rows, vocab, 6, True)
+    w = torch.rand(rows, device=DEV)
+    up = torch.ones((), device=DEV)
+
+    def loss():
+        return kf.topk_distillation(z, ids, t, tail=True, weight=w, reduction="sum")
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        want = {f: torch.autograd.grad(loss(), z, torch.full((), f, device=DEV))[0] for f in (1.0, 3.0)}
+        eager = None if captured_forward else loss()
+    stream.synchronize()
+    forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    if captured_forward:
+        with torch.cuda.graph(forward, stream=stream):
+            eager = loss()
+        forward.replay()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(backward, stream=stream):
+        (out,) = torch.autograd.grad(eager, z, up)
+    for f in (1.0, 3.0, 1.0, 1.0):
+        up.fill_(f)
+        backward.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[f]), f
+        out.mul_(0.5)  # as clipping by norm does
+        torch.cuda.synchronize()
+
+
+@gpu
 def test_repeatable():
     z = _logits(500, 32000, torch.bfloat16)
     tok = _tokens(500, 32000)
