@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <stdexcept>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -87,6 +88,12 @@ at::Tensor once_differentiable(const at::Tensor& dz, const variable_list& grads,
   return (*err)(variable_list{dz.detach().requires_grad_()})[0];
 }
 
+// A tangent of the logits would not reach the results: the kernels have no forward mode.
+void refuse_tangent(const at::Tensor& logits, const char* name) {
+  require<std::runtime_error>(!logits._fw_grad(/*level=*/0).defined(), name,
+                              ": forward-mode differentiation is not supported on CUDA");
+}
+
 using Logprobs = std::tuple<OptTensor, at::Tensor, OptTensor, OptTensor>;
 
 struct LogprobsOut {
@@ -154,6 +161,7 @@ struct LogprobsFn : torch::autograd::Function<LogprobsFn> {
 Logprobs token_logprobs(const at::Tensor& logits, const OptTensor& given, int64_t top_k, double temperature,
                         int64_t ignore_index) {
   const char* name = "token_logprobs";
+  refuse_tangent(logits, name);
   at::Tensor z;
   {
     at::NoGradGuard no_grad;
@@ -247,6 +255,7 @@ struct DistillationFn : torch::autograd::Function<DistillationFn> {
 at::Tensor topk_distillation(const at::Tensor& logits, const at::Tensor& teacher_ids, const at::Tensor& teacher_logits,
                              double temperature, bool tail, const OptTensor& given_weight, bool summed) {
   const char* name = "topk_distillation";
+  refuse_tangent(logits, name);
   const bool differentiable = at::GradMode::is_enabled() && logits.requires_grad();
   at::NoGradGuard no_grad;
   const at::Tensor z = vocab_rows(logits, name);

@@ -284,7 +284,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     zeros and ids of -1; a token outside the vocabulary has a NaN log
     probability. Logits of -inf are never produced (they add nothing to the
     entropy); a row of -inf only, or with a NaN or +inf, gives NaN. NaN logits
-    rank above all others.
+    rank above all others. On CUDA, logits with a forward-mode tangent are
+    refused.
     """
 
     if use_native(logits):
@@ -396,7 +397,8 @@ def topk_distillation(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     returns fp32 losses ``[...]``; ``"sum"`` returns their sum weighted by
     ``weight`` (``[...]``, ones when None), where rows of weight zero are left
     out altogether. The gradient reaches the logits only; it is not scaled by
-    the temperature's square.
+    the temperature's square. On CUDA, logits with a forward-mode tangent are
+    refused.
     """
 
     name = "topk_distillation"

@@ -1000,6 +1000,33 @@ def test_second_derivatives_are_refused():
             g.sum().backward()
 
 
+def _forward_mode(token_logprobs, topk_distillation, device):
+    import torch.autograd.forward_ad as fwad
+
+    z, d = torch.randn(2, 3, 40, device=device).unbind()
+    ids, t = torch.tensor([[3, 5]] * 3, device=device), torch.zeros(3, 2, device=device)
+    with fwad.dual_level():
+        for grad in (False, True):
+            dual = fwad.make_dual(z.clone().requires_grad_(grad), d)
+            for f in (lambda: token_logprobs(dual), lambda: topk_distillation(dual, ids, t)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    f()
+
+
+@gpu
+def test_forward_mode_is_refused():
+    _forward_mode(kf.token_logprobs, kf.topk_distillation, DEV)
+
+
+def test_forward_mode_is_refused_without_a_gpu():
+    from koochak_b200.ops import available, native
+
+    if not available():
+        pytest.skip("native library not built")
+    _forward_mode(lambda z: native().token_logprobs(z, None, 0, 1.0, IGNORE),
+                  lambda z, ids, t: native().topk_distillation(z, ids, t, 1.0, False, None, False), "cpu")
+
+
 @gpu
 def test_logits_changed_after_the_forward_pass_are_noticed():
     z = _logits(3, 64, torch.float32, "contiguous").requires_grad_()
