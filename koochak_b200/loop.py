@@ -598,9 +598,9 @@ class _Run:
         if not (s.ddp_enabled and self.world_size > 1):
             return
         assert dist_lib.is_initialized()
-        if self.on_cuda and str(torch.distributed.get_backend()).lower() == "nccl":
-            from .parallel.ddp import DataParallel
+        from .parallel.ddp import DataParallel, note_wrapper
 
+        if self.on_cuda and str(torch.distributed.get_backend()).lower() == "nccl":
             owners, shard_rest = {}, False
             commit = getattr(self.optimizer, "kb_commit_gradient_plan", None)
             if s.comm_transport.lower() in ("fused", "p2p") and callable(commit):
@@ -625,7 +625,9 @@ class _Run:
                 kw["bucket_cap_mb_list"] = list(s.ddp_bucket_cap_mb_list)
             if self.on_cuda:
                 kw["device_ids"] = [torch.cuda.current_device()]
-            self.model = DistributedDataParallel(self.model, **kw)
+            module = self.model
+            self.model = DistributedDataParallel(module, **kw)
+            note_wrapper(module, self.model)
         self.ctx["model"] = self.model
 
     def _pick_resume(self) -> Optional[str]:

@@ -13,12 +13,14 @@
 
 from __future__ import annotations
 
-from typing import Dict, Iterable, List, Optional
+import threading
+from typing import Any, Dict, Iterable, List, Optional
 
 import torch
 import torch.nn as nn
 
 from ..ops import functional as kf
+from ..parallel.ddp import check_entry
 
 
 def compute_dtype(device: torch.device) -> Optional[torch.dtype]:
@@ -196,7 +198,31 @@ class HeadLogits(torch.autograd.Function):
 
 
 class TokenLosses:
-    """Per-token losses of a language model over its vocabulary; mixed into models that have ``logits(idx)``."""
+    """Per-token losses of a language model over its vocabulary; mixed into models that have ``logits(idx)``.
+
+    ``model(idx, method="distillation_loss", ...)`` is ``model.distillation_loss(idx, ...)`` by way of ``forward``, which
+    data-parallel wrappers need: theirs starts the reduction of the gradients. ``DataParallel`` has the methods too.
+    """
+
+    _entered = threading.local()  # .model: the one whose forward hands a call on
+
+    def _by_method(self, method: str, idx: torch.Tensor, targets, ignore_index: int, options: Dict[str, Any]):
+        if method not in ("logits", "token_logprobs", "distillation_loss"):
+            raise ValueError(f"method must be 'logits', 'token_logprobs' or 'distillation_loss', got {method!r}")
+        if targets is not None:
+            raise ValueError(f"targets do not go with method={method!r}")
+        if method == "token_logprobs":
+            options = {"ignore_index": ignore_index, **options}
+        before = getattr(self._entered, "model", None)
+        self._entered.model = self
+        try:
+            return getattr(self, method)(idx, **options)
+        finally:
+            self._entered.model = before
+
+    def _check_entry(self, name: str) -> None:
+        if getattr(self._entered, "model", None) is not self:
+            check_entry(self, name)
 
     def token_logprobs(self, idx: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, top_k: int = 0,
                        temperature: float = 1.0, ignore_index: int = -100) -> kf.TokenLogprobs:
@@ -206,6 +232,7 @@ class TokenLosses:
         ``distillation_loss(..., tail=True)`` takes.
         """
 
+        self._check_entry("token_logprobs")
         return kf.token_logprobs(self.logits(idx), tokens, top_k=top_k, temperature=temperature,
                                  ignore_index=ignore_index)
 
@@ -215,6 +242,7 @@ class TokenLosses:
         """Mean of ``ops.functional.topk_distillation`` over the positions that have teacher slots, or the mean
         weighted by ``weight`` (``[B, S]``)."""
 
+        self._check_entry("distillation_loss")
         logits = self.logits(idx)
         if weight is None:
             weight = ((teacher_ids >= 0) & (teacher_ids < logits.shape[-1])).any(-1)

@@ -260,7 +260,12 @@ class GPT2(TokenLosses, nn.Module):
             elif isinstance(mod, nn.Embedding):
                 nn.init.normal_(mod.weight, mean=0.0, std=std)
 
-    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, ignore_index: int = -100):
+    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, ignore_index: int = -100, *,
+                method: Optional[str] = None, **options):
+        if method is not None:
+            return self._by_method(method, idx, targets, ignore_index, options)
+        if options:
+            raise TypeError(f"unexpected arguments without a method: {sorted(options)}")
         cdt = compute_dtype(idx.device)
         if cdt is None or targets is None:
             return self._forward_reference(idx, targets, ignore_index)
@@ -290,6 +295,7 @@ class GPT2(TokenLosses, nn.Module):
     def logits(self, idx: torch.Tensor) -> torch.Tensor:
         """Differentiable ``[B, S, vocab]`` logits (16-bit under autocast on CUDA)."""
 
+        self._check_entry("logits")
         cdt = compute_dtype(idx.device)
         if cdt is None:
             return self._forward_reference(idx, None, 0)

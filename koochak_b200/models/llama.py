@@ -306,7 +306,12 @@ class Llama(TokenLosses, nn.Module):
             self._rope[key] = rope_tables(S, D, self.config.rope_theta, device)
         return self._rope[key]
 
-    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, ignore_index: int = -100):
+    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, ignore_index: int = -100, *,
+                method: Optional[str] = None, **options):
+        if method is not None:
+            return self._by_method(method, idx, targets, ignore_index, options)
+        if options:
+            raise TypeError(f"unexpected arguments without a method: {sorted(options)}")
         cdt = compute_dtype(idx.device)
         B, S = idx.shape
         cos, sin = self.rope(S, idx.device)
@@ -338,6 +343,7 @@ class Llama(TokenLosses, nn.Module):
     def logits(self, idx: torch.Tensor) -> torch.Tensor:
         """Differentiable ``[B, S, vocab]`` logits (16-bit under autocast on CUDA)."""
 
+        self._check_entry("logits")
         cdt = compute_dtype(idx.device)
         cos, sin = self.rope(idx.shape[1], idx.device)
         if cdt is None:

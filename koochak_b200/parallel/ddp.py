@@ -47,13 +47,38 @@ from __future__ import annotations
 
 import contextlib
 import os
+import weakref
 from typing import Callable, Dict, List, Optional, Sequence, Union
 
 import torch
 import torch.distributed as dist
 import torch.nn as nn
 
-__all__ = ["DataParallel", "Bucket", "split_buckets"]
+__all__ = ["DataParallel", "Bucket", "split_buckets", "note_wrapper", "check_entry"]
+
+_wrappers: "weakref.WeakKeyDictionary[nn.Module, weakref.ref]" = weakref.WeakKeyDictionary()
+
+
+def note_wrapper(module: nn.Module, wrapper: nn.Module) -> None:
+    """Remember that ``wrapper`` reduces ``module``'s gradients, for ``check_entry``."""
+
+    _wrappers[module] = weakref.ref(wrapper)
+
+
+def check_entry(module: nn.Module, name: str) -> None:
+    """Refuse a differentiable ``module.name(...)`` that passes by the wrapper: its gradients would stay this rank's own.
+
+    Only a wrapper's ``forward`` prepares the reduction. Under ``no_sync()`` the call is what it seems.
+    """
+
+    ref = _wrappers.get(module)
+    wrapper = None if ref is None else ref()
+    if wrapper is None or not torch.is_grad_enabled():
+        return
+    if getattr(wrapper, "require_sync" if isinstance(wrapper, DataParallel) else "require_backward_grad_sync", True):
+        raise RuntimeError(
+            f"{type(module).__name__}.{name} was called past its {type(wrapper).__name__} wrapper, so its gradients would "
+            f"not be reduced; call wrapper(idx, method={name!r}, ...), or use torch.no_grad() or wrapper.no_sync()")
 
 
 def split_buckets(numels: Sequence[int], caps: Sequence[int]) -> List[List[int]]:
@@ -184,6 +209,7 @@ class DataParallel(nn.Module):
         self._hooks = [p.register_post_accumulate_grad_hook(self._on_grad) for p in params]
         self._armed = False
         self._callback_queued = False
+        note_wrapper(module, self)
 
     # ------------------------------------------------------------------ setup
     def _pick_transport(self, transport: str, backend: str) -> str:
@@ -219,6 +245,22 @@ class DataParallel(nn.Module):
             self._arm()
         return self.module(*args, **kwargs)
 
+    # Losses of the language models (``models/common.py:TokenLosses``), by way of forward.
+    def _method(self, name: str, idx, options):
+        if not hasattr(self.module, name):
+            raise AttributeError(f"{type(self.module).__name__} has no {name}")
+        return self(idx, method=name, **options)
+
+    def logits(self, idx):
+        return self._method("logits", idx, {})
+
+    def token_logprobs(self, idx, tokens=None, **options):
+        return self._method("token_logprobs", idx, {"tokens": tokens, **options})
+
+    def distillation_loss(self, idx, teacher_ids, teacher_logits, **options):
+        return self._method("distillation_loss", idx,
+                            {"teacher_ids": teacher_ids, "teacher_logits": teacher_logits, **options})
+
     @contextlib.contextmanager
     def no_sync(self):
         prev = self.require_sync
@@ -236,6 +278,8 @@ class DataParallel(nn.Module):
             self._reserving = on
 
     def _arm(self) -> None:
+        if self._armed and not self._callback_queued:
+            return  # several forward passes before one backward pass: nothing has changed since the first
         self._set_reserve(False)
         if self._fused is not None and self._fused_ready:
             # The previous synchronised backward was never gated: close its
