@@ -311,10 +311,12 @@ def token_logprobs_ref(logits, tokens, *, top_k: int = 0, temperature: float = 1
     """2-D logits, 1-D tokens; (logprobs, entropy, top_logprobs, top_ids) in fp32 (fp64 for fp64 logits)."""
 
     zf = logits if logits.dtype == torch.float64 else logits.float()
+    counted = torch.ones(len(zf), dtype=torch.bool, device=zf.device) if tokens is None else tokens != ignore_index
+    if not counted.all():  # rows left out have gradient zero, whatever they hold
+        zf = torch.where(counted[:, None], zf, 0.0)
     logp = torch.log_softmax(zf / temperature, dim=-1)
     masked = torch.isneginf(zf) & torch.isfinite(logp.detach().amax(-1, keepdim=True))
     entropy = -torch.where(masked, 0.0, logp.exp() * logp.masked_fill(masked, 0.0)).sum(-1)
-    counted = torch.ones_like(entropy, dtype=torch.bool) if tokens is None else tokens != ignore_index
     logprobs = top_logprobs = top_ids = None
     if tokens is not None:
         inside = (tokens >= 0) & (tokens < logits.shape[1])
@@ -422,22 +424,26 @@ def topk_distillation(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
         if other is not None and other.device != logits.device:
             raise ValueError(f"{name}: all tensors must be on {logits.device}")
     k = teacher_ids.shape[-1]
-    loss = topk_distillation_ref(z, teacher_ids.reshape(-1, k), teacher_logits.detach().reshape(-1, k).float(),
-                                 temperature=temperature, tail=tail)
+    ids = teacher_ids.reshape(-1, k)
+    if weight is not None:
+        weight = weight.detach().float().reshape(-1)
+        ids = torch.where((weight != 0)[:, None], ids, -1)
+    loss = topk_distillation_ref(z, ids, teacher_logits.detach().reshape(-1, k).float(), temperature=temperature,
+                                 tail=tail)
     if reduction == "none":
         return loss.view(lead)
-    if weight is None:
-        return loss.sum()
-    weight = weight.detach().float().reshape(-1)
-    return torch.where(weight == 0, 0.0, loss * weight).sum()
+    return loss.sum() if weight is None else torch.where(weight == 0, 0.0, loss * weight).sum()
 
 
 def topk_distillation_ref(logits, teacher_ids, teacher_logits, *, temperature: float = 1.0, tail: bool = False):
     """2-D logits and ``[rows, k]`` teachers; loss rows in fp32 (fp64 for fp64 logits)."""
 
     zf = logits if logits.dtype == torch.float64 else logits.float()
-    logp = torch.log_softmax(zf / temperature, dim=-1)
     valid = (teacher_ids >= 0) & (teacher_ids < logits.shape[1])
+    some = valid.any(-1)
+    if not some.all():  # rows without slots have gradient zero, whatever they hold
+        zf = torch.where(some[:, None], zf, 0.0)
+    logp = torch.log_softmax(zf / temperature, dim=-1)
     at = torch.where(valid, teacher_ids, 0)
     t = torch.where(valid, teacher_logits.to(zf.dtype), -math.inf)
     if tail:
@@ -453,9 +459,11 @@ def topk_distillation_ref(logits, teacher_ids, teacher_logits, *, temperature: f
     if tail:
         listed = torch.zeros_like(logp.detach()).scatter_add_(1, at, valid.to(logp.dtype)) > 0
         rest = (1.0 - q.sum(-1)).clamp_min(0.0)
-        log_rest = torch.logsumexp(logp.masked_fill(listed, -math.inf), -1)
+        off = logp.masked_fill(listed, -math.inf)
+        none = off.detach().amax(-1) == -math.inf  # no student mass off the list: an infinite constant
+        log_rest = torch.where(none, -math.inf, torch.logsumexp(off.masked_fill(none[:, None], 0.0), -1))
         loss = loss + torch.where(rest == 0, 0.0, rest * (rest.log() - log_rest).masked_fill(rest == 0, 0.0))
-    return torch.where(valid.any(-1), loss, 0.0)
+    return torch.where(some, loss, 0.0)
 
 
 def bias_grad(g: torch.Tensor) -> torch.Tensor:

@@ -282,6 +282,54 @@ def test_leading_shapes_and_empty_batches(device):
         assert kf.topk_distillation(empty, tok.new_zeros(*lead, 4), z.new_zeros(*lead, 4), reduction="sum") == 0
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("tail", [False, True])
+def test_gradients_of_rows_left_out(device, tail):
+    """Zeros, whatever the rows hold: an ignored token, no slots, weight zero (whose teacher may be anything too)."""
+
+    z = _logits(4, 300, torch.float32, "contiguous", device=device)
+    z[0], z[2] = math.nan, math.inf
+    z.requires_grad_()
+    tok = torch.tensor([IGNORE, 3, IGNORE, 4], device=device)
+    ids, t = _teacher(4, 300, 5, tail, ragged=False, device=device)
+    none = ids.masked_fill(torch.tensor([[True], [False], [True], [False]], device=device), -1)
+    weight = torch.tensor([0.0, 1.0, 0.0, 0.5], device=device)
+    bad = t.clone()
+    bad[0] = math.nan
+    bad[2] = math.inf
+    res = kf.token_logprobs(z, tok, ignore_index=IGNORE)
+    for total in (res.logprobs.sum() + res.entropy.sum(), kf.topk_distillation(z, none, bad, tail=tail).sum(),
+                  kf.topk_distillation(z, none, bad, tail=tail, reduction="sum"),
+                  kf.topk_distillation(z, ids, bad, tail=tail, weight=weight, reduction="sum")):
+        (dz,) = torch.autograd.grad(total, z)
+        assert total.isfinite() and dz.isfinite().all()
+        assert not dz[::2].any() and dz[1::2].any(1).all()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [50, 5000, 20000])
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_gradient_without_student_mass_off_the_list(device, dtype, vocab, reduction):
+    """With a tail and every token off the list masked, the loss is infinite and the rest adds nothing to the gradient,
+    which is (Q p - q) / T. Three numbers of at most 1, each accurate to 2^-18, and half a step of the logits' type."""
+
+    rows, k, temperature = 160, 6, 2.0
+    gen = torch.Generator().manual_seed(2)
+    ids = torch.stack([torch.randperm(vocab, generator=gen)[:k] for _ in range(8)]).repeat(rows // 8, 1)
+    t = torch.log_softmax(torch.randn(8, k + 1, generator=gen), -1)[:, :k].repeat(rows // 8, 1)
+    z = torch.full((rows, vocab), -math.inf).scatter_(1, ids, torch.randn(8, k, generator=gen).repeat(rows // 8, 1))
+    z = z.to(device, dtype).requires_grad_()
+    loss = kf.topk_distillation(z, ids.to(device), t.to(device), temperature=temperature, tail=True,
+                                reduction=reduction)
+    (dz,) = torch.autograd.grad(loss.sum(), z)
+    assert (loss == math.inf).all()
+    q = torch.zeros(rows, vocab, dtype=torch.float64).scatter_(1, ids, t.double().exp())
+    p = torch.softmax(z.detach().cpu().double() / temperature, 1)
+    want = (q.sum(1, keepdim=True) * p - q) / temperature
+    _close(dz, want, 2.0**-16 / temperature + want.abs() * _half_step(dtype) * 1.01, "dlogits")
+
+
 # ------------------------------------------------------- log probabilities
 
 
