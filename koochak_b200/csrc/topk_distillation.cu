@@ -94,6 +94,16 @@ __device__ __forceinline__ ListStats list_stats(float c, int K, const ListShared
   return r;
 }
 
+// The teacher's rest, against the student's mass off the list (`str` of `all`). One minus the sum of q is not zero where
+// the slots hold everything: token_logprobs' log probabilities are off by 2^-20 + |t| 2^-22, which is (1 + H / 4) 2^-20 of
+// the sum with H <= ln 128, and the exponentials and the sum add less than 1.2 2^-20. A rest below 2^-18 therefore counts
+// as none where the student's probability of it is none either (below 2^-126): its term would be infinite, or 1e32 where
+// the lowest value masks, from nothing but rounding.
+__device__ __forceinline__ float rest_of(const Acc& str, const Acc& all, const ListStats& list, float c) {
+  const float down = str.m == all.m ? 0.f : (str.m - all.m) * c;
+  return list.q_rest <= 0x1p-18f && log2f(str.s) + down - log2f(all.s) < -126.f ? 0.f : list.q_rest;
+}
+
 // From the statistics of the streamed elements (all of them, or with TAIL those off the list).
 template <bool TAIL>
 __device__ __forceinline__ KdStats row_stats(const Acc& str, const ListStats& list, float c) {
@@ -105,11 +115,12 @@ __device__ __forceinline__ KdStats row_stats(const Acc& str, const ListStats& li
   r.m = all.m;
   r.inv_s = 1.f / all.s;
   // Where the student has no mass off the list, a rest is an infinite constant: it has no gradient.
-  r.mass = TAIL && str.s != 0.f ? list.q_sum + list.q_rest : list.q_sum;
+  const float rest = TAIL ? rest_of(str, all, list, c) : 0.f;
+  r.mass = TAIL && str.s != 0.f ? list.q_sum + rest : list.q_sum;
   r.coef = r.mass * r.inv_s;
   if (TAIL) {
     const float down = str.m == all.m ? 0.f : str.m - all.m;
-    r.coef = str.s == 0.f ? 0.f : r.coef * ex2(down * c) - list.q_rest / str.s;
+    r.coef = str.s == 0.f ? 0.f : r.coef * ex2(down * c) - rest / str.s;
   }
   r.ms = str.m == -INFINITY ? 0.f : str.m;
   return r;
@@ -132,9 +143,10 @@ __device__ __forceinline__ float row_loss(const Acc& str, const ListStats& list,
     if (q != 0.f) loss += q * (lq - ((sh.z[i] - all.m) * inv_t - ln_s));
   }
   loss = warp_sum(loss);
-  if (TAIL && list.q_rest != 0.f) {
+  const float rest = TAIL ? rest_of(str, all, list, c) : 0.f;
+  if (rest != 0.f) {
     const float down = str.m == all.m ? 0.f : str.m - all.m;
-    loss += list.q_rest * (kLn2 * (log2f(list.q_rest) - log2f(str.s)) - down * inv_t + ln_s);
+    loss += rest * (kLn2 * (log2f(rest) - log2f(str.s)) - down * inv_t + ln_s);
   }
   return loss;
 }

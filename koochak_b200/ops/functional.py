@@ -391,9 +391,10 @@ def topk_distillation(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     * ``tail=True``: ``teacher_logits`` are log probabilities at this
       temperature (``token_logprobs(...).top_logprobs``), ``q`` their
       exponentials, and the teacher's remaining mass ``1 - sum q`` is compared
-      with the student's mass outside the listed tokens as one more slot
-      (where the student has none, the loss is infinite and that slot adds
-      nothing to the gradient).
+      with the student's mass outside the listed tokens as one more slot.
+      Where the student has none, the loss is infinite and that slot adds
+      nothing to the gradient, but a rest below 2^-18, which rounding alone
+      leaves of a teacher that lists everything, counts as none there.
 
     Rows without slots have loss and gradient zero. ``reduction="none"``
     returns fp32 losses ``[...]``; ``"sum"`` returns their sum weighted by
@@ -462,6 +463,8 @@ def topk_distillation_ref(logits, teacher_ids, teacher_logits, *, temperature: f
         off = logp.masked_fill(listed, -math.inf)
         none = off.detach().amax(-1) == -math.inf  # no student mass off the list: an infinite constant
         log_rest = torch.where(none, -math.inf, torch.logsumexp(off.masked_fill(none[:, None], 0.0), -1))
+        # What rounding leaves of a teacher that lists everything, where the student has no mass for it.
+        rest = torch.where((rest <= 2.0**-18) & (log_rest.detach() < -126 * math.log(2.0)), 0.0, rest)
         loss = loss + torch.where(rest == 0, 0.0, rest * (rest.log() - log_rest).masked_fill(rest == 0, 0.0))
     return torch.where(some, loss, 0.0)
 

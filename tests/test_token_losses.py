@@ -330,6 +330,38 @@ def test_gradient_without_student_mass_off_the_list(device, dtype, vocab, reduct
     _close(dz, want, 2.0**-16 / temperature + want.abs() * _half_step(dtype) * 1.01, "dlogits")
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("mask", [-math.inf, "lowest"])
+@pytest.mark.parametrize("vocab,left,k", [(40, 7, 7), (5000, 60, 64), (20000, 100, 128)])
+def test_teacher_that_lists_every_token_left(device, dtype, mask, vocab, left, k):
+    """Teacher and student under one mask that leaves no more tokens than the teacher has slots. What one minus the sum
+    of its probabilities is then is rounding: the loss is that of the tokens left, and so is the gradient. Tolerances as
+    in _check_distill, of log probabilities below 24 (logits of about 8 and down to -8); a rest of up to 2^-18 that is
+    found or not changes a finite log probability's factor, so that the loss may move by as much again."""
+
+    rows = 160
+    low = torch.finfo(dtype).min if mask == "lowest" else mask
+    masked = torch.ones(rows, vocab, dtype=torch.bool)
+    for i in range(rows):
+        masked[i, torch.randperm(vocab, generator=torch.Generator().manual_seed(i))[:left]] = False
+    teacher, student = (_logits(rows, vocab, dtype, "contiguous", seed=s, device=device)
+                        .masked_fill_(masked.to(device), low) for s in (1, 2))
+    got = kf.token_logprobs(teacher, top_k=k, temperature=1.5)
+    z = student.requires_grad_()
+    q = torch.softmax(teacher.cpu().double() / 1.5, 1)
+    logp = torch.log_softmax(z.detach().cpu().double() / 1.5, 1)
+    want = torch.where(q > 0, q * (q.clamp_min(1e-300).log() - logp.clamp_min(-1e300)), 0.0).sum(1)
+    dwant = (logp.exp() - q) / 1.5 / rows
+    for reduction in ("none", "sum"):
+        loss = kf.topk_distillation(z, got.top_ids, got.top_logprobs, temperature=1.5, tail=True, reduction=reduction)
+        (dz,) = torch.autograd.grad(loss.sum() / rows, z)
+        goal = want if reduction == "none" else want.sum()
+        _close(loss.detach(), goal, (24 + 16) * 2.0**-18 * (1 if reduction == "none" else rows), "loss")
+        tol = 2.0**-16 / rows + dwant.abs() * _half_step(dtype) * 1.01 + torch.finfo(dtype).tiny * _half_step(dtype) * 2
+        _close(dz, dwant, tol, "dlogits")
+
+
 # ------------------------------------------------------- log probabilities
 
 
