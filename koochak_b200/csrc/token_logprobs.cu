@@ -272,6 +272,81 @@ __device__ void select_top(const Row<T>& row, int u0, int u1, int ragged, float 
 
 // --------------------------------------------------- log probabilities
 
+// Statistics of a set of elements, told apart from those of the one thread that has more than half of the sum, if one
+// has (owner >= 0): `own` is its sum to all.m, `others` the rest's statistics. Only there can the set have an element
+// more likely than all others together.
+struct Apart {
+  Acc all, others;
+  float own = 0.f;
+  int owner = -1;
+};
+struct WarpStats {
+  Acc others;
+  float s = 0.f, a = 0.f;  // of the lane with more than half of the warp's sum
+  int lane = 0;
+};
+
+__device__ __forceinline__ WarpStats warp_apart(const Run<true>& run, float c) {
+  const float2 ss = split(run.s), aa = split(run.a);
+  const float off = run.plain ? fmaf(run.m, c, -run.r) : 0.f, f = ex2(-off);  // of every x
+  const float s = (ss.x + ss.y) * f, a = (aa.x + aa.y) * f - off * s;
+  WarpStats w;
+  w.others.m = run.m;
+  w.others.s = warp_sum(s);
+  const uint32_t most = __ballot_sync(0xffffffffu, 2.f * s > w.others.s);
+  if (most) {
+    w.lane = __ffs(most) - 1;
+    w.s = __shfl_sync(0xffffffffu, s, w.lane);
+    w.a = __shfl_sync(0xffffffffu, a, w.lane);
+  }
+  const bool apart = most && (int)(threadIdx.x & 31) == w.lane;
+  if (most) w.others.s = warp_sum(apart ? 0.f : s);
+  w.others.a = warp_sum(apart ? 0.f : a);
+  return w;
+}
+
+// Joins the parts that the first N lanes of a warp hold: `owner` of its part, and the part's lane.
+template <int N>
+__device__ __forceinline__ Apart join_apart(const Acc& all, const Acc& others, float own, int owner, float c, int& part) {
+  Apart r;
+  r.all = join_lanes<N, true>(all, c);
+  const bool mine = (int)(threadIdx.x & 31) < N;
+  const float mass = mine && owner >= 0 ? own * (all.m == r.all.m ? 1.f : ex2((all.m - r.all.m) * c)) : 0.f;
+  const uint32_t most = __ballot_sync(0xffffffffu, 2.f * mass > r.all.s);
+  if (most) {
+    part = __ffs(most) - 1;
+    r.own = __shfl_sync(0xffffffffu, mass, part);
+    r.owner = __shfl_sync(0xffffffffu, owner, part);
+    const bool apart = (int)(threadIdx.x & 31) == part;
+    Acc rest;
+    rest.m = all.m;
+    rest.s = apart ? others.s : all.s;
+    rest.a = apart ? others.a : all.a;
+    if (apart) rest.m = others.m;
+    r.others = join_lanes<N, true>(rest, c);
+  }
+  return r;
+}
+
+// The same for a block's warps; the first warp returns with it.
+template <int NT>
+__device__ __forceinline__ Apart block_apart(const Run<true>& run, float c, WarpStats* sm) {
+  const WarpStats mine = warp_apart(run, c);
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = mine;
+  __syncthreads();
+  Apart r;
+  if (threadIdx.x < 32) {
+    const WarpStats w = sm[threadIdx.x & (NT / 32 - 1)];
+    Acc all = w.others;
+    all.s += w.s;
+    all.a += w.a;
+    int warp = 0;
+    r = join_apart<NT / 32>(all, w.others, w.s, w.lane, c, warp);
+    if (r.owner >= 0) r.owner += 32 * warp;
+  }
+  return r;
+}
+
 // A block per row, or with SPLIT a cluster of blocks that share it: statistics
 // in one pass, then the alternatives. The blocks of a cluster select their own
 // alternatives, and the first block merges the sorted lists.
@@ -314,7 +389,11 @@ __global__ void __launch_bounds__(NT, 1280 / NT)
     mine = tid < ragged ? Elem<T>::load(row.z + row.ragged_index(tid)) : -INFINITY;
     run.add_one(mine, c);
   }
-  __shared__ Acc join_sm[NT / 32], result, own;
+  __shared__ WarpStats join_sm[NT / 32];
+  __shared__ Acc result;
+  __shared__ Apart mine_apart;
+  __shared__ float star_logp;
+  __shared__ int star;
   __shared__ std::conditional_t<TOPK, SelectShared<NT>, int> sh;
   stream_units<T, NT, TOPK>(FromMemory{row.unit_ptr()}, u0, u1, c, run, NoMarks{}, [&](int batch, float mx) {
     if constexpr (TOPK) {
@@ -323,24 +402,12 @@ __global__ void __launch_bounds__(NT, 1280 / NT)
       kept = batch < sh.kGroups ? mx : max_nan(kept, mx);
     }
   });
-  // The thread that saw the given token stays out of the sum: see below.
-  const bool inside = tokens && token >= 0 && token < V;
   const int per = (row.units + parts - 1) / parts;
-  int owner = -1, owner_part = 0;
-  if (inside) {
-    const int at = (int)token - row.head;
-    owner = at < 0 ? (int)token : (int)token - row.units * Elem<T>::kUnit;  // a ragged element's
-    if (at >= 0 && at < row.units * Elem<T>::kUnit) {
-      owner_part = at / Elem<T>::kUnit / per;
-      owner = (at / Elem<T>::kUnit - owner_part * per) % NT;
-    }
-    if (tid == owner && part == owner_part) own = run.take(c);
-  }
-  Acc all = block_join<NT, true>(run, c, join_sm), theirs;
-  if (!SPLIT && inside) theirs = own;
+  Apart got = block_apart<NT>(run, c, join_sm);
+  int owner_part = 0;
   if constexpr (SPLIT) {
     __shared__ unsigned long long sorted[TOPK ? kMaxList : 1];
-    if (tid == 0) result = all;
+    if (tid == 0) mine_apart = got;
     if constexpr (TOPK) {
       for (int i = tid; i < k; i += NT) sorted[i] = 0;  // below every key
       select_top<T, NT>(row, u0, u1, ragged, mine, k, 64, sh,
@@ -349,10 +416,9 @@ __global__ void __launch_bounds__(NT, 1280 / NT)
     cg::this_cluster().sync();
     if (part == 0) {
       if (tid < 32) {
-        all = *cg::this_cluster().map_shared_rank(&result, (tid & 7) < parts ? tid & 7 : 0);
-        if ((tid & 7) >= parts) all = Acc();
-        all = join_lanes<8, true>(all, c);
-        if (inside) theirs = *cg::this_cluster().map_shared_rank(&own, owner_part);
+        Apart theirs;
+        if ((tid & 31) < parts) theirs = *cg::this_cluster().map_shared_rank(&mine_apart, tid & 7);
+        got = join_apart<8>(theirs.all, theirs.others, theirs.own, theirs.owner, c, owner_part);
       }
       if constexpr (TOPK) {
         for (int i = tid; i < parts * k; i += NT) sh.merged[i] = *cg::this_cluster().map_shared_rank(&sorted[i % k], i / k);
@@ -363,40 +429,58 @@ __global__ void __launch_bounds__(NT, 1280 / NT)
   }
   // Log probabilities are taken in units of z / T, not of c z: (lowest - m) c would overflow.
   if (tid < 32) {
-    const Acc others = all;
-    if (inside) all.join<true>(theirs.m, theirs.s, theirs.a, c);
+    const Acc all = got.all;
     const float log2s = log2f(all.s);
     float logp = NAN, h = kLn2 * (log2s - all.a / all.s);
-    if (inside) {
-      const float z = Elem<T>::load(row.z + token), x = (z - all.m) * c, e = ex2(x);
-      logp = (z - all.m) * inv_t - kLn2 * log2s;
+    if (tokens && token >= 0 && token < V)
+      logp = (Elem<T>::load(row.z + token) - all.m) * inv_t - kLn2 * log2s;
+    int best = -1;
+    float best_logp = 0.f;
+    if (got.owner >= 0) {
+      // An element more likely than all others together: its ln p and the entropy are small differences of large numbers,
+      // unless they are taken from the rest of the sum, -ln p = ln(1 + rest / e) and
+      // H = -ln p - sum over the rest of p_j ln 2 (x_j - x). What its thread has added to the sum is summed anew.
+      const int first = owner_part * per + got.owner, last = min(row.units, (owner_part + 1) * per);
+      const int mine_u = first + tid * NT;  // the lane's only unit where a thread has at most 32
+      uint4 q = make_uint4(0, 0, 0, 0);
+      if (mine_u < last) q = load_unit(row.unit_ptr() + mine_u);
+      const auto each = [&](const auto& take) {
+        for (int u = mine_u; u < last; u += 32 * NT) {
+          float v[Elem<T>::kUnit];
+          Elem<T>::unpack(u == mine_u ? q : load_unit(row.unit_ptr() + u), v);
+#pragma unroll
+          for (int j = 0; j < Elem<T>::kUnit; ++j) take(v[j], row.head + u * Elem<T>::kUnit + j);
+        }
+        if (tid == 0 && owner_part == 0 && got.owner < row.ragged) {
+          const int i = row.ragged_index(got.owner);
+          take(Elem<T>::load(row.z + i), i);
+        }
+      };
+      float z = -INFINITY;
+      int at = 0x7FFFFFFF;
+      each([&](float v, int i) {
+        at = v > z || (v == z && i < at) ? i : at;
+        z = fmaxf(z, v);
+      });
+      const float most = warp_max_nan(z), x = (most - all.m) * c, e = ex2(x);
+      at = __reduce_min_sync(0xffffffffu, z == most ? at : 0x7FFFFFFF);
       if (2.f * e > all.s) {
-        // A token more likely than all others together: ln p and the entropy are small differences of large numbers,
-        // unless they are taken from the rest of the sum, -ln p = ln(1 + rest / e) and
-        // H = -ln p - sum over the rest of p_j ln 2 (x_j - x). What the token's thread has added to it is summed anew.
         Acc rest;
         rest.m = all.m;
-        const int first = owner_part * per + owner, last = min(row.units, (owner_part + 1) * per);
-        const auto add = [&](float v) {
+        each([&](float v, int i) {
+          if (i == at) return;
           const float y = (v - all.m) * c, f = ex2(y);
           rest.s += f;
           rest.a = fmaf(f, fmaxf(y, -256.f), rest.a);
-        };
-        for (int u = first + tid * NT; u < last; u += 32 * NT) {
-          float v[Elem<T>::kUnit];
-          Elem<T>::unpack(load_unit(row.unit_ptr() + u), v);
-#pragma unroll
-          for (int j = 0; j < Elem<T>::kUnit; ++j)
-            if (row.head + u * Elem<T>::kUnit + j != (int)token) add(v[j]);
-        }
-        if (tid == 0 && owner_part == 0 && owner < row.ragged && row.ragged_index(owner) != (int)token)
-          add(Elem<T>::load(row.z + row.ragged_index(owner)));
+        });
         rest.s = warp_sum(rest.s);
         rest.a = warp_sum(rest.a);
-        rest.join<true>(others.m, others.s, others.a, c);
+        rest.join<true>(got.others.m, got.others.s, got.others.a, c);
         const float l = log1pf(rest.s / e);
-        logp = -l;
+        best = at;
+        best_logp = -l;
         h = l - kLn2 * (rest.a - x * rest.s) / (rest.s + e);
+        if (tokens && token == at) logp = -l;
       }
     }
     if (tid == 0) {
@@ -409,13 +493,17 @@ __global__ void __launch_bounds__(NT, 1280 / NT)
       if (TOPK) {
         result.m = all.m;
         result.s = kLn2 * log2s;
+        star = best;
+        star_logp = best_logp;
       }
     }
   }
   if constexpr (TOPK) {
     auto emit = [&](int place, unsigned long long key) {
-      top_ids[row_i * k + place] = (int64_t)(uint32_t)~(uint32_t)key;
-      top_logprobs[row_i * k + place] = (value_of((uint32_t)(key >> 32)) - result.m) * inv_t - result.s;
+      const int id = (int)~(uint32_t)key;
+      top_ids[row_i * k + place] = id;
+      top_logprobs[row_i * k + place] =
+          id == star ? star_logp : (value_of((uint32_t)(key >> 32)) - result.m) * inv_t - result.s;
     };
     if constexpr (SPLIT) {
       __syncthreads();

@@ -272,17 +272,6 @@ struct Run {
     raise(z, c);
     add_any<false>(z, c);
   }
-  // The lane's own statistics to the reference's m; the lane is left without any.
-  __device__ __forceinline__ Acc take(float c) {
-    Acc t;
-    const float2 ss = split(s), aa = split(a);
-    const float off = plain ? fmaf(m, c, -r) : 0.f, f = ex2(-off);  // of every x
-    t.m = m;
-    t.s = (ss.x + ss.y) * f;
-    t.a = ENT ? (aa.x + aa.y) * f - off * t.s : 0.f;
-    s = a = pair(0.f, 0.f);
-    return t;
-  }
   // The warp's statistics to its reference's m, in every lane.
   __device__ __forceinline__ Acc total(float c) const {
     Acc t;

@@ -421,6 +421,58 @@ def test_likely_tokens_keep_their_digits(dtype, rows, vocab, layout):
     _close(res.entropy.cpu()[likely], ent[likely], ent[likely] * 2.0**-16, "entropy")
 
 
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,layout", [(12, 1003, "offset"), (12, 50257, "padded"), (3, 50257, "contiguous"),
+                                               (500, 4099, "contiguous"), (400, 17, "offset"), (700, 32001, "contiguous")])
+@pytest.mark.parametrize("given", [False, True])
+def test_likely_alternatives_and_entropies_keep_their_digits(dtype, rows, vocab, layout, given):
+    """The same for the most likely alternative and the entropy where another token is given or none; tolerances as
+    above. Nothing has a positive log probability or a negative entropy."""
+
+    z = _logits(rows, vocab, dtype, layout, sigma=1.0)
+    likely = _tokens(rows, vocab, ignored=False)
+    likely[0], likely[1], likely[2] = 0, vocab - 1, min(8, vocab - 1)
+    z.scatter_(1, likely[:, None], (torch.arange(rows, device=DEV) % 12 * 2.0 + 12.0)[:, None].to(dtype))
+    tok = (likely + 1) % vocab if given else None
+    d = z.double() - z.double().gather(1, likely[:, None])
+    e = d.exp().scatter_(1, likely[:, None], 0.0)
+    logp = -torch.log1p(e.sum(1))
+    ent = -logp - (e * d).sum(1) / (1 + e.sum(1))
+    sure = logp > math.log(0.5) + 1e-3
+    assert sure.any()
+    for top_k in (0, 1, 7):
+        res = kf.token_logprobs(z, tok, top_k=top_k)
+        _close(res.entropy[sure], ent[sure], (ent[sure] * 2.0**-16).cpu(), "entropy")
+        assert (res.entropy >= 0).all() and (not given or (res.logprobs <= 0).all())
+        if given:
+            want = logp + d.gather(1, tok[:, None])[:, 0]
+            _close(res.logprobs, want, _logprob_tol(want.cpu()), "logprobs")
+        if top_k:
+            assert torch.equal(res.top_ids[sure, 0], likely[sure]) and (res.top_logprobs <= 0).all()
+            _close(res.top_logprobs[sure, 0], logp[sure], (logp[sure].abs() * 2.0**-17).cpu(), "top_logprobs")
+            same = kf.token_logprobs(z, res.top_ids[:, 0].contiguous())
+            # one token's log probability, in either place: within both tolerances of the exact value
+            first = res.top_logprobs[:, 0]
+            _close(same.logprobs, first, torch.where(first > -0.69, first.abs() * 2.0**-16, 2 * _logprob_tol(first)),
+                   "places")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [2, 33, 5000, 50257])
+def test_two_tokens_with_all_of_the_probability(dtype, vocab):
+    """Equal logits side by side (in one thread's share, most often) and apart: neither has more than half."""
+
+    for first, second in ((0, 1), (vocab // 2, vocab // 2 + 1 if vocab > 2 else 0), (0, vocab - 1)):
+        z = torch.full((150, vocab), -math.inf, device=DEV, dtype=dtype)
+        z[:, first] = z[:, second] = torch.linspace(-30, 30, 150, device=DEV).to(dtype)
+        res = kf.token_logprobs(z, torch.full((150,), second, device=DEV), top_k=2, temperature=0.7)
+        for got in (-res.logprobs, res.entropy, -res.top_logprobs[:, 0], -res.top_logprobs[:, 1]):
+            _close(got, torch.full((150,), math.log(2.0)), 2.0**-20, "ln 2")
+        assert (res.top_ids.sort(1).values == torch.tensor(sorted((first, second)), device=DEV)).all()
+
+
 def _hard_rows(vocab, dtype, device):
     """Rows where selection and sums can go wrong: ties, masks, order in memory, extremes."""
 
