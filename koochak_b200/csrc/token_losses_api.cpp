@@ -78,11 +78,10 @@ OptTensor row_gradient(const at::Tensor& g) {
   return f.reshape({-1}).contiguous();
 }
 
-// The backward passes are kernels without a derivative of their own: differentiating their result raises.
-at::Tensor once_differentiable(const at::Tensor& dz, const variable_list& grads, bool recorded) {
-  bool follows = false;
-  for (const at::Tensor& g : grads) follows |= g.defined() && g.requires_grad();
-  if (!recorded || !follows) return dz;
+// The backward passes are kernels without a derivative of their own: differentiating their result raises, with respect to
+// the upstream gradient or to the logits, which it always depends on.
+at::Tensor once_differentiable(const at::Tensor& dz, bool recorded) {
+  if (!recorded) return dz;
   at::AutoGradMode on(true);
   auto err = std::make_shared<torch::autograd::DelayedError>("this backward pass cannot be differentiated", 1);
   return (*err)(variable_list{dz.detach().requires_grad_()})[0];
@@ -154,7 +153,7 @@ struct LogprobsFn : torch::autograd::Function<LogprobsFn> {
                             row_gradient(grads[0]), dz, z.size(1), ctx->saved_data["temperature"].toDouble(),
                             ctx->saved_data["ignore_index"].toInt());
     const at::Tensor shaped = logits.dim() == 2 ? dz : dz.view(logits.sizes());
-    return {once_differentiable(shaped, grads, recorded), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    return {once_differentiable(shaped, recorded), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 
@@ -248,7 +247,7 @@ struct DistillationFn : torch::autograd::Function<DistillationFn> {
                                summed ? g : OptTensor(), dz, z.size(1), ctx->saved_data["temperature"].toDouble(),
                                ctx->saved_data["tail"].toBool(), ready);
     const at::Tensor shaped = logits.dim() == 2 ? dz : dz.view(logits.sizes());
-    return {once_differentiable(shaped, grads, recorded), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    return {once_differentiable(shaped, recorded), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 

@@ -1132,6 +1132,21 @@ def test_second_derivatives_are_refused():
             g.sum().backward()
 
 
+@gpu
+def test_second_derivatives_with_a_constant_upstream_gradient_are_refused():
+    """A penalty on the gradient of a plain sum: beside other terms it would be left out without a word."""
+
+    z = _logits(3, 64, torch.float32, "contiguous").requires_grad_()
+    ids, t = _teacher(3, 64, 4, False, ragged=False)
+    for loss in (kf.token_logprobs(z, _tokens(3, 64, ignored=False)).logprobs.sum(), kf.topk_distillation(z, ids, t).sum(),
+                 kf.topk_distillation(z, ids, t, reduction="sum")):
+        (g,) = torch.autograd.grad(loss, z, create_graph=True)
+        (once,) = torch.autograd.grad(z.square().sum() + (2 * z).sum(), z)  # unrelated terms go on working
+        assert g.requires_grad and once.isfinite().all()
+        with pytest.raises(RuntimeError, match="differentiate"):
+            (z.sum() + g.square().sum()).backward()
+
+
 def _forward_mode(token_logprobs, topk_distillation, device):
     import torch.autograd.forward_ad as fwad
 
