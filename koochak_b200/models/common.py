@@ -173,11 +173,12 @@ class HeadLogits(torch.autograd.Function):
         x2 = x.reshape(M, C)
         h, mean, rstd = kf.norm_forward(x2, norm_w, norm_b, eps, rms=rms, out_dtype=cdt)
         vpad = (V + 63) // 64 * 64
-        logits = torch.empty((M, vpad), device=x.device, dtype=cdt)
-        kf.gemm(h, head_w16, out=logits[:, :V])
+        # A tensor of its own, not a view of a padded one: callers may mask it in place.
+        logits = torch.empty_strided((B, S, V), (S * vpad, vpad, 1), device=x.device, dtype=cdt)
+        kf.gemm(h, head_w16, out=logits.view(M, V))
         ctx.save_for_backward(x2, h, mean, rstd, norm_w, head_w16)
         ctx.meta = (B, S, C, V, rms)
-        return logits.view(B, S, vpad)[..., :V]
+        return logits
 
     @staticmethod
     @torch.autograd.function.once_differentiable

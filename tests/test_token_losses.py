@@ -1253,3 +1253,30 @@ def test_models_teacher_and_student_native(which, dtype):
     for n in g_r:
         err = ((g_n[n] - g_r[n]).abs().max() / (g_r[n].abs().max() + 1e-6)).item()
         assert err < 0.08, (n, err)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_models_logits_masked_in_place(which, device):
+    """Tokens that may not be produced are masked in the logits themselves, and take no gradient."""
+
+    model = _small_models(device)[which][1]
+    idx = torch.randint(0, 1000, (2, 64), device=device)
+    tok = torch.randint(100, 1000, (2, 64), device=device)
+
+    def step(native):
+        model.zero_grad(set_to_none=True)
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=native):
+            z = model.logits(idx)
+            z[..., :100] = -math.inf
+            z[0, :, 700:] += 1.0
+            res = kf.token_logprobs(z, tok, top_k=5)
+        assert (res.top_ids >= 100).all()
+        (-res.logprobs.mean()).backward()
+        return res.logprobs.detach(), {n: q.grad.clone() for n, q in model.named_parameters()}
+
+    lp, g = step(device == "cuda")
+    lp_r, g_r = step(False)
+    assert (lp - lp_r).abs().max() < 2e-2
+    for n in g_r:  # as in the test above
+        assert ((g[n] - g_r[n]).abs().max() / (g_r[n].abs().max() + 1e-6)).item() < 0.08, n
