@@ -186,7 +186,8 @@ class HeadLogits(torch.autograd.Function):
         x2, h, mean, rstd, norm_w, head_w16 = ctx.saved_tensors
         B, S, C, V, rms = ctx.meta
         dlog = dlogits.to(h.dtype).reshape(B * S, V)
-        if dlog.stride(1) != 1 or dlog.stride(0) % 8 or dlog.data_ptr() % 16:  # the GEMM's operands: 16-byte aligned rows
+        # The GEMM's operands: rows of their own (a gradient may be one row, expanded) at 16-byte boundaries.
+        if dlog.stride(1) != 1 or dlog.stride(0) < V or dlog.stride(0) % 8 or dlog.data_ptr() % 16:
             padded = torch.empty((B * S, (V + 63) // 64 * 64), device=h.device, dtype=h.dtype)[:, :V]
             dlog = padded.copy_(dlog)
         dh = kf.gemm(dlog, head_w16, b_mn_major=True)

@@ -1280,3 +1280,28 @@ def test_models_logits_masked_in_place(which, device):
     assert (lp - lp_r).abs().max() < 2e-2
     for n in g_r:  # as in the test above
         assert ((g[n] - g_r[n]).abs().max() / (g_r[n].abs().max() + 1e-6)).item() < 0.08, n
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_models_logits_with_gradients_of_any_strides(which, device):
+    """Upstream gradients that are expanded rows, one number, transposed, or views at odd places."""
+
+    model = _small_models(device)[which][1]
+    idx = torch.randint(0, 1000, (2, 64), device=device)
+    V = model.config.vocab_size
+    rows = torch.randn(1, 1, V, device=device)
+    many = torch.randn(64, 2, V, device=device)
+    odd = torch.randn(2, 64, V + 9, device=device)
+    for g in (rows.expand(2, 64, V), rows[..., :1].expand(2, 64, V), many.transpose(0, 1), odd[..., 3:V + 3],
+              many[:1, :1].transpose(0, 1).expand(2, 64, V)):
+        got = []
+        for native in (device == "cuda", False):
+            with torch.autocast("cuda", dtype=torch.bfloat16, enabled=native):
+                z = model.logits(idx)
+            up = g.to(z.dtype) if g.stride(-1) else g[..., :1].to(z.dtype).expand(2, 64, V)
+            if g.stride(1) == 0:
+                up = up[:1, :1].expand(2, 64, V)  # a cast of an expanded tensor is expanded no more
+            got.append(torch.autograd.grad(z, list(model.parameters()), up))
+        for a, b in zip(*got):  # as in the tests above
+            assert ((a - b).abs().max() / (b.abs().max() + 1e-6)).item() < 0.08
