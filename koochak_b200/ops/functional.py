@@ -282,10 +282,10 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     by their index, and ``top_logprobs`` their log probabilities. All are fp32
     but the ids. The results of a row with ``tokens == ignore_index`` are
     zeros and ids of -1; a token outside the vocabulary has a NaN log
-    probability. Logits of -inf are never produced (they add nothing to the
-    entropy); a row of -inf only, or with a NaN or +inf, gives NaN. NaN logits
-    rank above all others. On CUDA, logits with a forward-mode tangent are
-    refused.
+    probability, and a NaN gradient where the upstream one is not zero. Logits
+    of -inf are never produced (they add nothing to the entropy); a row of -inf
+    only, or with a NaN or +inf, gives NaN. NaN logits rank above all others.
+    On CUDA, logits with a forward-mode tangent are refused.
     """
 
     if use_native(logits):
@@ -321,7 +321,9 @@ def token_logprobs_ref(logits, tokens, *, top_k: int = 0, temperature: float = 1
     if tokens is not None:
         inside = (tokens >= 0) & (tokens < logits.shape[1])
         got = logp.gather(1, torch.where(inside, tokens, 0)[:, None])[:, 0]
-        logprobs = torch.where(counted, torch.where(inside, got, math.nan), 0.0)
+        if got.requires_grad:  # the gradient of a NaN is one, if any of it is asked for
+            got.register_hook(lambda g: g if g is None else torch.where(inside | (g == 0), g, math.nan))
+        logprobs = torch.where(counted, got + torch.where(inside, 0.0, math.nan), 0.0)
     if top_k:
         ids = zf.detach().sort(dim=-1, descending=True, stable=True).indices[:, :top_k]
         top_logprobs = torch.where(counted[:, None], logp.detach().gather(1, ids), 0.0)

@@ -541,6 +541,19 @@ def test_rows_left_out_are_not_read():
     assert dz[3].isfinite().all() and dz[3].any() and not dz[:3].any()
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_gradients_of_tokens_outside_the_vocabulary(device):
+    z = _logits(5, 99, torch.float32, "contiguous", device=device).requires_grad_()
+    tok = torch.tensor([99, -3, 7, IGNORE, 1 << 40], device=device)
+    res = kf.token_logprobs(z, tok)
+    assert res.logprobs.isnan().tolist() == [True, True, False, False, True]
+    up = torch.tensor([1.0, 0.0, 1.0, 1.0, -2.0], device=device)
+    (dz,) = torch.autograd.grad(res.logprobs, z, up, retain_graph=True)
+    assert dz[0].isnan().all() and not dz[1].any() and dz[2].isfinite().all() and not dz[3].any() and dz[4].isnan().all()
+    (dz,) = torch.autograd.grad(res.entropy.sum(), z)
+    assert dz.isfinite().all() and dz[[0, 1, 2, 4]].any(1).all()
+
+
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_in_place_gradients(dtype):
