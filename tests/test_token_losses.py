@@ -757,6 +757,151 @@ def test_rows_left_out_in_any_order(tail, left_out, how):
     assert torch.equal(back, dz)
 
 
+def _kernels(f):
+    """Names of the CUDA kernels that a call launches (none where the profiler sees none)."""
+
+    f()
+    torch.cuda.synchronize()
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        f()
+        torch.cuda.synchronize()
+    return {e.key for e in prof.key_averages()}
+
+
+@gpu
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype,vocab,ld", [(torch.bfloat16, 17001, 17001), (torch.float16, 33001, 33024),
+                                            (torch.float32, 12345, 12345), (torch.bfloat16, 16392, 16397)])
+def test_staged_rows_left_out_in_any_order(tail, dtype, vocab, ld):
+    """As above, for rows that are staged in shared memory: two blocks per SM take several rows each, and any of a block's
+    rows may be left out, by weight, by slots, or by either in turn."""
+
+    rows = 1500
+    buf = torch.randn(rows, ld, device=DEV, generator=torch.Generator(DEV).manual_seed(3)).mul_(2).to(dtype)
+    z = buf[:, :vocab]
+    ids, t = (x.repeat(rows // 10, 1) for x in _teacher(10, vocab, 7, tail, ragged=False))
+    base = torch.rand(rows, device=DEV, generator=torch.Generator(DEV).manual_seed(4)) + 0.5
+    want_loss, stats = kf.topk_distillation_forward(z, ids, t, tail=tail)
+    want = kf.topk_distillation_backward(z, ids, t, stats, row_scale=base, tail=tail)
+    names = _kernels(lambda: kf.topk_distillation_grad(z, ids, t, weight=base, tail=tail))
+    assert not names or any("distill_grad_kernel" in n for n in names), names
+    i = torch.arange(rows, device=DEV)
+    for out in (i % 2 == 0, i % 2 == 1, i < 300, i > 40, i % 3 != 0, (i // 200) % 2 == 0, (i // 296) % 2 == 1,
+                (i // 296) % 3 != 1, torch.rand(rows, device=DEV) < 0.5, i >= 0, i < 0):
+        by_slots = torch.rand(rows, device=DEV) < 0.5
+        weight, listed = base.clone(), ids.clone()
+        weight[out & ~by_slots] = 0
+        listed[out & by_slots] = -1
+        x = z.clone()
+        x[out] = math.nan  # not read
+        loss, kept, dz = kf.topk_distillation_grad(x, listed, t, weight=weight, tail=tail)
+        assert not loss[out].any() and not dz[out].any() and not kept[out].any() and (kept[~out, 7] == 1).all()
+        # Loss: both kernels within (16 + log V) 2^-20 of the exact value. Gradient: 2^-16 each (see _check_distill), and
+        # half a step of the logits' type each, relative.
+        _close(loss[~out], (base * want_loss)[~out], 1.5 * (16 + math.log(vocab)) * 2.0**-19, "loss")
+        _close(dz[~out], want[~out], 1.5 * 2.0**-15 + 2 * _half_step(dtype) * want[~out].double().abs().cpu(), "dlogits")
+
+
+def _relative_error_of_p(z, temperature):
+    """Bound on the relative error of a probability 2^x / S, x = (z - max) / T / ln 2, per element.
+
+    2^x is off by 2^-22, and by ln 2 |x| (2^-24 three times: the difference, 1 / T, the product). S adds the same of
+    its terms, and rounding: a thread (128 or more per row) adds two sums of V / 256 terms, which grow, so the
+    additions cost half of that many 2^-24, and some 16 more follow. log2 S is rounded at its own size."""
+
+    v = z.double().nan_to_num(neginf=-1e4) / temperature
+    x = (v - v.amax(1, keepdim=True)) / math.log(2.0)
+    log2s = torch.logsumexp(v - v.amax(1, keepdim=True), 1, keepdim=True) / math.log(2.0)
+    return 2.0**-21 + (3 * x.abs() + 3 * log2s + 16 + z.shape[1] / 512) * 2.0**-24
+
+
+def _output_tol(want, dtype):
+    """Half a step of a normal or subnormal result."""
+
+    return want.abs() * _half_step(dtype) * (1 + 2.0**-10) + torch.finfo(dtype).tiny * _half_step(dtype)
+
+
+SMALL_P = [(3, 129, "offset"), (5, 32000, "padded"), (4, 50257, "contiguous"), (300, 4099, "contiguous"),
+           (400, 9001, "offset"), (700, 20011, "contiguous"), (160, 50257, "padded"), (2, 131072, "padded")]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,layout", SMALL_P)
+@pytest.mark.parametrize("which", ["logprobs", "entropy", "both"])
+def test_every_element_of_logprob_gradients(dtype, rows, vocab, layout, which):
+    """Each element to its own size: most are products with a probability of 1e-6, which a tolerance of the row's largest
+    would let pass as zeros. Three factors make up dz = (g hot - p (g + gh (ln p + H))) / T."""
+
+    temperature = 1.25
+    z = _logits(rows, vocab, dtype, layout).requires_grad_()
+    tok = _tokens(rows, vocab)
+    gen = torch.Generator(DEV).manual_seed(8)
+    g = torch.randn(rows, device=DEV, generator=gen) * (which != "entropy")
+    gh = torch.randn(rows, device=DEV, generator=gen) * (which != "logprobs")
+    res = kf.token_logprobs(z, tok, temperature=temperature)
+    (dz,) = torch.autograd.grad((res.logprobs, res.entropy), z, (g, gh))
+    step = max(1, 2**24 // vocab)
+    for i in range(0, rows, step):
+        part = slice(i, i + step)
+        zp = z.detach()[part].double()
+        logp = torch.log_softmax(zp / temperature, 1)
+        p, counted = logp.exp(), (tok[part] != IGNORE)[:, None]
+        h = -(p * logp).sum(1, keepdim=True)
+        a, b = g[part].double()[:, None], gh[part].double()[:, None]
+        hot = torch.zeros_like(p).scatter_(1, tok[part].clamp_min(0)[:, None], 1.0)
+        want = torch.where(counted, (a * (hot - p) - b * p * (logp + h)) / temperature, 0.0)
+        rel = _relative_error_of_p(zp, temperature)
+        # p's own error in the product, that of ln p (the same) and of H (as at the top of this file) beside it
+        inner = rel + (h + math.log(vocab)) * 2.0**-20 + 2.0**-19 + logp.abs() * 2.0**-22
+        tol = p * (rel * (a.abs() + b.abs() * (logp.abs() + h)) + inner * b.abs() + 2.0**-22 * (a.abs() + b.abs() * h))
+        tol = (tol + hot * a.abs() * 2.0**-22 + 2.0**-124 * (a.abs() + b.abs() * 100)) / temperature
+        _close(dz[part], want, (tol + _output_tol(want, dtype)).cpu(), f"rows {i}")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,layout", SMALL_P)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("how", ["none", "sum", "scaled"])
+def test_every_element_of_distillation_gradients(dtype, rows, vocab, layout, tail, how):
+    """The same for dz = g / T ((Q + r) p - q - [off the list] r p / p_r): each of the three terms is accurate to its
+    probability's relative error, and the teacher's q and rest r to 2^-20 (of one, for the rest)."""
+
+    temperature = 1.0 if tail else 2.0
+    z = _logits(rows, vocab, dtype, layout).requires_grad_()
+    ids, t = _teacher(rows, vocab, 12, tail)
+    weight = torch.rand(rows, device=DEV, generator=torch.Generator(DEV).manual_seed(8)) + 0.5
+    if how == "none":
+        loss = kf.topk_distillation(z, ids, t, temperature=temperature, tail=tail)
+        (dz,) = torch.autograd.grad(loss, z, weight)
+    else:
+        loss = kf.topk_distillation(z, ids, t, temperature=temperature, tail=tail, weight=weight, reduction="sum")
+        factor = 1.0 if how == "sum" else 0.375
+        (dz,) = torch.autograd.grad(loss, z, torch.full((), factor, device=DEV))
+        weight = weight * factor
+    step = max(1, 2**24 // vocab)
+    for i in range(0, rows, step):
+        part = slice(i, i + step)
+        zp = z.detach()[part].double()
+        p = torch.softmax(zp / temperature, 1)
+        valid = (ids[part] >= 0) & (ids[part] < vocab)
+        tp = t[part].double().masked_fill(~valid, -math.inf)
+        q = tp.exp() if tail else torch.softmax(tp / temperature, 1).nan_to_num(0.0)
+        at = torch.where(valid, ids[part], 0)
+        listed = torch.zeros_like(p).scatter_add_(1, at, q)
+        off = torch.zeros_like(p).scatter_add_(1, at, valid.double()) == 0
+        total = q.sum(1, keepdim=True)
+        rest = (1 - total).clamp_min(0.0) if tail else torch.zeros_like(total)
+        share = torch.where(off, p, 0.0)
+        share = share / share.sum(1, keepdim=True) if tail else torch.zeros_like(p)
+        w = torch.where(valid.any(1), weight[part], 0.0).double()[:, None] / temperature
+        want = w * ((total + rest) * p - listed - rest * share)
+        rel = _relative_error_of_p(zp, temperature) + 2.0**-22
+        tol = rel * ((total + rest) * p + 2 * rest * share) + 2.0**-20 * (p + share * bool(tail) + 2 * listed)
+        _close(dz[part], want, (w * (tol + 2.0**-124) + _output_tol(want, dtype)).cpu(), f"rows {i}")
+
+
 @gpu
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("rows", [148, 200, 296, 600])
@@ -1318,3 +1463,62 @@ def test_models_logits_with_gradients_of_any_strides(which, device):
             got.append(torch.autograd.grad(z, list(model.parameters()), up))
         for a, b in zip(*got):  # as in the tests above
             assert ((a - b).abs().max() / (b.abs().max() + 1e-6)).item() < 0.08
+
+
+@gpu
+@pytest.mark.parametrize("which", [0, 1])
+def test_distillation_through_a_captured_training_step(which):
+    """The training loop's captured step: a teacher's alternatives, the student's loss and a policy term, scaled as a loop
+    with several micro-steps does. Each replay against an eager step on the same batch and weights, as in the graph
+    mode's own test."""
+
+    from koochak_b200.runtime.graphed_step import GraphedStep
+
+    teacher, student = _small_models(DEV)[which]
+    gen = torch.Generator().manual_seed(2)
+    named = list(student.named_parameters())
+    step = GraphedStep(student, warmup=1)
+
+    def batch():
+        idx = torch.randint(0, 1000, (4, 65), generator=gen).to(DEV)
+        with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+            got = teacher.token_logprobs(idx[:, :-1].contiguous(), top_k=16)
+        return {"idx": idx[:, :-1].contiguous(), "targets": idx[:, 1:].contiguous(), "ids": got.top_ids,
+                "logprobs": got.top_logprobs}
+
+    def forward(b):
+        kd = student.distillation_loss(b["idx"], b["ids"], b["logprobs"], tail=True)
+        lp = student(b["idx"], method="token_logprobs", tokens=b["targets"])
+        loss = 0.5 * kd - 0.1 * lp.logprobs.mean() - 0.01 * lp.entropy.mean()
+        return {"loss": loss}, loss, loss / 4 * 64
+
+    def eager(b):
+        student.zero_grad(set_to_none=True)
+        with torch.autocast("cuda", dtype=torch.bfloat16), step.on_side_stream():
+            _, loss, scaled = forward(b)
+            scaled.backward()
+        return loss.item(), {n: q.grad.detach().clone() for n, q in named}
+
+    def rel(a, b):
+        return float((a - b).norm() / (b.norm() + 1e-12))
+
+    eager(batch())
+    step.note_eager()
+    for i in range(4):
+        b = batch()
+        want_loss, want = eager(b)
+        _, again = eager(b)
+        student.zero_grad(set_to_none=True)
+        with torch.autocast("cuda", dtype=torch.bfloat16), step.on_side_stream():
+            _, loss = step.run(b, forward)
+        assert abs(loss.item() - want_loss) <= 2e-3 * max(1.0, abs(want_loss))
+        for n, q in named:
+            a, w, r = q.grad.detach(), want[n], again[n]
+            if n.endswith("attn.c_attn.bias"):  # the key third's exact gradient is zero
+                third = len(a) // 3
+                a, w, r = (torch.cat([x[:third], x[2 * third:]]) for x in (a, w, r))
+            assert rel(a, w) < max(2e-2, 4 * rel(r, w)), (i, n)
+        with torch.no_grad():
+            for _, q in named:
+                q.mul_(0.99).add_(torch.randn_like(q), alpha=1e-3)
+    assert step.graph is not None and not step.disabled
