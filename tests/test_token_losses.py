@@ -575,6 +575,30 @@ def test_in_place_gradients(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("rows,vocab", [(37, 1003), (20, 20001), (400, 20001)])
+def test_loss_and_gradient_in_place(dtype, tail, rows, vocab):
+    """Short rows, two kernels, and staged rows: over the logits, or over other columns of their buffer; what lies around
+    stays as it was."""
+
+    ld = vocab + 11
+    buf = torch.full((rows + 1, 2 * ld), 7.0, device=DEV, dtype=dtype)
+    buf[:rows, 3:3 + vocab] = _logits(rows, vocab, dtype, "contiguous")
+    ids, t = _teacher(rows, vocab, 9, tail)
+    weight = torch.rand(rows, device=DEV) + 0.5
+    weight[::4] = 0
+    apart = kf.topk_distillation_grad(buf[:rows, 3:3 + vocab], ids, t, weight=weight, tail=tail)
+    for first in (3, 3 + ld):
+        b = buf.clone()
+        got = kf.topk_distillation_grad(b[:rows, 3:3 + vocab], ids, t, weight=weight, tail=tail,
+                                        out=b[:rows, first:first + vocab])
+        assert all(torch.equal(x, y) for x, y in zip(got, apart))
+        b[:rows, first:first + vocab] = buf[:rows, first:first + vocab]
+        assert torch.equal(b, buf)
+
+
+@gpu
 def test_outputs_that_overlap_are_refused():
     buf = _logits(6, 64, torch.float32, "contiguous")
     z = buf[:, :20]
