@@ -288,7 +288,7 @@ struct WarpStats {
 
 __device__ __forceinline__ WarpStats warp_apart(const Run<true>& run, float c) {
   const float2 ss = split(run.s), aa = split(run.a);
-  const float off = run.plain ? fmaf(run.m, c, -run.r) : 0.f, f = ex2(-off);  // of every x
+  const float off = run.offset(c), f = ex2(-off);
   const float s = (ss.x + ss.y) * f, a = (aa.x + aa.y) * f - off * s;
   WarpStats w;
   w.others.m = run.m;

@@ -272,15 +272,14 @@ struct Run {
     raise(z, c);
     add_any<false>(z, c);
   }
-  // The warp's statistics to its reference's m, in every lane.
+  // What every x is too large by, to the reference's m.
+  __device__ __forceinline__ float offset(float c) const { return plain ? fmaf(m, c, -r) : 0.f; }
+  // The warp's maximum and sum to its reference's m, in every lane.
   __device__ __forceinline__ Acc total(float c) const {
     Acc t;
-    const float2 ss = split(s), aa = split(a);
-    const float off = plain ? fmaf(m, c, -r) : 0.f;  // of every x
-    const float f = ex2(-off);
+    const float2 ss = split(s);
     t.m = m;
-    t.s = warp_sum(ss.x + ss.y) * f;
-    t.a = ENT ? warp_sum(aa.x + aa.y) * f - off * t.s : 0.f;
+    t.s = warp_sum(ss.x + ss.y) * ex2(-offset(c));
     return t;
   }
 };
@@ -502,14 +501,14 @@ __device__ __forceinline__ Acc join_lanes(Acc v, float c) {
   return r;
 }
 
-// Joins the statistics of a block's warps; the first warp returns with them.
-template <int NT, bool ENT>
-__device__ __forceinline__ Acc block_join(const Run<ENT>& run, float c, Acc* sm) {
+// Joins the maxima and sums of a block's warps; the first warp returns with them.
+template <int NT>
+__device__ __forceinline__ Acc block_join(const Run<false>& run, float c, Acc* sm) {
   const Acc w = run.total(c);
   if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = w;
   __syncthreads();
   Acc r;
-  if (threadIdx.x < 32) r = join_lanes<NT / 32, ENT>(sm[threadIdx.x & (NT / 32 - 1)], c);
+  if (threadIdx.x < 32) r = join_lanes<NT / 32, false>(sm[threadIdx.x & (NT / 32 - 1)], c);
   return r;
 }
 

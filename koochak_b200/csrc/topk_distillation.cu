@@ -9,7 +9,8 @@ namespace kb {
 namespace {
 
 constexpr int kGradThreads = 512;  // streaming threads of the kernel that writes loss and gradient
-constexpr int kChunks = 8;  // bulk copies a block stages its units with, at most
+constexpr int kStageBytes = 107 * 1024;  // of staged units and marks, for two blocks on an SM
+constexpr int kChunks = (kStageBytes / 16 + kBatch * kGradThreads - 1) / (kBatch * kGradThreads);  // bulk copies of a row
 constexpr int kStats = kTopkDistillationStats;  // KdStats, and 0 for a row without slots
 
 // --------------------------------------------------------- distillation
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(NT)
   const FromMemory src{row.unit_ptr()};
   if constexpr (TAIL) stream_units<T, NT, false>(src, u0, u1, c, run, marks, [](int, float) {});
   else stream_units<T, NT, false>(src, u0, u1, c, run, NoMarks{}, [](int, float) {});
-  Acc all = block_join<NT, false>(run, c, join_sm);
+  Acc all = block_join<NT>(run, c, join_sm);
   if constexpr (SPLIT) {
     if (tid == 0) {
       result = all;
@@ -623,7 +624,7 @@ void topk_distillation_forward(const at::Tensor& logits, const at::Tensor& ids, 
   const int stage_units = (int)((units + 7) / 8 * 8);
   const int64_t staged = 16 * (int64_t)stage_units + 4 * Marks<__half, kGradThreads>::size(stage_units);
   const bool twice = out && row_bytes <= 32 * 1024;
-  const bool together = out && !twice && staged <= 107 * 1024 && rows >= num_sms(device);
+  const bool together = out && !twice && staged <= kStageBytes && rows >= num_sms(device);
   if (out && !twice && !together) {
     KB_CHECK(stats.has_value(), "the gradient needs stats");
     topk_distillation_forward(logits, ids, teacher, weight, loss, stats, c10::nullopt, vocab, temperature, tail);
