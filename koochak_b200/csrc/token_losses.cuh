@@ -664,9 +664,13 @@ void check_out(const at::Tensor& out, const at::Tensor& logits, int64_t vocab) {
 // 50257 bf16: 8.0 us with 512 threads, 8.4 with 256, 11.0 with 128; rows of 16 KB: 3.7 with 256, 3.9 with 512), and
 // clusters while each block keeps at least 16 KB and has an SM of its own, or at least 64 KB and a third of one (one row
 // of 50257 bf16: 5.1 us with four blocks, 5.8 with one; 40 rows of 131072 fp32: 6.8 with eight, 12.3 with one; but 257
-// rows of 50257 bf16: 9.7 with two, 8.0 with one). A `light` kernel, of which an SM holds three blocks of 512 threads,
-// takes them for up to 1024 long rows (distillation, 1024 rows of 131072 fp32: 89 us, 100 with 256; log probabilities,
-// of which an SM holds two: 90 with 256, 89 with 512, but 65 against 55 on 700 rows).
+// rows of 50257 bf16: 9.7 with two, 8.0 with one). A `light` kernel, of which an SM holds three blocks of 512 threads or
+// five of 256, takes long rows by waves: 512 threads up to three rows per SM, which all run at once then, 256 up to five
+// and a little more, 512 up to nine, where three whole waves beat one and a part of a second (distillation, rows of
+// 131072 fp32, 512 against 256 threads in us: 400 rows 36 and 42, 700 62 and 58, 850 71 and 69, 1024 91 and 102, 1200 99
+// and 108, 1500 124 and 120, 2048 161 and 168, 4096 314 and 305; of 50257 fp32: 400 15 and 18, 700 27 and 23, 850 31 and
+// 28, 1024 39 and 42, 1200 43 and 44, 1500 54 and 48). Log probabilities, of which an SM holds two blocks of 512 threads,
+// take 256 (rows of 131072 fp32: 1024 rows 89 and 90 us, 700 65 and 55).
 struct RowLaunch {
   int threads, parts;
 };
@@ -681,7 +685,7 @@ RowLaunch row_launch(int64_t rows, int64_t row_bytes, bool light, int device) {
   if (how.parts > 1) how.threads = 256;
   else if (row_bytes <= 32768) how.threads = rows < 400 && row_bytes >= 8192 ? 256 : 128;
   else if (rows <= 2 * sms) how.threads = 512;
-  else if (row_bytes > 131072 && light && rows <= 1024) how.threads = 512;
+  else if (row_bytes > 131072 && light && (rows <= 3 * sms || (rows > 6 * sms && rows <= 9 * sms))) how.threads = 512;
   else if (rows < 1000 || row_bytes > 131072) how.threads = 256;
   return how;
 }
