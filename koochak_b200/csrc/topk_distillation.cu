@@ -282,12 +282,12 @@ struct FromStage {
   static constexpr bool kPatch = true;  // marked elements are put to -inf where they are
   uint4* stage;
   uint64_t* full;
-  uint32_t parity;
+  uint32_t phases;  // a chunk's parity each
   volatile int* abort_flag;
   int* status;
   // Waits for the batch's chunk to be there; a copy that does not arrive is recorded, and the host raises on it.
   __device__ __forceinline__ void begin(int batch) const {
-    mbar_wait(&full[batch], parity, abort_flag, status, kStatusTimeoutRowStage);
+    mbar_wait(&full[batch], (phases >> batch) & 1u, abort_flag, status, kStatusTimeoutRowStage);
   }
   __device__ __forceinline__ uint4 load(int u) const { return stage[u]; }
   template <typename T>
@@ -351,13 +351,15 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     return mbar_wait(bar, parity & 1u, &sh.abort_flag, status, kStatusTimeoutRowStage);
   };
-  // Rows so far, and rows with slots: `full` and `empty` complete once per row with slots, `told` once per other row (one
-  // barrier for even rows and one for odd ones), the other barriers once per row. Each may complete only after everyone
-  // who waits on it has seen it complete before: joined and solved(n + 1) follow done(n), which needs every streaming warp
-  // to have seen solved(n); ready(n + 1) follows joined(n); told(n + 2) follows done(n), which the fetching warp
-  // arrives on once it has seen told(n + 1). told(n + 1) follows nothing that the fetching warp does in row n, so on one
-  // barrier it could complete twice before that warp looks.
-  uint32_t count = 0, staged = 0;
+  // Rows so far, and for each chunk the parity of the rows that had units in it. Rows at other boundaries may end just
+  // before the last chunk; they leave it alone, since no one would see it filled before it is given up. `told` completes
+  // once per other row (one barrier for even rows and one for odd ones), the other barriers once per row. Each may
+  // complete only after everyone who waits on it has seen it complete before: joined and solved(n + 1) follow done(n),
+  // which needs every streaming warp to have seen solved(n); ready(n + 1) follows joined(n); told(n + 2) follows done(n),
+  // which the fetching warp arrives on once it has seen told(n + 1). told(n + 1) follows nothing that the fetching warp
+  // does in row n, so on one barrier it could complete twice before that warp looks.
+  uint32_t count = 0, phases = 0;
+  auto chunks_of = [&](const Row<T>& row) { return (row.units + kChunk - 1) / kChunk; };
 
   if (tid < NT) {
     for (long long r = blockIdx.x; r < rows; r += gridDim.x, ++count) {
@@ -376,7 +378,7 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
         continue;
       }
       Run<false> run;
-      const FromStage src{stage, sh.full, staged & 1u, &sh.abort_flag, status};
+      const FromStage src{stage, sh.full, phases, &sh.abort_flag, status};
       const Marks<T, NT> marks(words, 0, row.units);
       if (tid < 32) run.add_one(TAIL && tid < row.ragged && marks.ragged(tid) ? -INFINITY : rag, c);
       if constexpr (TAIL) stream_units<T, NT, false>(src, 0, row.units, c, run, marks, [](int, float) {});
@@ -394,10 +396,8 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
         return mul2(pair(ex2(x.x), ex2(x.y)), dd);
       };
       const bool same = same_boundaries(row.z, o);
-      for (int i = 0; i < chunks; ++i) {
-        // Rows at other boundaries may end just before a chunk. No one has waited for it in the first pass then, and it
-        // may not be given up before the fetching warp has come to it.
-        if (i * kChunk >= row.units) wait(&sh.full[i], staged);
+      const int used = chunks_of(row);
+      for (int i = 0; i < used; ++i) {
         map_batch<T, NT, true, false>(row, src, o, same, i * kChunk + tid, row.units, gradient, [&] {
           // The chunk's place is written by a bulk copy next, through another proxy: without the fence that copy could
           // overtake these loads (it did, for some hundred of 10^9 elements), and what was put to -inf.
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
       if (tid < row.ragged) Elem<T>::store(o + row.ragged_index(tid), split(gradient(pair(rag, 0.f), 0)).x);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.done);
-      ++staged;
+      phases ^= (1u << used) - 1u;
     }
     return;
   }
@@ -417,8 +417,8 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
   if (tid < NT + 32) {
     // The fetching warp: told(n) says whether row n of this block has slots, or is behind
     // the last.
-    int filled = chunks;  // chunks of the row under way whose copies are issued
-    for (long long r = blockIdx.x; filled == chunks; r += gridDim.x, ++count) {
+    bool open = true;
+    for (long long r = blockIdx.x; open; r += gridDim.x, ++count) {
       if (!__all_sync(0xffffffffu, wait(&sh.told[count & 1], count >> 1))) break;
       const bool some = sh.fetch[count & 1];
       __syncwarp();
@@ -426,28 +426,24 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
       if (r >= rows) return;
       if (!some) continue;
       const Row<T> row(logits + r * ld, V);
-      for (filled = 0; filled < chunks; ++filled) {
-        const int i = filled;
-        if (staged > 0 && !__all_sync(0xffffffffu, wait(&sh.empty[i], staged - 1))) break;
+      const int used = chunks_of(row);
+      for (int i = 0; i < used; ++i) {
+        // Of the row before; a new barrier lets the first one pass.
+        open = __all_sync(0xffffffffu, wait(&sh.empty[i], ~(phases >> i)));
+        if (!open) break;
         if (lane == 0) {
-          const int n = min(kChunk, row.units - i * kChunk);
-          if (n > 0) {
-            mbar_arrive_expect_tx(&sh.full[i], (uint32_t)n * 16);
-            bulk_load_1d(stage + i * kChunk, row.unit_ptr() + i * kChunk, (uint32_t)n * 16, &sh.full[i]);
-          } else {
-            mbar_arrive(&sh.full[i]);
-          }
+          const uint32_t bytes = 16u * (uint32_t)min(kChunk, row.units - i * kChunk);
+          mbar_arrive_expect_tx(&sh.full[i], bytes);
+          bulk_load_1d(stage + i * kChunk, row.unit_ptr() + i * kChunk, bytes, &sh.full[i]);
         }
+        phases ^= 1u << i;
         __syncwarp();
       }
-      if (filled == chunks) ++staged;
     }
     // A wait ran out: no more is fetched, and what is on its way to this block's memory is waited for (with a limit).
     volatile int never = 0;
-    for (int i = 0; i < chunks; ++i) {
-      const uint32_t copies = staged + (filled < chunks && i < filled ? 1 : 0);
-      if (copies > 0 && !mbar_wait(&sh.full[i], (copies - 1) & 1u, &never, status, kStatusTimeoutDrain)) break;
-    }
+    for (int i = 0; i < chunks; ++i)
+      if (!mbar_wait(&sh.full[i], ~(phases >> i) & 1u, &never, status, kStatusTimeoutDrain)) break;
     return;
   }
 
@@ -554,7 +550,6 @@ __global__ void __launch_bounds__(NT + 64, 1024 / NT)
     if (some) {
       __syncwarp();
       write_listed<T>(row, out + r * ld_out, 0, row.units, true, K, c, w_now * inv_t, k, now, lane, 32);
-      ++staged;
     } else {
       if (stats && lane < kStats) stats[r * kStats + lane] = 0.f;
       if (lane == 0) loss[r] = 0.f;
