@@ -304,8 +304,8 @@ struct FromStage {
 // lists: the next row's list is read, marked and summed during this row's second pass, and the listed elements are
 // written after the dense gradient. Two blocks share an SM, so that one stores and fetches while the other is between
 // its passes.
-// 16384 x 50257 bf16 with 64 slots: 620 us with the rest, 582 without, 0.82 and 0.87 of the copy rate; issue slots and
-// 2^x are busy 62 % of the time each. Reading the row twice through L2 instead took 849 us, more than two kernels
+// 16384 x 50257 bf16 with 64 slots: 625 us with the rest, 596 without, 0.81 and 0.85 of the copy rate (up to 8 % more on
+// some devices); issue slots and 2^x are busy 62 % of the time each. Reading the row twice through L2 instead took 849 us, more than two kernels
 // (815 us): too many rows are in flight for L2 to hold them.
 constexpr int kOwn = kMaxList / 32;  // slots per lane of the serving warp
 
