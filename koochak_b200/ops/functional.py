@@ -446,7 +446,8 @@ def topk_distillation_ref(logits, teacher_ids, teacher_logits, *, temperature: f
     some = valid.any(-1)
     if not some.all():  # rows without slots have gradient zero, whatever they hold
         zf = torch.where(some[:, None], zf, 0.0)
-    logp = torch.log_softmax(zf / temperature, dim=-1)
+    x = zf / temperature
+    logp = torch.log_softmax(x, dim=-1)
     at = torch.where(valid, teacher_ids, 0)
     t = torch.where(valid, teacher_logits.to(zf.dtype), -math.inf)
     if tail:
@@ -462,9 +463,13 @@ def topk_distillation_ref(logits, teacher_ids, teacher_logits, *, temperature: f
     if tail:
         listed = torch.zeros_like(logp.detach()).scatter_add_(1, at, valid.to(logp.dtype)) > 0
         rest = (1.0 - q.sum(-1)).clamp_min(0.0)
-        off = logp.masked_fill(listed, -math.inf)
-        none = off.detach().amax(-1) == -math.inf  # no student mass off the list: an infinite constant
-        log_rest = torch.where(none, -math.inf, torch.logsumexp(off.masked_fill(none[:, None], 0.0), -1))
+        # From the largest logit off the list, whose distance from the row's may have no digits below one.
+        top = x.detach().amax(-1, keepdim=True)
+        high = x.detach().masked_fill(listed, -math.inf).amax(-1, keepdim=True)
+        none = high == -math.inf  # no student mass off the list: an infinite constant
+        off = (x - torch.where(none, 0.0, high)).masked_fill(listed, -math.inf).masked_fill(none, 0.0)
+        log_rest = torch.logsumexp(off, -1) + (high - top)[:, 0] - torch.logsumexp(x - top, -1)
+        log_rest = torch.where(none[:, 0], -math.inf, log_rest)
         # What rounding leaves of a teacher that lists everything, where the student has no mass for it.
         rest = torch.where((rest <= 2.0**-18) & (log_rest.detach() < -126 * math.log(2.0)), 0.0, rest)
         loss = loss + torch.where(rest == 0, 0.0, rest * (rest.log() - log_rest).masked_fill(rest == 0, 0.0))

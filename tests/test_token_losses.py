@@ -183,6 +183,27 @@ def test_reference_distillation_and_gradient_by_differences(tail):
     assert torch.allclose(g[0], dz / temperature)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("far", [1e3, 1e8, 1e30])
+def test_reference_rest_far_below_the_list(dtype, far):
+    """The gradient off the list is the rest's share, softmax over the tokens off the list, however far they are. The
+    listed token has all of the student's mass, so its own gradient is the rest's probability."""
+
+    gen = torch.Generator().manual_seed(9)
+    z = torch.randn(2, 50, generator=gen, dtype=dtype)
+    z[:, 7] = far
+    z.requires_grad_()
+    t = torch.tensor([[0.75]] * 2, dtype=dtype).log()
+    loss = kf.topk_distillation_ref(z, torch.tensor([[7]] * 2), t, temperature=2.0, tail=True)
+    (dz,) = torch.autograd.grad(loss.sum(), z)
+    share = torch.softmax(torch.cat([z[:, :7], z[:, 8:]], 1).detach().double() / 2.0, 1)
+    want = -0.25 * torch.cat([share[:, :7], torch.full((2, 1), -1.0), share[:, 7:]], 1) / 2.0
+    # a few roundings of a share, a product and a quotient
+    assert ((dz.double() - want).abs() <= want.abs() * 32 * torch.finfo(dtype).eps).all()
+    size = 0.25 * far / 2.0
+    assert ((loss.double() - size).abs() <= size * 4 * torch.finfo(dtype).eps + 3.0).all()
+
+
 def test_reference_masks():
     z = torch.randn(4, 6, dtype=torch.float64)
     z[0, 1:4] = -math.inf
