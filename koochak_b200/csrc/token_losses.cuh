@@ -224,8 +224,9 @@ __device__ __forceinline__ float warp_sum(float v) {
 // reference r that all lanes share, so that they need no rescaling when they are
 // joined; each lane holds its sums as two halves. With m the largest element when
 // the reference was last taken, r is m c rounded, which makes x one exact
-// product and one rounding; total() makes up for the rounding of r. Where
-// m c would overflow (or m is infinite or NaN), x = (z - m) c instead.
+// product and one rounding; total() makes up for the rounding of r, which is
+// at most 1/2 below 2^24. Where m c is larger (a mask like -1e30, or infinite
+// or NaN), r could be off by more than 2^x can hold, and x = (z - m) c instead.
 template <bool ENT>
 struct Run {
   float m = -INFINITY, r = 0.f;
@@ -235,8 +236,9 @@ struct Run {
   __device__ __forceinline__ void raise(float wide, float c) {
     if (!__any_sync(0xffffffffu, !(wide <= m))) return;
     const float mn = max_nan(m, warp_max_nan(wide)), rn = mn * c;
-    const bool pn = fabsf(rn) < 1e37f;
-    const float x = plain && pn ? r - rn : (m - mn) * c;
+    const bool pn = fabsf(rn) < 16777216.f;
+    // From the old reference, r or m c, to the new one.
+    const float x = plain ? (pn ? r - rn : fmaf(-mn, c, r)) : pn ? fmaf(m, c, -rn) : (m - mn) * c;
     const float f = (m == mn) ? 1.f : ex2(x);
     const F2 ff = pair(f, f);
     if (ENT) {

@@ -527,6 +527,63 @@ def test_hard_rows(dtype, vocab, top_k):
     _check_logprobs(z, _tokens(len(z), vocab, ignored=False), top_k=top_k)
 
 
+def _far_rows(vocab, dtype):
+    """Logits, or masks other than the type's lowest value, so large that a product with 1 / T has no digits below one."""
+
+    big = [v for v in (3e4, 1e7, 2e7, 1e9, 1e10, 1e15, 1e30, 1e37, 3e38) if v < torch.finfo(dtype).max]
+    r = torch.randn(vocab, generator=torch.Generator().manual_seed(4))
+    at = torch.arange(vocab)
+    rows = []
+    for v in big:
+        rows += [torch.full((vocab,), v), torch.full((vocab,), -v),   # one value throughout
+                 torch.where(at < vocab // 2, -v, r),                 # masked in front, behind, and here and there
+                 torch.where(at < vocab // 2, r, -v), torch.where(at % 3 == 0, r, -v),
+                 torch.where(at == vocab // 3, v, r),                 # one far above
+                 (r / 4).clamp(-1, 1) * v, v * (1 + r.clamp(-1, 1) * 2.0**-7).clamp(max=1.0)]
+    return torch.stack(rows).to(dtype).to(DEV)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [70, 3001, 40001])
+@pytest.mark.parametrize("temperature", [1.0, 0.3])
+def test_far_logits_and_masks(dtype, vocab, temperature):
+    z = _far_rows(vocab, dtype)
+    wide = z.double()
+    wide = (wide.amax(1) - wide.amin(1)) / temperature > 3e38  # log probabilities beyond fp32 are infinite
+    for top_k in (0, 9):
+        got = kf.token_logprobs(z[wide], _tokens(int(wide.sum()), vocab, ignored=False), top_k=top_k,
+                                temperature=temperature)
+        want = kf.token_logprobs_ref(z[wide].double(), _tokens(int(wide.sum()), vocab, ignored=False), top_k=top_k,
+                                     temperature=temperature)
+        for a, b in zip(got, (want[0], want[1], want[2], want[3])):
+            if a is not None:
+                _close(a, b.float(), _logprob_tol(b.float().double()) + 2.0**-16, "beyond fp32")
+    z = z[~wide]
+    rows = len(z)
+    for top_k in (0, 9):
+        _check_logprobs(z, _tokens(rows, vocab, ignored=False), top_k=top_k, temperature=temperature, grads=top_k == 0)
+    ids, t = _teacher(rows, vocab, 8, False, ragged=False)
+    ids[:, 0] = z.float().argmax(1)
+    q = torch.log_softmax(torch.randn(rows, 9, generator=torch.Generator().manual_seed(6)), -1)[:, :8].to(DEV)
+    # Losses one by one: of all rows together only the largest, 1e30, would be looked at. As in _check_distill, with
+    # |log p| up to the loss's own size over the least q (2^-6 or more of these), and 24 where that is less.
+    for tail, teacher in ((False, t), (True, q)):
+        want = kf.topk_distillation_ref(z.double(), ids, teacher, temperature=temperature, tail=tail)
+        got = kf.topk_distillation(z, ids, teacher, temperature=temperature, tail=tail)
+        _close(got, want.float(), 2.0**-14 * want.abs().cpu().clamp(max=3e38) + 40 * 2.0**-20, "loss")
+        for n in (1, 200 // rows + 1):  # clusters and staged rows
+            many, ids_n, t_n = (x.repeat(n, 1) for x in (z, ids, teacher))
+            loss, stats, dz = kf.topk_distillation_grad(many, ids_n, t_n, temperature=temperature, tail=tail)
+            _close(loss, want.float().repeat(n), (2.0**-14 * want.abs().cpu().clamp(max=3e38) + 40 * 2.0**-20).repeat(n), "loss")
+            zr = z.double().requires_grad_()
+            finite = want.isfinite() | tail
+            dwant = torch.autograd.grad(kf.topk_distillation_ref(zr, ids, teacher, temperature=temperature, tail=tail)
+                                        .nan_to_num(posinf=0.0).sum(), zr)[0][finite].repeat(n, 1)
+            tol = 2.0**-16 / temperature + dwant.abs().cpu() * _half_step(dtype) * 1.01
+            _close(dz[finite.repeat(n)], dwant, tol, "dlogits")
+
+
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_without_distribution(dtype):
