@@ -222,7 +222,8 @@ class _HeadLossFn(torch.autograd.Function):
 
 class GPT2(TokenLosses, nn.Module):
     """GPT-2 language model. ``forward(idx, targets)`` returns the mean loss;
-    ``forward(idx)`` returns logits (reference path only materialises them)."""
+    ``forward(idx)`` returns logits (reference path only materialises them);
+    ``forward(idx, method=name, ...)`` is one of the ``TokenLosses`` methods."""
 
     def __init__(self, cfg: Optional[GPT2Config] = None, **overrides) -> None:
         super().__init__()

@@ -266,7 +266,8 @@ class _Model(nn.Module):
 
 
 class Llama(TokenLosses, nn.Module):
-    """``forward(idx, targets)`` returns the mean loss; ``forward(idx)`` returns logits (reference path)."""
+    """``forward(idx, targets)`` returns the mean loss; ``forward(idx)`` returns logits (reference path);
+    ``forward(idx, method=name, ...)`` is one of the ``TokenLosses`` methods."""
 
     def __init__(self, cfg: Optional[LlamaConfig] = None, **overrides) -> None:
         super().__init__()
