@@ -1050,6 +1050,46 @@ def test_vocabularies_one_after_another(dtype, tail, vocabs):
 
 
 @gpu
+def test_two_host_threads():
+    """Two vocabularies in two threads with a stream each, every call setting up the kernels anew for its sizes."""
+
+    import threading
+
+    work = []
+    for vocab, tail in ((50257, True), (20001, True), (33001, False), (270000, True)):
+        rows = 200 if vocab < 100000 else 400
+        z = _logits(20, vocab, torch.bfloat16, "padded").repeat(rows // 20, 1)
+        ids, t = (x.repeat(rows // 20, 1) for x in _teacher(20, vocab, 11, tail))
+        work.append((z, ids, t, tail))
+
+    def call(z, ids, t, tail):
+        x = z.detach().requires_grad_()
+        loss = kf.topk_distillation(x, ids, t, tail=tail, reduction="sum")
+        return loss.detach(), torch.autograd.grad(loss, x)[0], *kf.token_logprobs(z, ids[:, 0].contiguous(), top_k=7)
+
+    want = [call(*w) for w in work]
+    torch.cuda.synchronize()
+    errors = []
+
+    def run(first):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(24):
+                    n = (first + i) % len(work)
+                    got = call(*work[n])
+                    assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(got, want[n])), n
+        except BaseException as e:  # noqa: BLE001 (raised again below)
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in (0, 1, 3)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors, errors[0]
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_wide_vocabularies_one_after_another(dtype):
     """The same for the loss alone, whose marks take 64 KB of shared memory at the widest vocabulary."""
